@@ -1,0 +1,486 @@
+// Attention of a few rows per sequence (one token, or the nodes of a drafted tree) over a cached context, on the warp-level tensor
+// cores (mma.sync m16n8k16, f16 x f16 -> f32).
+//
+//   o_r = sum_t softmax_t(q_r k_t / sqrt(128)) v_t     over the rows t that r sees
+//
+// A query row r is a node and one of the query heads that share the kv head (r = node * group + head).  The products are formed
+// transposed, with the cache as the 16-row operand and eight query rows as the columns, so that few rows waste little:
+//   S^T [16 positions x 8 rows] = K Q^T,   O^T [16 dimensions x 8 rows] = V^T P^T
+// A warp takes 16 positions at a time for all 8 * NT rows of its block; its softmax state and the unnormalised O^T stay in registers.
+// P goes from the accumulator layout to the operand layout by movmatrix.  e4m3 codes become f16 exactly (no rounding); the key scale
+// multiplies the score, the value scale the probability, there relative to the largest one met so far (a power of two), which keeps
+// the f16 operand in range whatever the values' size.
+// fp32 activations: Q and P are split in an f16 high part and an f16 remainder (22 significant bits) and multiplied twice; bfloat16
+// activations: once, which rounds P to 11 bits where the result keeps 8.  Each query row is brought to a maximum of 1 to 2 by a power
+// of two first.
+// The running maximum moves only when a score exceeds the reference by more than 2^14 / 2^6: otherwise no lane needs another's score.
+#pragma once
+#include <float.h>
+
+#include "attention_mma.cuh"
+#include "common.cuh"
+#include "kv_cache.cuh"
+#include "lm_device.cuh"
+
+namespace bw {
+namespace tree {
+
+using kv::kHd;
+constexpr int kMaxNodes = 64;
+constexpr int kWarps = 4;
+constexpr int kTile = 16;               // positions a warp takes at once
+constexpr int kPart = kHd + 4;          // floats of a partial record: outputs, maximum, sum, padding
+constexpr float kHead = 6.f, kSlack = 14.f;   // P up to 2^6 when the maximum is new, 2^14 before it is moved
+
+struct Args {
+    void* out;                          // [M * T][nq * 128]
+    const void* q;                      // the same
+    kv::View c;
+    const int *first, *count;
+    const unsigned long long* mask;     // [M * T] or NULL: node j <= i
+    int nq, M, T, group, rows, tiles;   // rows = T * group query rows per kv head, in `tiles` blocks of 8 * NT
+    int nsplit;
+    float* part;                        // [M][heads][rows][nsplit][kPart] where nsplit > 1
+};
+
+template <int NT, bool kCoded>
+struct Shape {
+    static constexpr int kRows = 8 * NT;
+    static constexpr int kStages = kCoded ? 4 : 3;
+    static constexpr int kSide = kTile * kHd * (kCoded ? 1 : 2);           // bytes of 16 K or V rows
+    static constexpr int kStage = 2 * kSide + (kCoded ? 2 * kTile * 4 : 0); // and their scales
+    static constexpr int kWarp = kStages * kStage;
+    static constexpr int kO = kRows * kHd * 4;                             // a warp's O, over its stages once they have drained
+    static constexpr int kPerWarp = kWarp > kO ? kWarp : kO;
+    static constexpr int kSmem = kWarps * kPerWarp;
+};
+
+// f16 pair of two e4m3 codes (exact).
+__device__ __forceinline__ uint32_t codes_f16x2(uint32_t two) {
+    uint32_t r;
+    asm("{\n\t.reg .b16 c;\n\tcvt.u16.u32 c, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, c;\n\t}" : "=r"(r) : "r"(two));
+    return r;
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float2 load_q2(const float* p) { return *reinterpret_cast<const float2*>(p); }
+__device__ __forceinline__ float2 load_q2(const __nv_bfloat16* p) {
+    const uint32_t u = *reinterpret_cast<const uint32_t*>(p);
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
+}
+__device__ __forceinline__ void store_o4(float* p, const float4& v) { *reinterpret_cast<float4*>(p) = v; }
+__device__ __forceinline__ void store_o4(__nv_bfloat16* p, const float4& v) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(lm::pack_bf16(v.x, v.y), lm::pack_bf16(v.z, v.w));
+}
+// Power of two at or below |x| (1 for zero and what has no such), and its reciprocal.
+__device__ __forceinline__ float2 binade(float x) {
+    uint32_t e = __float_as_uint(x) >> 23 & 255;
+    e = e < 1 ? 127 : min(max(e, 2u), 252u);
+    return make_float2(__uint_as_float(e << 23), __uint_as_float((254 - e) << 23));
+}
+
+// What a sequence's rows see: positions [0, ctx) all of them, node j (position ctx + j, j < nodes) by its mask bit.
+struct Seen {
+    int ctx, end;                       // end: positions in all
+    unsigned long long any;             // nodes that some row of the sequence sees
+};
+__device__ __forceinline__ unsigned long long low_bits(int n) { return n >= 64 ? ~0ull : (1ull << n) - 1; }
+__device__ __forceinline__ int node_count(const Args& a, int m) { return a.count ? max(0, min(a.count[m], a.T)) : a.T; }
+__device__ __forceinline__ unsigned long long mask_of(const Args& a, int m, int node, int nodes) {
+    return (a.mask ? a.mask[(size_t)m * a.T + node] : low_bits(node + 1)) & low_bits(nodes);
+}
+
+template <int NT, bool kCoded, typename A>
+__global__ void __launch_bounds__(kWarps * 32) attend_kernel(const Args a) {
+    using Sh = Shape<NT, kCoded>;
+    constexpr bool kSplit = sizeof(A) == 4;             // fp32 activations: two products
+    extern __shared__ __align__(128) unsigned char dsm[];
+    __shared__ unsigned long long s_mask[Sh::kRows], s_any;
+    __shared__ float s_m[kWarps][Sh::kRows], s_l[kWarps][Sh::kRows];
+    __shared__ uint4 s_q[NT > 2 ? 8 * NT * 32 : 1];     // query operand where it does not fit in registers
+    const int t = threadIdx.x, warp = t >> 5, lane = t & 31, g = lane >> 2, tq = lane & 3;
+    const int split = blockIdx.x, head = blockIdx.y / a.tiles, r0 = (blockIdx.y - head * a.tiles) * Sh::kRows, m = blockIdx.z;
+    pdl_trigger();
+    pdl_wait();
+    const int first = a.first[m], nodes = node_count(a, m);
+    if (first < 0 || r0 >= nodes * a.group) return;
+    // masks: this block's rows, and of all nodes
+    if (t == 0) s_any = 0;
+    __syncthreads();
+    if (t < nodes) atomicOr(&s_any, mask_of(a, m, t, nodes));
+    for (int r = t; r < Sh::kRows; r += kWarps * 32) s_mask[r] = (r0 + r) < nodes * a.group ? mask_of(a, m, (r0 + r) / a.group, nodes) : 0;
+    __syncthreads();
+    Seen see;
+    see.ctx = min(first, a.c.max_seq);
+    see.end = (int)min((long)first + nodes, (long)a.c.max_seq);
+    see.any = s_any;
+    const int ntile = (see.end + kTile - 1) / kTile;
+    const int tile0 = (int)((long)ntile * split / a.nsplit), tile1 = (int)((long)ntile * (split + 1) / a.nsplit);
+
+    const size_t row0 = a.c.row(m, head, 0);
+    constexpr int kRowBytes = kCoded ? kHd : 2 * kHd, kChunks = kRowBytes / 16;
+    const unsigned char *Kb = a.c.k + row0 * kRowBytes, *Vb = a.c.v + row0 * kRowBytes;
+    const uint32_t stage0 = smem_u32(dsm + warp * Sh::kPerWarp);
+    // 16 rows of K and V (and their scales) to a stage; rows that nobody sees become zeros, whatever lies there
+    auto issue = [&](int tile, int stage) {
+        const int p0 = tile * kTile;
+        const uint32_t to = stage0 + stage * Sh::kStage;
+        const bool all = p0 + kTile <= see.ctx;
+#pragma unroll
+        for (int i = 0; i < kTile * kChunks / 32; ++i) {
+            const int idx = i * 32 + lane, r = idx / kChunks, c = idx % kChunks, p = p0 + r;
+            const bool there = all || p < see.ctx || (p < see.end && (see.any >> (p - see.ctx) & 1));
+            const size_t from = (size_t)(there ? p : 0) * kRowBytes + c * 16;
+            const uint32_t at = to + r * kRowBytes + ((c ^ (r & 7)) << 4);
+            lm::cp_async16z(at, Kb + from, there);
+            lm::cp_async16z(at + Sh::kSide, Vb + from, there);
+        }
+        if (kCoded) {
+            const int r = lane & 15, p = p0 + r;
+            const bool there = all || p < see.ctx || (p < see.end && (see.any >> (p - see.ctx) & 1));
+            const float* s = (lane < 16 ? a.c.ks : a.c.vs) + row0 + (there ? p : 0);
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + 2 * Sh::kSide + lane * 4), "l"(s), "r"(there ? 4 : 0) : "memory");
+        }
+    };
+    int next = tile0 + warp;
+#pragma unroll
+    for (int i = 0; i < Sh::kStages - 1; ++i) {
+        if (next < tile1) issue(next, i);
+        lm::cp_async_commit();
+        next += kWarps;
+    }
+
+    // The query operand: column n of tile j is row r0 + 8 j + n.  Coded keys: a thread's four dimensions of k-step s are 32 tq + 4 s ...,
+    // as it finds them in 16 bytes of a key row; otherwise 16 s + 2 tq, + 1, + 8, + 9.
+    constexpr int kRegs = NT > 2 ? 1 : NT;
+    uint32_t qh[kRegs][8][2], ql[kSplit ? kRegs : 1][8][2];
+    float qf[NT][2];                                    // factor of the scores of columns 2 tq, 2 tq + 1, base 2
+    {
+        float2 unit[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const int r = r0 + 8 * j + g, node = r / a.group;
+            const bool there = node < nodes;
+            const A* q = static_cast<const A*>(a.q) + (((size_t)m * a.T + (there ? node : 0)) * a.nq + head * a.group + (there ? r - node * a.group : 0)) * kHd;
+            float2 x[8][2];
+            float top = 0.f;
+#pragma unroll
+            for (int s = 0; s < 8; ++s)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    x[s][e] = there ? load_q2(q + (kCoded ? 32 * tq + 4 * s + 2 * e : 16 * s + 2 * tq + 8 * e)) : make_float2(0.f, 0.f);
+                    top = fmaxf(top, fmaxf(fabsf(x[s][e].x), fabsf(x[s][e].y)));
+                }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            unit[j] = binade(top);
+#pragma unroll
+            for (int s = 0; s < 8; ++s) {
+                uint32_t h[2], l[2] = {0, 0};
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    if (kSplit) {
+                        amma::split_hi_lo(x[s][e].x * unit[j].y, x[s][e].y * unit[j].y, h[e], l[e]);
+                    } else {
+                        const __half2 v = __floats2half2_rn(x[s][e].x * unit[j].y, x[s][e].y * unit[j].y);
+                        h[e] = *reinterpret_cast<const uint32_t*>(&v);
+                    }
+                }
+                if (NT > 2) {
+                    if (j % kWarps == warp) s_q[(s * NT + j) * 32 + lane] = make_uint4(h[0], h[1], l[0], l[1]);
+                } else {
+                    qh[NT > 2 ? 0 : j][s][0] = h[0]; qh[NT > 2 ? 0 : j][s][1] = h[1];
+                    if (kSplit) { ql[NT > 2 ? 0 : j][s][0] = l[0]; ql[NT > 2 ? 0 : j][s][1] = l[1]; }
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e)                 // (column 2 tq + e is lane group 2 tq + e's row)
+                qf[j][e] = __shfl_sync(0xffffffffu, unit[j].x, (2 * tq + e) * 4) * (0.08838834764831845f * 1.4426950408889634f);
+        }
+    }
+    if (NT > 2) __syncthreads();
+
+    float o[NT][8][4], mx[NT][2], l[NT][2], vref = __uint_as_float(2u << 23);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        mx[j][0] = mx[j][1] = -FLT_MAX;
+        l[j][0] = l[j][1] = 0.f;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) o[j][d][0] = o[j][d][1] = o[j][d][2] = o[j][d][3] = 0.f;
+    }
+
+    int stage = 0;
+    for (int tile = tile0 + warp; tile < tile1; tile += kWarps) {
+        if (next < tile1) issue(next, stage == 0 ? Sh::kStages - 1 : stage - 1);
+        lm::cp_async_commit();
+        next += kWarps;
+        lm::cp_async_wait<Sh::kStages - 1>();
+        __syncwarp();
+        const uint32_t ks = stage0 + stage * Sh::kStage, vs = ks + Sh::kSide;
+        const float* scales = reinterpret_cast<const float*>(dsm + warp * Sh::kPerWarp + stage * Sh::kStage + 2 * Sh::kSide);
+
+        // ---- S^T: rows g, g + 8 of the tile's positions, columns 2 tq, 2 tq + 1 of each query tile
+        float s[NT][4], s2[kSplit ? NT : 1][4];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+            if (kSplit) s2[j][0] = s2[j][1] = s2[j][2] = s2[j][3] = 0.f;
+        }
+        auto key_step = [&](int st, const uint32_t (&k)[4]) {
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                if (NT > 2) {
+                    const uint4 b = s_q[(st * NT + j) * 32 + lane];
+                    mma_f16(s[j], k, b.x, b.y);
+                    if (kSplit) mma_f16(s2[kSplit ? j : 0], k, b.z, b.w);
+                } else {
+                    mma_f16(s[j], k, qh[NT > 2 ? 0 : j][st][0], qh[NT > 2 ? 0 : j][st][1]);
+                    if (kSplit) mma_f16(s2[kSplit ? j : 0], k, ql[NT > 2 || !kSplit ? 0 : j][st][0], ql[NT > 2 || !kSplit ? 0 : j][st][1]);
+                }
+            }
+        };
+        if (kCoded) {
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {            // 16 bytes: four k-steps
+                uint4 lo, hi;
+                const uint32_t at = ks + g * kHd + (((2 * tq + hf) ^ g) << 4);
+                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(lo.x), "=r"(lo.y), "=r"(lo.z), "=r"(lo.w) : "r"(at));
+                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(hi.x), "=r"(hi.y), "=r"(hi.z), "=r"(hi.w) : "r"(at + 8 * kHd));
+                const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t k[4] = {codes_f16x2(wl[e]), codes_f16x2(wh[e]), codes_f16x2(wl[e] >> 16), codes_f16x2(wh[e] >> 16)};
+                    key_step(4 * hf + e, k);
+                }
+            }
+        } else {
+            const int mi = lane >> 3, rr = lane & 7;
+#pragma unroll
+            for (int st = 0; st < 8; ++st) {
+                uint32_t k[4];
+                amma::ldmatrix_x4(ks + ((mi & 1) * 8 + rr) * 2 * kHd + (((2 * st + (mi >> 1)) ^ rr) << 4), k[0], k[1], k[2], k[3]);
+                key_step(st, k);
+            }
+        }
+        // ---- scores in base 2; masks where the tile reaches the nodes
+        float vsc[2] = {1.f, 1.f};
+        float ksc[2] = {1.f, 1.f};
+        if (kCoded) {
+            ksc[0] = scales[g]; ksc[1] = scales[g + 8];
+            vsc[0] = scales[16 + g]; vsc[1] = scales[16 + g + 8];
+        }
+        bool move = false;
+        const int p0 = tile * kTile;
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float x = s[j][e];
+                if (kSplit) x += s2[kSplit ? j : 0][e];
+                x *= qf[j][e & 1];
+                if (kCoded) x *= ksc[e >> 1];
+                s[j][e] = x;
+            }
+        if (p0 + kTile > see.ctx) {
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int p = p0 + g + 8 * (e >> 1);
+                    const bool yes = p < see.ctx || (p < see.end && (s_mask[8 * j + 2 * tq + (e & 1)] >> (p - see.ctx) & 1));
+                    s[j][e] = yes ? s[j][e] : -INFINITY;
+                }
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) move |= fmaxf(s[j][e], s[j][e + 2]) > mx[j][e] + kSlack;
+        float vtop = vref;
+        if (kCoded) {
+            vtop = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fabsf(vsc[0]), fabsf(vsc[1])))));
+            move |= vtop > vref;
+        }
+        if (__any_sync(0xffffffffu, move)) {
+            float fv = 1.f;
+            if (kCoded && vtop > vref) {                // the next power of two
+                const float to = __uint_as_float(min((__float_as_uint(vtop) + 0x7FFFFFu) & 0x7F800000u, 252u << 23));
+                fv = vref * __uint_as_float((254u << 23) - __float_as_uint(to));
+                vref = to;
+            }
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                float f[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float top = fmaxf(s[j][e], s[j][e + 2]);
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                    const float to = fmaxf(mx[j][e], top - kHead), c = lm::exp2_fast(mx[j][e] - to);
+                    mx[j][e] = to;
+                    l[j][e] *= c;
+                    f[e] = c * fv;
+                }
+#pragma unroll
+                for (int d = 0; d < 8; ++d) {
+                    o[j][d][0] *= f[0]; o[j][d][1] *= f[1];
+                    o[j][d][2] *= f[0]; o[j][d][3] *= f[1];
+                }
+            }
+        }
+        // ---- P^T, and to the operand layout
+        const float vdiv = kCoded ? __uint_as_float((254u << 23) - __float_as_uint(vref)) : 1.f;
+        const float vr[2] = {vsc[0] * vdiv, vsc[1] * vdiv};
+        uint32_t ph[NT][2], pl[kSplit ? NT : 1][2];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            float p[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                p[e] = lm::exp2_fast(s[j][e] - mx[j][e & 1]);
+                l[j][e & 1] += p[e];
+                if (kCoded) p[e] *= vr[e >> 1];
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                if (kSplit) {
+                    uint32_t h, lo;
+                    amma::split_hi_lo(p[2 * e], p[2 * e + 1], h, lo);
+                    ph[j][e] = transpose8x8(h);
+                    pl[kSplit ? j : 0][e] = transpose8x8(lo);
+                } else {
+                    const __half2 h = __floats2half2_rn(p[2 * e], p[2 * e + 1]);
+                    ph[j][e] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h));
+                }
+            }
+        }
+        // ---- O^T += V^T P^T.  Coded values: rows g / g + 8 of dimension tile d are dimensions 16 g + 2 d / + 1, 16 bytes of a value row.
+        auto value_step = [&](int d, const uint32_t (&v)[4]) {
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                mma_f16(o[j][d], v, ph[j][0], ph[j][1]);
+                if (kSplit) mma_f16(o[j][d], v, pl[kSplit ? j : 0][0], pl[kSplit ? j : 0][1]);
+            }
+        };
+        if (kCoded) {
+            uint4 w[4];                                 // positions 2 tq, + 1, + 8, + 9
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = 2 * tq + (i & 1) + 8 * (i >> 1);
+                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[i].x), "=r"(w[i].y), "=r"(w[i].z), "=r"(w[i].w)
+                             : "r"(vs + r * kHd + ((g ^ (r & 7)) << 4)));
+            }
+#pragma unroll
+            for (int d = 0; d < 8; d += 2) {
+                const uint32_t x[4] = {d < 2 ? w[0].x : d < 4 ? w[0].y : d < 6 ? w[0].z : w[0].w, d < 2 ? w[1].x : d < 4 ? w[1].y : d < 6 ? w[1].z : w[1].w,
+                                       d < 2 ? w[2].x : d < 4 ? w[2].y : d < 6 ? w[2].z : w[2].w, d < 2 ? w[3].x : d < 4 ? w[3].y : d < 6 ? w[3].z : w[3].w};
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {           // bytes 2 e, 2 e + 1 of two positions: b0 b0' b1 b1'
+                    const uint32_t lo = prmt(x[0], x[1], e ? 0x7362 : 0x5140), hi = prmt(x[2], x[3], e ? 0x7362 : 0x5140);
+                    const uint32_t v[4] = {codes_f16x2(lo), codes_f16x2(lo >> 16), codes_f16x2(hi), codes_f16x2(hi >> 16)};
+                    value_step(d + e, v);
+                }
+            }
+        } else {
+            const int mi = lane >> 3, rr = lane & 7;
+#pragma unroll
+            for (int d = 0; d < 8; ++d) {
+                uint32_t v[4];
+                amma::ldmatrix_x4_trans(vs + ((mi >> 1) * 8 + rr) * 2 * kHd + (((2 * d + (mi & 1)) ^ rr) << 4), v[0], v[1], v[2], v[3]);
+                value_step(d, v);
+            }
+        }
+        __syncwarp();                                   // the stage is filled again in the next turn
+        stage = stage == Sh::kStages - 1 ? 0 : stage + 1;
+    }
+    lm::cp_async_wait<0>();
+    __syncwarp();
+
+    // ---- the warps' results to shared memory: [row][128]
+    float* so = reinterpret_cast<float*>(dsm + warp * Sh::kPerWarp);
+    const float vmul = kCoded ? vref : 1.f;
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            float sum = l[j][e];
+            sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+            const int r = 8 * j + 2 * tq + e;
+            if (g == 0) { s_m[warp][r] = mx[j][e]; s_l[warp][r] = sum; }
+#pragma unroll
+            for (int d = 0; d < 8; ++d) {
+                if (kCoded) {
+                    *reinterpret_cast<float2*>(so + r * kHd + 16 * g + 2 * d) = make_float2(o[j][d][e] * vmul, o[j][d][e + 2] * vmul);
+                } else {
+                    so[r * kHd + 16 * d + g] = o[j][d][e];
+                    so[r * kHd + 16 * d + g + 8] = o[j][d][e + 2];
+                }
+            }
+        }
+    __syncthreads();
+    for (int r = warp; r < Sh::kRows; r += kWarps) {    // a warp per row, four dimensions a lane
+        const int row = r0 + r, node = row / a.group;
+        if (node >= nodes) break;
+        float top = -FLT_MAX, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_m[w][r]);
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float c = lm::exp2_fast(s_m[w][r] - top);
+            const float4 v = *reinterpret_cast<const float4*>(dsm + w * Sh::kPerWarp + (r * kHd + 4 * lane) * 4);
+            sum = fmaf(s_l[w][r], c, sum);
+            acc.x = fmaf(v.x, c, acc.x); acc.y = fmaf(v.y, c, acc.y); acc.z = fmaf(v.z, c, acc.z); acc.w = fmaf(v.w, c, acc.w);
+        }
+        if (a.nsplit == 1) {
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;   // a row that sees nothing: 0
+            A* out = static_cast<A*>(a.out) + (((size_t)m * a.T + node) * a.nq + head * a.group + row - node * a.group) * kHd + 4 * lane;
+            store_o4(out, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+        } else {
+            float* rec = a.part + ((((size_t)m * a.c.heads + head) * a.rows + row) * a.nsplit + split) * kPart;
+            *reinterpret_cast<float4*>(rec + 4 * lane) = acc;
+            if (lane == 0) *reinterpret_cast<float2*>(rec + kHd) = make_float2(top, sum);
+        }
+    }
+}
+
+// The splits' records of a row, a warp each.
+template <typename A>
+__global__ void __launch_bounds__(128) attend_merge_kernel(const Args a) {
+    pdl_trigger();
+    pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const long at = (long)blockIdx.x * 4 + (threadIdx.x >> 5);     // (m, head, row)
+    if (at >= (long)a.M * a.c.heads * a.rows) return;
+    const int row = (int)(at % a.rows), mh = (int)(at / a.rows), m = mh / a.c.heads, head = mh - m * a.c.heads, node = row / a.group;
+    if (a.first[m] < 0 || node >= node_count(a, m)) return;
+    const float* rec = a.part + (size_t)at * a.nsplit * kPart;
+    float top = -FLT_MAX, sum = 0.f;
+    for (int s = lane; s < a.nsplit; s += 32) top = fmaxf(top, rec[(size_t)s * kPart + kHd]);
+    top = warp_max(top);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < a.nsplit; ++s) {
+        const float2 ml = *reinterpret_cast<const float2*>(rec + (size_t)s * kPart + kHd);
+        const float4 v = *reinterpret_cast<const float4*>(rec + (size_t)s * kPart + 4 * lane);
+        const float c = lm::exp2_fast(ml.x - top);
+        sum = fmaf(ml.y, c, sum);
+        acc.x = fmaf(v.x, c, acc.x); acc.y = fmaf(v.y, c, acc.y); acc.z = fmaf(v.z, c, acc.z); acc.w = fmaf(v.w, c, acc.w);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    A* out = static_cast<A*>(a.out) + (((size_t)m * a.T + node) * a.nq + head * a.group + row - node * a.group) * kHd + 4 * lane;
+    store_o4(out, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+}
+
+}  // namespace tree
+}  // namespace bw

@@ -1,0 +1,284 @@
+// Rows of a KV cache: written from the QKV projection (head norm, rotation, quantising), moved between the beams of a search, and
+// moved together once a path of a drafted tree has been accepted.
+#include <cuda_bf16.h>
+#include <math.h>
+
+#include "common.cuh"
+#include "host_util.h"
+#include "kv_cache.cuh"
+#include "lm_device.cuh"
+
+namespace bw {
+namespace kv {
+
+// ------------------------------------------------------------------------------------------------------------------ writing
+struct WriteArgs {
+    void* q_out;
+    View c;
+    const void* qkv;
+    const float *q_w, *k_w;
+    const int *first, *offset, *count;
+    int nq, M, T;
+    float eps;
+    double ratio;                       // base^(-2/128)
+};
+__device__ __forceinline__ float4 load_act4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float4 load_act4(const __nv_bfloat16* p) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u), __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xFFFF0000u));
+}
+__device__ __forceinline__ void store_act4(float* p, const float4& v) { *reinterpret_cast<float4*>(p) = v; }
+__device__ __forceinline__ void store_act4(__nv_bfloat16* p, const float4& v) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(lm::pack_bf16(v.x, v.y), lm::pack_bf16(v.z, v.w));
+}
+// base^(-2i/128) = ratio^i for i = 2 lane, by the bits of lane.  64 bits: a position times a 32-bit frequency is off by position * 2^-24,
+// a visible angle from some thousand positions on.
+__device__ __forceinline__ double even_frequency(double ratio, int lane) {
+    double f = 1.0, s = ratio * ratio;
+#pragma unroll
+    for (int bit = 1; bit < 32; bit <<= 1) {
+        if (lane & bit) f *= s;
+        s *= s;
+    }
+    return f;
+}
+// cos, sin of position * frequency, reduced to a half turn in 64 bits.
+__device__ __forceinline__ float2 turn_of(double position, double frequency) {
+    const double a = position * frequency;
+    const float r = (float)fma(-rint(a * 0.15915494309189535), 6.283185307179586, a);
+    float s, c;
+    sincosf(r, &s, &c);
+    return make_float2(c, s);
+}
+
+// A warp takes HW heads of one row (token or node), four dimensions of each per lane.  x / sqrt(mean x^2 + eps) * w, then pairs
+// (2i, 2i + 1) turned; a cached row is stored in binary16, or divided by absmax / 448 and rounded to e4m3.
+template <typename A, int HW>
+__global__ void __launch_bounds__(256) write_rows_kernel(const WriteArgs a) {
+    pdl_trigger();
+    pdl_wait();
+    const int lane = threadIdx.x & 31, heads = a.nq + 2 * a.c.heads, per_row = (heads + HW - 1) / HW;
+    const long gw = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const long at = gw / per_row;                       // row of the call
+    if (at >= (long)a.M * a.T) return;
+    const int m = (int)(at / a.T), i = (int)(at - (long)m * a.T), h0 = (int)(gw - at * per_row) * HW;
+    const int first = a.first[m];
+    if (first < 0 || (a.count && i >= a.count[m])) return;
+    const A* x = static_cast<const A*>(a.qkv) + (at * heads + h0) * kHd + 4 * lane;
+    float4 v[HW];
+#pragma unroll
+    for (int j = 0; j < HW; ++j) v[j] = h0 + j < heads ? load_act4(x + j * kHd) : make_float4(0.f, 0.f, 0.f, 0.f);
+    float2 r0 = make_float2(1.f, 0.f), r1 = r0;
+    if (h0 < a.nq + a.c.heads) {
+        const double p = (double)((long)first + (a.offset ? a.offset[at] : i));
+        const double f = even_frequency(a.ratio, lane);
+        r0 = turn_of(p, f);
+        r1 = turn_of(p, f * a.ratio);
+    }
+    const long row = (long)first + i;
+#pragma unroll
+    for (int j = 0; j < HW; ++j) {
+        const int h = h0 + j;
+        if (h >= heads) break;
+        float4 y = v[j];
+        if (h < a.nq + a.c.heads) {
+            const float* w = h < a.nq ? a.q_w : a.k_w;
+            if (w) {
+                const float ss = warp_sum(fmaf(y.w, y.w, fmaf(y.z, y.z, fmaf(y.y, y.y, y.x * y.x))));
+                const float is = rsqrtf(ss / 128.0f + a.eps);
+                const float4 g = *reinterpret_cast<const float4*>(w + 4 * lane);
+                y = make_float4(y.x * is * g.x, y.y * is * g.y, y.z * is * g.z, y.w * is * g.w);
+            }
+            y = make_float4(fmaf(y.x, r0.x, -(y.y * r0.y)), fmaf(y.x, r0.y, y.y * r0.x), fmaf(y.z, r1.x, -(y.w * r1.y)),
+                            fmaf(y.z, r1.y, y.w * r1.x));
+        }
+        if (h < a.nq) {
+            store_act4(static_cast<A*>(a.q_out) + (at * a.nq + h) * kHd + 4 * lane, y);
+            continue;
+        }
+        if (row >= a.c.max_seq) continue;               // a row outside of the cache is never written
+        const bool is_k = h < a.nq + a.c.heads;
+        const size_t to = a.c.row(m, h - a.nq - (is_k ? 0 : a.c.heads), row);
+        unsigned char* side = is_k ? a.c.k : a.c.v;
+        if (!a.c.coded()) {
+            const __half2 lo = __floats2half2_rn(y.x, y.y), hi = __floats2half2_rn(y.z, y.w);
+            *reinterpret_cast<uint2*>(side + (to * kHd + 4 * lane) * 2) =
+                make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+        } else {
+            const float top = warp_max(fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
+            const bool tiny = top < kTinyRow;
+            const float up = tiny ? 1.f : kCodeMax / top;
+            const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y.x * up, y.y * up), __NV_SATFINITE, __NV_E4M3);
+            const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y.z * up, y.w * up), __NV_SATFINITE, __NV_E4M3);
+            *reinterpret_cast<uint32_t*>(side + to * kHd + 4 * lane) = lo | hi << 16;
+            if (lane == 0) (is_k ? a.c.ks : a.c.vs)[to] = tiny ? 1.f : top / kCodeMax;
+        }
+    }
+}
+
+template <typename A>
+static cudaError_t write_launch(const WriteArgs& a, cudaStream_t st) {
+    const int heads = a.nq + 2 * a.c.heads;
+    const long rows = (long)a.M * a.T;
+    // Few rows: a warp per head, everything is latency.  Many: four heads a warp share the angles and keep four loads in flight.
+    const bool many = rows * heads > 32L * sm_count(current_device());
+    const long warps = rows * (many ? (heads + 3) / 4 : heads), blocks = (warps + 7) / 8;
+    if (blocks > 0x7FFFFFFFL) return cudaErrorInvalidValue;
+    const cudaError_t e = launch_pdl(many ? write_rows_kernel<A, 4> : write_rows_kernel<A, 1>, dim3((unsigned)blocks), dim3(256), 0, st, a);
+    count_launch(1);
+    return e != cudaSuccess ? e : cudaPeekAtLastError();
+}
+
+// ------------------------------------------------------------------------------------------------------------------ moving
+struct MoveArgs {
+    View c;
+    size_t layer_stride;                // rows
+    int layers;
+    const int *index, *from, *to;       // parents / path; rows [from, to) / first row and count
+    int n;                              // beams / most rows of a path
+};
+constexpr int kMaxBeams = 32, kMaxPath = 64;
+
+// Sequence m * beams + b takes the rows [from, to) of m * beams + parent[b].  A thread owns 16 bytes of a row (and the row's scale,
+// the first of them) in all beams of a group: it reads what every changed beam gets, then writes, so that parents may change too.
+template <int NB>
+__global__ void __launch_bounds__(256) reorder_kernel(const MoveArgs a) {
+    pdl_trigger();
+    pdl_wait();
+    const int m = blockIdx.z, side = blockIdx.y & 1, plane = blockIdx.y >> 1;
+    const int layer = plane / a.c.heads, g = plane - layer * a.c.heads;
+    const int lo = a.from ? max(a.from[m], 0) : 0, hi = min(a.to[m], a.c.max_seq);
+    const bool coded = a.c.coded();
+    const int cols = coded ? 8 : 16;                    // 16-byte pieces of a row
+    uint4* data = reinterpret_cast<uint4*>(side ? a.c.v : a.c.k);
+    float* scale = side ? a.c.vs : a.c.ks;
+    int parent[NB];
+    bool any = false;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        const int p = b < a.n ? a.index[m * a.n + b] : b;
+        parent[b] = p >= 0 && p < a.n && p != b ? p : -1;
+        any |= parent[b] >= 0;
+    }
+    if (!any) return;
+    const size_t base = a.c.row(m * a.n, g, 0) + layer * a.layer_stride, seq = a.c.batch / kHd;
+    for (long u = (long)blockIdx.x * 256 + threadIdx.x; u < (long)(hi - lo) * cols; u += (long)gridDim.x * 256) {
+        const long r = u / cols;
+        const int col = (int)(u - r * cols);
+        const size_t row = base + lo + r;
+        uint4 x[NB];
+        float s[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+            if (parent[b] >= 0) {
+                x[b] = data[(row + parent[b] * seq) * cols + col];
+                if (coded && col == 0) s[b] = scale[row + parent[b] * seq];
+            }
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+            if (parent[b] >= 0) {
+                data[(row + b * seq) * cols + col] = x[b];
+                if (coded && col == 0) scale[row + b * seq] = s[b];
+            }
+    }
+}
+
+// Row first + i takes row first + path[i], i < count: a block reads all rows of a plane (one side of a head in a layer), then writes.
+__global__ void __launch_bounds__(256) keep_rows_kernel(const MoveArgs a) {
+    pdl_trigger();
+    pdl_wait();
+    const int m = blockIdx.y, side = blockIdx.x & 1, plane = blockIdx.x >> 1;
+    const int layer = plane / a.c.heads, g = plane - layer * a.c.heads;
+    const int first = a.from[m], n = min(a.to[m], a.n);
+    if (first < 0 || n <= 0) return;
+    const bool coded = a.c.coded();
+    const int cols = coded ? 8 : 16;
+    uint4* data = reinterpret_cast<uint4*>(side ? a.c.v : a.c.k);
+    float* scale = side ? a.c.vs : a.c.ks;
+    const size_t base = a.c.row(m, g, first) + layer * a.layer_stride;
+    constexpr int kPer = kMaxPath * 16 / 256;
+    uint4 x[kPer];
+    float s[kPer];
+    bool moves[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+        const int u = threadIdx.x + 256 * j, i = u / cols, col = u - i * cols;
+        moves[j] = false;
+        if (i < n) {
+            const int p = a.index[(size_t)m * a.n + i];
+            moves[j] = p >= 0 && p < a.n && p != i && (long)first + max(p, i) < a.c.max_seq;
+            if (moves[j]) {
+                x[j] = data[(base + p) * cols + col];
+                if (coded && col == 0) s[j] = scale[base + p];
+            }
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kPer; ++j)
+        if (moves[j]) {
+            const int u = threadIdx.x + 256 * j, i = u / cols, col = u - i * cols;
+            data[(base + i) * cols + col] = x[j];
+            if (coded && col == 0) scale[base + i] = s[j];
+        }
+}
+
+}  // namespace kv
+}  // namespace bw
+
+using namespace bw;
+
+extern "C" int bw_qk_norm_rope_kv_rows(void* q_out, const bw_kv_cache* cache, const void* qkv, const float* q_norm_w_or_null,
+                                       const float* k_norm_w_or_null, const int* d_first_row, const int* d_offset_or_null,
+                                       const int* d_count_or_null, int num_q_heads, int M, int T, float eps, float rope_base, int bf16,
+                                       void* stream) {
+    kv::WriteArgs a{};
+    if (!kv::view(cache, &a.c) || !a.c.apart(M) || !q_out || !qkv || !d_first_row || num_q_heads < 1 || M < 1 || T < 1 || !(rope_base > 0.f) || !(eps >= 0.f))
+        return cudaErrorInvalidValue;
+    if (!kv::aligned(q_out, 16) || !kv::aligned(qkv, 16) || !kv::aligned(q_norm_w_or_null, 16) || !kv::aligned(k_norm_w_or_null, 16))
+        return cudaErrorInvalidValue;
+    a.q_out = q_out; a.qkv = qkv; a.q_w = q_norm_w_or_null; a.k_w = k_norm_w_or_null;
+    a.first = d_first_row; a.offset = d_offset_or_null; a.count = d_count_or_null;
+    a.nq = num_q_heads; a.M = M; a.T = T; a.eps = eps;
+    a.ratio = pow((double)rope_base, -2.0 / kv::kHd);
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return bf16 ? kv::write_launch<__nv_bfloat16>(a, st) : kv::write_launch<float>(a, st);
+}
+
+// What both moves check of their planes: layers of layer_stride elements from the cache's own layer on.
+static bool move_args(const bw_kv_cache* cache, long sequences, int layers, size_t layer_stride_elems, kv::MoveArgs* a) {
+    if (!kv::view(cache, &a->c) || !a->c.apart(sequences) || layers < 1 || layer_stride_elems % kv::kHd) return false;
+    if (layers > 1 && layer_stride_elems / kv::kHd < (size_t)a->c.heads * a->c.max_seq) return false;
+    a->layers = layers;
+    a->layer_stride = layer_stride_elems / kv::kHd;
+    return true;
+}
+
+extern "C" int bw_kv_reorder(const bw_kv_cache* cache, const int* d_parent, const int* d_from_or_null, const int* d_to, int beams, int M,
+                             int layers, size_t layer_stride_elems, void* stream) {
+    kv::MoveArgs a{};
+    if (beams < 1 || beams > kv::kMaxBeams || M < 1 || M > 65535 || !move_args(cache, (long)M * beams, layers, layer_stride_elems, &a) || !d_parent || !d_to)
+        return cudaErrorInvalidValue;
+    a.index = d_parent; a.from = d_from_or_null; a.to = d_to; a.n = beams;
+    const long planes = 2L * layers * a.c.heads;
+    if (planes > 65535) return cudaErrorInvalidValue;
+    const long most = ((long)a.c.max_seq * (a.c.coded() ? 8 : 16) + 255) / 256, fill = (32L * sm_count(current_device()) + planes * M - 1) / (planes * M);
+    const dim3 grid((unsigned)(most < fill ? most : fill), (unsigned)planes, (unsigned)M);
+    auto kern = beams <= 4 ? kv::reorder_kernel<4> : beams <= 8 ? kv::reorder_kernel<8> : beams <= 16 ? kv::reorder_kernel<16> : kv::reorder_kernel<32>;
+    const cudaError_t e = launch_pdl(kern, grid, dim3(256), 0, static_cast<cudaStream_t>(stream), a);
+    count_launch(1);
+    return e != cudaSuccess ? e : cudaPeekAtLastError();
+}
+
+extern "C" int bw_kv_keep_rows(const bw_kv_cache* cache, const int* d_first_row, const int* d_path, const int* d_count, int M, int T, int layers,
+                               size_t layer_stride_elems, void* stream) {
+    kv::MoveArgs a{};
+    if (!move_args(cache, M, layers, layer_stride_elems, &a) || !d_first_row || !d_path || !d_count || M < 1 || M > 65535 || T < 1 || T > kv::kMaxPath)
+        return cudaErrorInvalidValue;
+    a.index = d_path; a.from = d_first_row; a.to = d_count; a.n = T;
+    const long planes = 2L * layers * a.c.heads;
+    if (planes > 0x7FFFFFFFL) return cudaErrorInvalidValue;
+    const cudaError_t e = launch_pdl(kv::keep_rows_kernel, dim3((unsigned)planes, (unsigned)M), dim3(256), 0, static_cast<cudaStream_t>(stream), a);
+    count_launch(1);
+    return e != cudaSuccess ? e : cudaPeekAtLastError();
+}

@@ -296,6 +296,62 @@ int bw_attention_decode_batched_gqa_noalloc(float* output, const float* Q, const
                                             int num_kv_heads, int head_dim, int max_seq_len, int M,
                                             size_t kv_batch_elems, size_t kv_layer_elems, void* stream);
 
+/* ---- Several continuations of a sequence on one KV cache (no counterpart in the reference) ----
+ * What a step needs that verifies a drafted tree, searches with beams or keeps its cache in 8 bits.  A cache as these calls take it: head g
+ * of sequence m holds row t (128 elements) from element m * batch_elems + layer_elems + (g * max_seq + t) * 128 of k and v on, in
+ * binary16 (k_scale, v_scale NULL: the layout of bw_attention_decode_f16kv) or in e4m3 codes with an fp32 scale >= 0 per row (value = code * scale), that of
+ * a row at its element / 128.  batch_elems and layer_elems are multiples of 128, k and v 16-byte aligned; calls that write need sequences that
+ * do not overlap.  Activations are fp32, or bfloat16 with bf16 != 0; q, qkv, out and norm weights 16-byte aligned.  All counts, rows, masks
+ * and parents are in device memory; nothing allocates, and no state is kept between calls: scratch is the caller's (16-byte aligned,
+ * contents of no matter; calls that may overlap need one each). */
+typedef struct bw_kv_cache {
+    void *k, *v;
+    float *k_scale, *v_scale;
+    int kv_heads, max_seq;
+    size_t batch_elems, layer_elems;
+} bw_kv_cache;
+
+/* T rows (tokens, or the nodes of a tree) of each of M sequences out of the fused QKV projection qkv [M][T][(nq + 2 nkv) * 128]: query and
+ * key heads get the RMS norm per head (weights fp32 [128]; NULL: none) and the rotation of interleaved pairs by position * rope_base^(-2i/128), the angle
+ * formed in 64 bits; queries go to q_out [M][T][nq * 128], keys and values to the rows first[m] + i of the cache.  The position of row i is
+ * first[m] + offset[m][i] (a node's depth), or first[m] + i where offset is NULL.  e4m3: scale = absmax / 448 (1 where absmax < 1e-10),
+ * code = the nearest to x * (448 / absmax).  Rows i >= count[m] (NULL: T) and those of a sequence with first[m] < 0 are skipped: nothing of
+ * them is read or written.  A row at or beyond max_seq is not stored; its query is. */
+int bw_qk_norm_rope_kv_rows(void* q_out, const bw_kv_cache* cache, const void* qkv, const float* q_norm_w_or_null,
+                            const float* k_norm_w_or_null, const int* d_first_row, const int* d_offset_or_null, const int* d_count_or_null,
+                            int num_q_heads, int M, int T, float eps, float rope_base, int bf16, void* stream);
+/* Attention of T <= 64 rows of each of M sequences, scale 1 / sqrt(128): node i of sequence m sees the cached rows below first[m] and, of
+ * the rows first[m] + j, those whose bit j is set in mask[m][i] (NULL: j <= i; T == 1 is a decode step with first[m] the token's position).  Nodes
+ * i >= count[m] (NULL: T) do not exist: nobody sees them and their outputs are left as they were, as are those of a sequence with
+ * first[m] < 0.  Rows at or beyond max_seq are not seen.  A node that sees nothing gets zeros.  Cached rows that no node of the sequence sees may
+ * hold anything; the others must be finite.  num_q_heads is any multiple of the cache's heads.  ctx_hint is a bound on
+ * first[m] + T that sizes the splits (0: max_seq); longer sequences are still right.  scratch: bw_attention_tree_scratch_bytes, with the largest
+ * sizes in use. */
+int bw_attention_tree(void* out, const void* q, const bw_kv_cache* cache, const int* d_first_row, const unsigned long long* d_mask_or_null,
+                      const int* d_count_or_null, int ctx_hint, int num_q_heads, int M, int T, int bf16, void* scratch, size_t scratch_bytes,
+                      void* stream);
+size_t bw_attention_tree_scratch_bytes(int M, int T, int num_q_heads, int num_kv_heads, int max_context);
+/* Beam search's selection for M requests of `beams` beams each: candidates score[m][b] + log_softmax(logits[m * beams + b])[v] over all beams and
+ * tokens, of which the `keep` best (largest first; equal ones by lower beam, then token) go to parent_out, token_out, score_out [M][keep].  logits fp32 [M * beams][row_stride].
+ * A beam that has ended (ended[m][b] != 0) offers itself alone, as (eos_id, score unchanged); ended_out = ended[parent] or token == eos_id.
+ * Candidates of score -inf are none: where fewer than `keep` are left, parent and token are -1 and the score -inf.  A NaN logit counts as -inf; a
+ * row with a logit of +inf offers nothing.  Log-sums and comparisons are in 64 bits.  beams <= 64, keep <= 64.  score_out may be score and
+ * ended_out ended, with keep == beams. */
+int bw_beam_select(int* parent_out, int* token_out, float* score_out, unsigned char* ended_out_or_null, const float* logits, long row_stride,
+                   int vocab, const float* score, const unsigned char* ended_or_null, int eos_id, int beams, int keep, int M, void* scratch,
+                   size_t scratch_bytes, void* stream);
+size_t bw_beam_select_scratch_bytes(int vocab, int beams, int keep, int M);
+/* Moves rows inside a cache, in `layers` layers from layer_elems on, layer_stride_elems apart (a multiple of 128).
+ * bw_kv_reorder: sequence m * beams + b takes the rows [from[m], to[m]) (from NULL: 0; cut off at max_seq) of sequence m * beams + parent[m][b], all beams at
+ * once: a beam may be overwritten and the parent of others.  A parent outside of 0 .. beams - 1 leaves its beam as it is.  beams <= 32.
+ * bw_kv_keep_rows: row first[m] + i takes row first[m] + path[m][i] for i < count[m], all at once (path [M][T], T <= 64): the accepted
+ * nodes of a tree, in order, become the sequence's next rows.  A row whose place or source is not inside 0 .. T - 1 and the cache, and a
+ * sequence with first[m] < 0, is left as it is. */
+int bw_kv_reorder(const bw_kv_cache* cache, const int* d_parent, const int* d_from_or_null, const int* d_to, int beams, int M, int layers,
+                  size_t layer_stride_elems, void* stream);
+int bw_kv_keep_rows(const bw_kv_cache* cache, const int* d_first_row, const int* d_path, const int* d_count, int M, int T, int layers,
+                    size_t layer_stride_elems, void* stream);
+
 /* ----------------------------------------------------------------- sampling -- */
 
 /* replaces sample_argmax_gpu: kernels.h:1095-1099, src/kernels/sample_gpu.cu:30-60,250-254 */

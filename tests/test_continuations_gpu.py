@@ -1,0 +1,604 @@
+"""Cache rows, tree attention, beam selection and moves of cached rows against plain evaluations in 64 bits."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+HD = 128
+F8 = torch.float8_e4m3fn
+BOTH = pytest.mark.parametrize("act", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+CACHES = pytest.mark.parametrize("coded", [False, True], ids=["f16", "e4m3"])
+
+
+def ints(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def kernels():
+    from blackwell_b200 import kernels
+    return kernels
+
+
+class Store:
+    """A cache of M sequences and some layers, filled with random rows (or NaN) and read back in 64 bits."""
+
+    def __init__(self, g, M, layers, nkv, max_seq, coded, fill="random", v_size=1.0):
+        shape = (M, layers, nkv, max_seq)
+        self.shape, self.coded, self.plane = shape, coded, nkv * max_seq * HD
+        x = [torch.empty(shape + (HD,), device="cuda").normal_(generator=g) for _ in range(2)]
+        if coded:
+            self.k, self.v = [(y * 100).clamp(-448, 448).to(F8) for y in x]
+            self.ks = torch.empty(shape, device="cuda").uniform_(0.002, 0.02, generator=g)
+            self.vs = torch.empty(shape, device="cuda").uniform_(0.002, 0.02, generator=g) * v_size
+        else:
+            self.k, self.v = x[0].half(), (x[1] * v_size).half()
+            self.ks = self.vs = None
+        if fill == "nan":
+            for t in (self.k, self.v):
+                t.view(torch.uint8).fill_(0x7F if coded else 0x7E)
+            if coded:
+                self.ks.fill_(math.nan)
+                self.vs.fill_(math.nan)
+
+    def args(self, layer=0):
+        return kernels().KVCache(self.k, self.v, self.ks, self.vs, self.shape[2], self.shape[3], self.shape[1] * self.plane, layer * self.plane)
+
+    def value(self, layer=0):
+        """k, v [M][nkv][max_seq][128] in 64 bits."""
+        k, v = self.k[:, layer].double(), self.v[:, layer].double()
+        return (k * self.ks[:, layer, ..., None].double(), v * self.vs[:, layer, ..., None].double()) if self.coded else (k, v)
+
+    def bits(self):
+        return [t.view(torch.uint8).clone() for t in (self.k, self.v) + ((self.ks, self.vs) if self.coded else ())]
+
+
+# ------------------------------------------------------------------------------------------------------------------ writing rows
+def check_write(M, T, nq, nkv, first, max_seq, coded, act, offset=None, count=None, norms=True, base=1e6, size=1.0, layers=2, layer=1, seed=0):
+    g = torch.Generator("cuda").manual_seed(seed)
+    st = Store(g, M, layers, nkv, max_seq, coded)
+    qkv = (torch.empty((M, T, nq + 2 * nkv, HD), device="cuda").normal_(generator=g) * size).to(act)
+    w = [torch.empty(HD, device="cuda").uniform_(0.5, 1.5, generator=g) for _ in range(2)] if norms else [None, None]
+    q = torch.full((M, T, nq, HD), 7.0, dtype=act, device="cuda")
+    before, old = st.bits(), st.value(layer)
+    kernels().qk_norm_rope_kv_rows(q, st.args(layer), qkv, w[0], w[1], ints(first), None if offset is None else ints(offset),
+                                   None if count is None else ints(count), nq, M, T, 1e-6, base)
+    x = qkv.double()
+    freq = base ** (-torch.arange(0, HD, 2, dtype=torch.float64, device="cuda") / HD)
+    after = st.value(layer)
+    written = torch.zeros((M, layers, nkv, max_seq), dtype=torch.bool, device="cuda")
+    half = torch.finfo(act).eps / 2
+
+    def near(got, want, whole, step):
+        # norm (a sum of 128 squares by pairs, rsqrt, two products), angle, sine and cosine to a few units, two products and a sum:
+        # under 16 half steps of 32 bits of the row's largest pair, then the rounding of what is stored
+        bar = 16 * 2.0 ** -24 * math.sqrt(2) * whole + step
+        assert ((got - want).abs() <= bar).all(), ((got - want).abs() / bar).max()
+
+    for m in range(M):
+        for i in range(T):
+            if first[m] < 0 or (count is not None and i >= count[m]):
+                assert (q[m, i] == 7).all()
+                continue
+            p = first[m] + (offset[m][i] if offset is not None else i)
+            c, s = (p * freq).cos(), (p * freq).sin()
+            y = x[m, i].clone()
+            for lo, hi, wt in ((0, nq, w[0]), (nq, nq + nkv, w[1])):
+                if norms:
+                    y[lo:hi] = y[lo:hi] / (y[lo:hi].square().mean(-1, keepdim=True) + 1e-6).sqrt() * wt.double()
+                a, b = y[lo:hi, 0::2].clone(), y[lo:hi, 1::2].clone()
+                y[lo:hi, 0::2], y[lo:hi, 1::2] = a * c - b * s, a * s + b * c
+            top = y.abs().amax(-1, keepdim=True)
+            near(q[m, i].double(), y[:nq], top[:nq], y[:nq].abs() * half if act == torch.bfloat16 else 0)
+            row = first[m] + i
+            if row >= max_seq:
+                continue
+            written[m, layer, :, row] = True
+            for got, want, t in ((after[0][m, :, row], y[nq:nq + nkv], top[nq:nq + nkv]), (after[1][m, :, row], y[nq + nkv:], top[nq + nkv:])):
+                if coded:   # half a step of three mantissa bits, or of the smallest codes (2^-9 apart), in units of absmax / 448
+                    near(got, want, t, torch.maximum(want.abs() * 2.0 ** -4, t / 448 * 2.0 ** -10) * (1 + 2.0 ** -18))
+                else:
+                    near(got, want, t, torch.maximum(want.abs() * 2.0 ** -11, torch.full_like(want, 2.0 ** -25)))
+    now = st.bits()
+    for b, a in zip(before, now):   # every other row is as it was
+        rows = b.reshape(M, layers, nkv, max_seq, -1), a.reshape(M, layers, nkv, max_seq, -1)
+        assert torch.equal(rows[0][~written], rows[1][~written])
+
+
+@BOTH
+@CACHES
+@pytest.mark.parametrize("M, T, nq, nkv", [(1, 1, 32, 8), (3, 5, 28, 4), (2, 7, 3, 3), (1, 200, 8, 1), (40, 1, 64, 8)])
+def test_write(cuda, M, T, nq, nkv, coded, act):
+    check_write(M, T, nq, nkv, [(11 * m) % 40 for m in range(M)], 300, coded, act)
+
+
+@CACHES
+def test_write_trees_counts_and_edges(cuda, coded):
+    off = [[0, 1, 1, 2, 2], [0, 0, 0, 1, 3], [0, 1, 2, 3, 4], [0, 0, 1, 1, 1], [0] * 5]
+    check_write(5, 5, 8, 2, [0, 17, -1, 28, 31], 32, coded, torch.float32, offset=off, count=[5, 3, 5, 9, 0])
+    check_write(3, 4, 8, 2, [30, 2 ** 31 - 2, 100], 32, coded, torch.float32)
+
+
+@CACHES
+def test_write_far_positions_and_sizes(cuda, coded):
+    check_write(1, 3, 4, 4, [120000], 120003, coded, torch.float32, layers=1, layer=0)
+    check_write(2, 3, 4, 2, [5, 9], 16, coded, torch.float32, norms=False, base=10000.0)
+    check_write(2, 3, 4, 2, [5, 9], 16, coded, torch.float32, size=1e-4)
+    check_write(2, 3, 4, 2, [5, 9], 16, coded, torch.bfloat16, size=50.0)
+
+
+def test_write_rows_of_zeros_and_tiny_rows(cuda):
+    g = torch.Generator("cuda").manual_seed(1)
+    st = Store(g, 1, 1, 1, 4, True, fill="nan")
+    qkv = torch.zeros((1, 2, 3, HD), device="cuda")
+    qkv[0, 1] = 3e-11
+    q = torch.empty((1, 2, 1, HD), device="cuda")
+    kernels().qk_norm_rope_kv_rows(q, st.args(), qkv, None, None, ints([1]), None, None, 1, 1, 2, 1e-6, 1e4)
+    k, v = st.value()
+    assert (k[0, 0, 1:3] == 0).all() and (v[0, 0, 1:3] == 0).all() and (st.ks[0, 0, 0, 1:3] == 1).all() and st.ks[0, 0, 0, 3].isnan()
+
+
+# ------------------------------------------------------------------------------------------------------------------ attention
+def tree_masks(g, M, T):
+    """Ancestor masks of random trees, as Python integers [M][T]."""
+    out = []
+    for _ in range(M):
+        u = torch.rand(T, generator=g)
+        bits = []
+        for i in range(T):
+            p = int(u[i] * (i + 1)) - 1
+            bits.append((bits[p] if p >= 0 else 0) | 1 << i)
+        out.append(bits)
+    return out
+
+
+def words(masks):
+    return torch.tensor([[b - (1 << 64) if b >> 63 else b for b in row] for row in masks], dtype=torch.int64, device="cuda")
+
+
+def check_attention(M, T, nq, nkv, first, max_seq, coded, act, masks=None, count=None, hint=0, layers=1, layer=0, q_size=1.5, v_size=1.0, seed=0,
+                    store=None, clean=True, stream=None, call=None):
+    g = torch.Generator("cuda").manual_seed(seed)
+    st = store or Store(g, M, layers, nkv, max_seq, coded, v_size=v_size)
+    q = (torch.empty((M, T, nq, HD), device="cuda").normal_(generator=g) * q_size).to(act)
+    out = torch.full((M, T, nq, HD), 7.0, dtype=act, device="cuda")
+    n = [T if count is None else max(0, min(T, c)) for c in (count or [T] * M)]
+    seen = []
+    for m in range(M):
+        f = min(first[m], max_seq)
+        end = min(first[m] + n[m], max_seq)
+        see = torch.zeros((T, max_seq), dtype=torch.bool)
+        for i in range(n[m] if first[m] >= 0 else 0):
+            see[i, :f] = True
+            bits = masks[m][i] if masks is not None else (1 << i + 1) - 1
+            for j in range(end - f):
+                see[i, f + j] = bool(bits >> j & 1)
+        seen.append(see.cuda())
+    if clean:   # what nobody sees holds NaN
+        for m in range(M):
+            for t in (st.k, st.v):
+                t.view(torch.uint8)[m, layer, :, ~seen[m].any(0)] = 0x7F if coded else 0x7E
+            for t in (st.ks, st.vs) if coded else ():
+                t[m, layer, :, ~seen[m].any(0)] = math.nan
+    k = kernels()
+    scratch = torch.full((k.attention_tree_scratch_bytes(M, T, nq, nkv, max_seq),), 255, dtype=torch.uint8, device="cuda")
+    a = (out, q, st.args(layer), ints(first), None if masks is None else words(masks), None if count is None else ints(count), hint, nq, M, T, scratch)
+    (call or k.attention_tree)(*a)
+    kk, vv = st.value(layer)
+    kk, vv = kk.nan_to_num(0), vv.nan_to_num(0)
+    group = nq // nkv
+    for m in range(M):
+        if first[m] < 0:
+            assert (out[m] == 7).all()
+            continue
+        assert (out[m, n[m]:] == 7).all()
+        if n[m] == 0:
+            continue
+        see = seen[m][:n[m], None, :]
+        x = q[m, :n[m]].double().view(n[m], nkv, group, HD)
+        score = torch.einsum("ihgd,htd->ihgt", x, kk[m]) / math.sqrt(HD)
+        score = score.masked_fill(~see[:, :, None].expand_as(score), -math.inf)
+        p = torch.softmax(score, -1).nan_to_num(0)
+        want = torch.einsum("ihgt,htd->ihgd", p, vv[m]).reshape(n[m], nq, HD)
+        got = out[m, :n[m]].double()
+        assert torch.isfinite(got).all()
+        # A score is off by 2^-21 (fp32: operands of 22 bits) or 2^-22 (bf16 operands are exact, 32-bit sums) of sum |q k| / sqrt(128) and by
+        # some roundings of its own size; a probability by that, by 2^-22 of exp2 and by its own rounding (2^-22 / 2^-12); sums of 16 products at a
+        # time, with 2^-23 each; the result is an average of v.
+        size = torch.einsum("ihgd,htd->ihgt", x.abs(), kk[m].abs()).div_(math.sqrt(HD)).masked_fill_(~see[:, :, None].expand_as(score), 0)
+        ds = 2.0 ** -21 * size.amax(-1) + 2.0 ** -22 * score.abs().masked_fill(score.isinf(), 0).amax(-1)
+        fine = 2.0 ** -12 if act == torch.bfloat16 else 2.0 ** -21
+        steps = (first[m] + T) / 16 + 64
+        bar = (2 * ds + 2 * fine + steps * 2.0 ** -23).reshape(n[m], nq, 1) * torch.einsum("ihgt,htd->ihgd", p, vv[m].abs()).reshape(n[m], nq, HD).amax(-1, keepdim=True)
+        if act == torch.bfloat16:
+            bar = bar + want.abs() * 2.0 ** -8
+        assert ((got - want).abs() <= bar).all(), (m, ((got - want).abs() / bar).max())
+    return out
+
+
+@BOTH
+@CACHES
+@pytest.mark.parametrize("M, T, nq, nkv, top", [
+    (1, 1, 32, 8, 1), (1, 1, 32, 8, 700), (5, 1, 28, 4, 300), (3, 1, 4, 4, 90), (2, 1, 48, 3, 1500),      # single tokens
+    (2, 2, 8, 8, 65), (3, 4, 32, 8, 400), (2, 8, 28, 4, 1000), (1, 17, 5, 1, 33), (2, 33, 8, 2, 257), (2, 64, 16, 4, 500), (1, 64, 64, 8, 2100)])
+def test_attention(cuda, M, T, nq, nkv, top, coded, act):
+    g = torch.Generator().manual_seed(T)
+    first = [max(0, top - 1 - (m * 61) % top) for m in range(M)]
+    check_attention(M, T, nq, nkv, first, top + T + 3, coded, act, masks=tree_masks(g, M, T) if T > 1 else None)
+
+
+@BOTH
+@CACHES
+def test_attention_chain_counts_and_slots(cuda, coded, act):
+    """No masks: a chain.  Counts of every kind, slots without a sequence, sequences that end at the cache's end."""
+    check_attention(7, 6, 12, 4, [0, 5, -1, 44, 47, 60, 2 ** 31 - 1], 50, coded, act, count=[6, 0, 6, 4, 6, 100, -3])
+    check_attention(4, 6, 12, 4, [600, 0, -5, 3], 606, coded, act, count=[1, 2, 3, 6], hint=40)
+
+
+@CACHES
+def test_attention_rows_that_see_nothing(cuda, coded):
+    out = check_attention(2, 5, 8, 2, [0, 0], 40, coded, torch.float32, masks=[[0, 2, 0, 4, 8], [0, 0, 0, 0, 0]])
+    assert (out[1] == 0).all() and (out[0, 0] == 0).all() and (out[0, 1] != 0).any()
+    # not itself, later nodes, bits of nodes that do not exist
+    check_attention(2, 5, 8, 2, [7, 0], 40, coded, torch.float32, masks=[[16, 1, 0, 31, 2 ** 64 - 1], [2 ** 63 | 1, 2, 2, 4, 2]], count=[5, 3])
+
+
+@CACHES
+@pytest.mark.parametrize("hint", [1, 300, 5000])
+def test_attention_any_hint(cuda, coded, hint):
+    check_attention(2, 3, 16, 4, [4500, 10], 4700, coded, torch.float32, hint=hint, masks=[[1, 3, 5], [1, 2, 7]])
+
+
+@CACHES
+def test_attention_other_layer_and_long_context(cuda, coded):
+    check_attention(2, 4, 8, 2, [300, 20], 320, coded, torch.float32, layers=3, layer=2)
+    check_attention(1, 3, 4, 1, [40000], 40010, coded, torch.float32, masks=[[1, 3, 5]])
+
+
+@BOTH
+@CACHES
+@pytest.mark.parametrize("q_size, v_size", [(1e-6, 1e-3), (6.0, 100.0), (0.0, 1.0)])
+def test_attention_sizes(cuda, q_size, v_size, coded, act):
+    check_attention(2, 3, 8, 2, [200, 33], 210, coded, act, q_size=q_size, v_size=v_size)
+
+
+def test_attention_value_scales_of_all_sizes(cuda):
+    """Value scales over twenty decades, growing and falling along the context, and rows of scale zero."""
+    g = torch.Generator("cuda").manual_seed(3)
+    for order in (1, -1):
+        st = Store(g, 1, 1, 2, 400, True)
+        st.vs *= torch.logspace(-10, 10, 400, device="cuda")[::order] if order == 1 else torch.logspace(-10, 10, 400, device="cuda").flip(0)
+        st.vs[0, 0, :, ::7] = 0
+        st.ks[0, 0, :, ::5] = 0
+        check_attention(1, 2, 4, 2, [390], 400, True, torch.float32, store=st)
+
+
+def test_attention_far_offsets(cuda):
+    """Sequences whose rows lie beyond 2^32 bytes and elements."""
+    g = torch.Generator("cuda").manual_seed(4)
+    k = kernels()
+    small = Store(g, 2, 1, 2, 300, True)
+    stride = (1 << 32) + 128 * 7
+    rows = stride // 128 + 2 * 300
+    kv = [torch.empty((rows, HD), dtype=F8, device="cuda") for _ in range(2)]
+    sc = [torch.empty(rows, device="cuda") for _ in range(2)]
+    for big, s in zip(kv + sc, (small.k, small.v, small.ks, small.vs)):
+        s = s.view(torch.uint8) if s.dtype == F8 else s
+        big = big.view(torch.uint8) if big.dtype == F8 else big
+        big[:600] = s[0].reshape((600,) + big.shape[1:])
+        big[stride // 128:] = s[1].reshape((600,) + big.shape[1:])
+    c = k.KVCache(kv[0], kv[1], sc[0], sc[1], 2, 300, stride)
+    q = torch.randn((2, 3, 4, HD), generator=g, device="cuda")
+    outs = []
+    for cache in (small.args(), c):
+        out = torch.zeros_like(q)
+        k.attention_tree(out, q, cache, ints([290, 250]), None, None, 0, 4, 2, 3, None)
+        outs.append(out)
+    assert torch.equal(*outs)
+    qkv = torch.randn((2, 1, 8, HD), generator=g, device="cuda")
+    for cache in (small.args(), c):
+        k.qk_norm_rope_kv_rows(torch.empty((2, 1, 4, HD), device="cuda"), cache, qkv, None, None, ints([5, 295]), None, None, 4, 2, 1, 0.0, 1e4)
+    assert torch.equal(kv[0].view(torch.uint8)[stride // 128:], small.k[1].view(torch.uint8).reshape(600, HD))
+    assert torch.equal(sc[1][stride // 128:], small.vs[1].reshape(600))
+
+
+@CACHES
+def test_attention_same_bits_again_and_in_graphs(cuda, coded):
+    """Repeated calls, a captured one that is replayed with other positions, and calls on two streams at once."""
+    g = torch.Generator("cuda").manual_seed(5)
+    k = kernels()
+    M, T, nq, nkv = 2, 4, 16, 4
+    st = Store(g, M, 1, nkv, 2100, coded)
+    q = torch.randn((M, T, nq, HD), generator=g, device="cuda")
+    first, out = ints([2000, 700]), torch.zeros((M, T, nq, HD), device="cuda")
+    new = lambda: torch.empty(k.attention_tree_scratch_bytes(M, T, nq, nkv, 2100), dtype=torch.uint8, device="cuda")  # noqa: E731
+    scratch, cache = new(), st.args()
+    k.attention_tree(out, q, cache, first, None, None, 0, nq, M, T, scratch)
+    want = out.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        k.attention_tree(out, q, cache, first, None, None, 0, nq, M, T, scratch)
+    for pos in ([2000, 700], [64, 1999], [2000, 700]):
+        first.copy_(ints(pos))
+        graph.replay()
+        eager = torch.zeros_like(out)
+        k.attention_tree(eager, q, cache, first, None, None, 0, nq, M, T, new())
+        assert torch.equal(eager, out)
+    assert torch.equal(out, want)
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], [torch.zeros_like(out) for _ in range(2)]
+    work = [new(), new()]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for s, o, w in zip(streams, outs, work):
+            k.attention_tree(o, q, cache, first, None, None, 0, nq, M, T, w, stream=s)
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+
+
+# ------------------------------------------------------------------------------------------------------------------ beam selection
+def check_select(logits, score, ended, eos, keep, M, B, stride=None, inplace=False):
+    V = logits.shape[1]
+    k = kernels()
+    parent, token = torch.full((M, keep), 99, dtype=torch.int32, device="cuda"), torch.full((M, keep), 99, dtype=torch.int32, device="cuda")
+    s_in, e_in = score.clone(), None if ended is None else ended.clone()
+    s_out = s_in if inplace else torch.full((M, keep), 99.0, device="cuda")
+    e_out = e_in if inplace else torch.full((M, keep), 99, dtype=torch.uint8, device="cuda")
+    scratch = torch.full((k.beam_select_scratch_bytes(V, B, keep, M),), 255, dtype=torch.uint8, device="cuda")
+    full = logits
+    if stride:
+        full = torch.full((M * B, stride), math.nan, device="cuda")
+        full[:, :V] = logits
+    k.beam_select(parent, token, s_out, e_out, full, stride or V, V, s_in, e_in, eos, B, keep, M, scratch)
+    x = torch.where(logits.isnan(), -math.inf, logits).double().view(M, B, V)
+    x = (score.double()[..., None] + torch.log_softmax(x, -1)).nan_to_num(-math.inf, math.inf, -math.inf)
+    if ended is not None:
+        own = torch.full((V,), -math.inf, dtype=torch.float64, device="cuda")
+        for m, b in ended.bool().nonzero().tolist():
+            x[m, b] = own
+            x[m, b, eos] = score[m, b].double()
+    val, at = x.view(M, -1).sort(dim=1, descending=True, stable=True)
+    if val.shape[1] < keep:
+        pad = keep - val.shape[1]
+        val, at = torch.nn.functional.pad(val, (0, pad), value=-math.inf), torch.nn.functional.pad(at, (0, pad))
+    val, at = val[:, :keep], at[:, :keep]
+    none = val == -math.inf
+    wp, wt = torch.where(none, -1, at // V), torch.where(none, -1, at % V)
+    assert torch.equal(parent.long(), wp) and torch.equal(token.long(), wt)
+    # exp2 of 32 bits in the log-sums (2^-21 of an argument under 2^5), then the rounding to 32 bits
+    assert torch.equal(s_out.isinf(), none)
+    fine = ~none
+    assert ((s_out.double() - val)[fine].abs() <= val[fine].abs() * 2.0 ** -24 + 2.0 ** -20).all()
+    gone = (wt == eos) & fine
+    if ended is not None:
+        gone |= fine & ended.bool().gather(1, wp.clamp(min=0))
+    assert torch.equal(e_out.bool(), gone)
+
+
+@pytest.mark.parametrize("M, B, V, keep", [(1, 1, 1, 1), (1, 1, 7, 10), (2, 4, 1000, 4), (1, 4, 32768, 8), (3, 7, 2049, 14), (2, 8, 151643, 8), (1, 64, 5000, 64),
+                                           (20, 16, 8193, 32), (1, 2, 300000, 1)])
+def test_select(cuda, M, B, V, keep):
+    g = torch.Generator("cuda").manual_seed(V + keep)
+    logits = torch.empty((M * B, V), device="cuda").normal_(generator=g) * 2
+    score = -torch.rand((M, B), generator=g, device="cuda") * 3
+    check_select(logits, score, None, -1, keep, M, B)
+    ended = (torch.rand((M, B), generator=g, device="cuda") < 0.4).to(torch.uint8)
+    check_select(logits, score, ended, min(2, V - 1), keep, M, B, stride=V + 5)
+    if keep == B:
+        check_select(logits, score, ended, min(2, V - 1), keep, M, B, inplace=True)
+
+
+@pytest.mark.parametrize("keep", [1, 5, 64])
+def test_select_equal_and_few_values(cuda, keep):
+    """Many equal logits (more than are ranked at once), rows of few values, nothing left."""
+    g = torch.Generator("cuda").manual_seed(keep)
+    B, V = 3, 20000
+    score = torch.tensor([[-1.0, -1.0, -1.0]], device="cuda")
+    check_select(torch.zeros((B, V), device="cuda"), score, None, -1, keep, 1, B)
+    steps = torch.randint(0, 3, (B, V), generator=g, device="cuda").float()
+    check_select(steps.repeat(2, 1), score.repeat(2, 1), None, 5, keep, 2, B)
+    some = torch.full((B, V), -math.inf, device="cuda")
+    some[0, 17], some[2, 17], some[2, 19999] = 1.0, 3.0, 3.0
+    check_select(some, score, None, 17, keep, 1, B)
+    many = torch.where(torch.rand((B, V), generator=g, device="cuda") < 0.2, steps, -math.inf)
+    many[1] = -math.inf
+    check_select(many, score, None, -1, keep, 1, B)
+    check_select(torch.arange(V, device="cuda").float().div(V / 8).repeat(B, 1), score, None, -1, keep, 1, B)
+    check_select(torch.arange(V, 0, -1, device="cuda").float().div(V / 8).repeat(B, 1), score, None, -1, keep, 1, B)
+
+
+def test_select_dead_beams_and_odd_values(cuda):
+    g = torch.Generator("cuda").manual_seed(9)
+    B, V = 4, 3000
+    logits = torch.empty((2 * B, V), device="cuda").normal_(generator=g)
+    score = torch.tensor([[0.0, -math.inf, -math.inf, -math.inf], [-2.0, -math.inf, -0.5, -1.0]], device="cuda")   # the first step of a search
+    check_select(logits, score, None, 7, 4, 2, B)
+    check_select(logits, score, torch.tensor([[1, 1, 0, 0], [0, 1, 1, 1]], dtype=torch.uint8, device="cuda"), 7, 8, 2, B)
+    logits[0, ::3] = math.nan
+    logits[5] = -math.inf
+    logits[6, 1] = -3e38
+    logits[7, 5] = 1e30
+    check_select(logits, score, None, 7, 4, 2, B)
+    logits[4, 9] = math.inf
+    check_select(logits, score, None, 7, 4, 2, B)
+
+
+def test_select_in_a_graph(cuda):
+    g = torch.Generator("cuda").manual_seed(10)
+    k, B, V = kernels(), 4, 9000
+    logits, score = torch.randn((B, V), generator=g, device="cuda"), torch.zeros((1, B), device="cuda")
+    out = [torch.zeros((1, B), dtype=torch.int32, device="cuda") for _ in range(2)] + [torch.zeros((1, B), device="cuda")]
+    scratch = torch.empty(k.beam_select_scratch_bytes(V, B, B, 1), dtype=torch.uint8, device="cuda")
+    call = lambda o: k.beam_select(o[0], o[1], o[2], None, logits, V, V, score, None, 0, B, B, 1, scratch)  # noqa: E731
+    call(out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(out)
+    for _ in range(3):
+        logits.normal_(generator=g)
+        graph.replay()
+        got = [o.clone() for o in out]
+        call(out)
+        assert all(torch.equal(a, b) for a, b in zip(got, out))
+
+
+# ------------------------------------------------------------------------------------------------------------------ moving rows
+@CACHES
+@pytest.mark.parametrize("M, B, layers, nkv, max_seq", [(1, 1, 1, 1, 5), (2, 4, 2, 3, 50), (1, 9, 3, 2, 130), (3, 32, 1, 1, 20), (2, 5, 2, 8, 700)])
+def test_reorder(cuda, M, B, layers, nkv, max_seq, coded):
+    g = torch.Generator("cuda").manual_seed(B)
+    st = Store(g, M * B, layers + 1, nkv, max_seq, coded)
+    for turn in range(3):
+        parent = torch.randint(-1, B + 1, (M, B), generator=g, device="cuda", dtype=torch.int32) if turn else torch.arange(B - 1, -1, -1, device="cuda", dtype=torch.int32).repeat(M, 1)
+        lo = ints([m % 3 for m in range(M)]) if turn else None
+        hi = ints([max_seq + 9 if m % 2 else max_seq - 2 - m for m in range(M)])
+        want = st.bits()
+        for w in want:
+            rows = w.view(M, B, layers + 1, nkv, max_seq, -1)
+            old = rows.clone()
+            for m in range(M):
+                for b in range(B):
+                    p = int(parent[m, b])
+                    a, z = (int(lo[m]) if lo is not None else 0), min(int(hi[m]), max_seq)
+                    if 0 <= p < B:
+                        rows[m, b, 1:, :, a:z] = old[m, p, 1:, :, a:z]
+        kernels().kv_reorder(st.args(1), parent, lo, hi, B, M, layers, st.plane)
+        assert all(torch.equal(a, b) for a, b in zip(want, st.bits()))
+
+
+@CACHES
+def test_reorder_of_nothing(cuda, coded):
+    st = Store(torch.Generator("cuda").manual_seed(1), 4, 1, 2, 30, coded)
+    before = st.bits()
+    kernels().kv_reorder(st.args(), ints([[1, 0], [1, 0]]), ints([9, -4]), ints([9, -1]), 2, 2, 1, st.plane)
+    kernels().kv_reorder(st.args(), ints([[0, 1], [0, 1]]), None, ints([30, 30]), 2, 2, 1, st.plane)
+    assert all(torch.equal(a, b) for a, b in zip(before, st.bits()))
+
+
+@CACHES
+@pytest.mark.parametrize("M, T, layers, nkv", [(1, 1, 1, 1), (1, 8, 5, 8), (3, 7, 2, 3), (5, 64, 2, 2), (2, 33, 3, 1)])
+def test_keep_rows(cuda, M, T, layers, nkv, coded):
+    g = torch.Generator("cuda").manual_seed(T)
+    max_seq = 2 * T + 6
+    st = Store(g, M, layers + 1, nkv, max_seq, coded)
+    for turn in range(4):
+        path = torch.randint(-1 if turn else 0, T + (1 if turn else 0), (M, T), generator=g, device="cuda", dtype=torch.int32)
+        if turn == 0:
+            path = path.sort(1).values.int()
+        first = [(3, -1, T + 4, 0, 2 ** 31 - 1)[(m + turn) % 5] for m in range(M)]
+        count = [(T, T // 2, T + 5, -1, 1)[(m + turn) % 5] for m in range(M)]
+        want = st.bits()
+        for w in want:
+            rows = w.view(M, layers + 1, nkv, max_seq, -1)
+            old = rows.clone()
+            for m in range(M):
+                for i in range(min(T, count[m])):
+                    p = int(path[m, i])
+                    if first[m] >= 0 and 0 <= p < T and first[m] + max(p, i) < max_seq:
+                        rows[m, 1:, :, first[m] + i] = old[m, 1:, :, first[m] + p]
+        kernels().kv_keep_rows(st.args(1), ints(first), path, ints(count), M, T, layers, st.plane)
+        assert all(torch.equal(a, b) for a, b in zip(want, st.bits()))
+
+
+# ------------------------------------------------------------------------------------------------------------------ together
+@CACHES
+def test_a_drafted_tree_is_verified_and_kept(cuda, coded):
+    """A prompt is written, a tree of six nodes drafted, attended and one path accepted; the next token's attention over what is kept has
+    the bits of one over a cache into which the path's tokens were written one after the other."""
+    g = torch.Generator("cuda").manual_seed(6)
+    k = kernels()
+    M, nq, nkv, max_seq, T, n = 2, 8, 2, 60, 6, [31, 17]
+    a, b = Store(g, M, 1, nkv, max_seq, coded), Store(g, M, 1, nkv, max_seq, coded, fill="nan")
+    b.k.copy_(a.k), b.v.copy_(a.v)
+    if coded:
+        b.ks.copy_(a.ks), b.vs.copy_(a.vs)
+    w = [torch.empty(HD, device="cuda").uniform_(0.5, 1.5, generator=g) for _ in range(2)]
+    prompt = torch.randn((M, 31, nq + 2 * nkv, HD), generator=g, device="cuda")
+    q = torch.empty((M, 31, nq, HD), device="cuda")
+    for st in (a, b):
+        k.qk_norm_rope_kv_rows(q, st.args(), prompt, w[0], w[1], ints([0, 0]), None, ints(n), nq, M, 31, 1e-6, 1e6)
+    depth = [[0, 1, 1, 2, 2, 3], [0, 0, 1, 1, 2, 3]]
+    masks = [[1, 3, 5, 11, 21, 43], [1, 2, 5, 10, 21, 53]]
+    path, count = [[0, 2, 4, 0, 0, 0], [0, 2, 4, 5, 0, 0]], [3, 4]
+    nodes = torch.randn((M, T, nq + 2 * nkv, HD), generator=g, device="cuda")
+    qt = torch.empty((M, T, nq, HD), device="cuda")
+    k.qk_norm_rope_kv_rows(qt, a.args(), nodes, w[0], w[1], ints(n), ints(depth), None, nq, M, T, 1e-6, 1e6)
+    check = torch.zeros((M, T, nq, HD), device="cuda")
+    k.attention_tree(check, qt, a.args(), ints(n), words(masks), None, 0, nq, M, T, None)
+    k.kv_keep_rows(a.args(), ints(n), ints(path), ints(count), M, T, 1, a.plane)
+    for i in range(4):   # the same tokens one by one; the first sequence has three
+        now = [n[0] + i if i < 3 else -1, n[1] + i]
+        one = torch.stack([nodes[0, path[0][min(i, 2)]], nodes[1, path[1][i]]])
+        q1, out = torch.zeros((M, nq, HD), device="cuda"), torch.zeros((M, nq, HD), device="cuda")
+        k.qk_norm_rope_kv_rows(q1, b.args(), one, w[0], w[1], ints(now), None, None, nq, M, 1, 1e-6, 1e6)
+        k.attention_tree(out, q1, b.args(), ints(now), None, None, 0, nq, M, 1, None)
+        for m in range(M):
+            if now[m] >= 0:   # (another order of the sums: 32-bit roundings)
+                assert torch.equal(q1[m], qt[m, path[m][i]])
+                assert torch.allclose(out[m], check[m, path[m][i]], rtol=0, atol=2.0 ** -17 * float(check.abs().max()))
+    for m in range(M):
+        end = n[m] + count[m]
+        assert torch.equal(a.k.view(torch.uint8)[m, 0, :, :end], b.k.view(torch.uint8)[m, 0, :, :end])
+    ends = [n[m] + count[m] for m in range(M)]
+    last = torch.randn((M, 1, nq + 2 * nkv, HD), generator=g, device="cuda")
+    outs = []
+    for st in (a, b):
+        q1, out = torch.empty((M, nq, HD), device="cuda"), torch.empty((M, nq, HD), device="cuda")
+        k.qk_norm_rope_kv_rows(q1, st.args(), last, w[0], w[1], ints(ends), None, None, nq, M, 1, 1e-6, 1e6)
+        k.attention_tree(out, q1, st.args(), ints(ends), None, None, 0, nq, M, 1, None)
+        outs.append(out)
+    assert torch.equal(*outs)
+
+
+def test_beams_share_a_prompt_and_part(cuda):
+    """Beams over one cache each: selection, reordering, the next row; every beam's cache is its parent's plus its own token."""
+    g = torch.Generator("cuda").manual_seed(7)
+    k = kernels()
+    B, nq, nkv, max_seq, V, L = 4, 4, 2, 40, 500, 2
+    st = Store(g, B, L, nkv, max_seq, True)
+    table = torch.randn((V, nq + 2 * nkv, HD), generator=g, device="cuda")
+    score = torch.tensor([[0.0, -math.inf, -math.inf, -math.inf]], device="cuda")
+    ended = torch.zeros((1, B), dtype=torch.uint8, device="cuda")
+    parent, token = torch.zeros((1, B), dtype=torch.int32, device="cuda"), torch.zeros((1, B), dtype=torch.int32, device="cuda")
+    scratch = torch.empty(k.beam_select_scratch_bytes(V, B, B, 1), dtype=torch.uint8, device="cuda")
+    tokens = [[] for _ in range(B)]
+    for step in range(6):
+        logits = torch.randn((B, V), generator=g, device="cuda")
+        k.beam_select(parent, token, score, ended, logits, V, V, score, ended, 3, B, B, 1, scratch)
+        k.kv_reorder(st.args(), parent, ints([10]), ints([10 + step]), B, 1, L, st.plane)
+        tokens = [tokens[int(parent[0, b])] + [int(token[0, b])] for b in range(B)]
+        for layer in range(L):
+            q = torch.empty((B, 1, nq, HD), device="cuda")
+            k.qk_norm_rope_kv_rows(q, st.args(layer), table[token[0].long()], None, None, ints([10 + step] * B), None, None, nq, B, 1, 1e-6, 1e4)
+    again = Store(g, B, L, nkv, max_seq, True)
+    for b in range(B):
+        rows = table[torch.tensor(tokens[b], device="cuda")]
+        q = torch.empty((1, 6, nq, HD), device="cuda")
+        one = Store(g, 1, 1, nkv, max_seq, True)
+        k.qk_norm_rope_kv_rows(q, one.args(), rows, None, None, ints([10]), None, None, nq, 1, 6, 1e-6, 1e4)
+        for layer in range(L):
+            assert torch.equal(one.k.view(torch.uint8)[0, 0, :, 10:16], st.k.view(torch.uint8)[b, layer, :, 10:16])
+            assert torch.equal(one.vs[0, 0, :, 10:16], st.vs[b, layer, :, 10:16])
+    del again
+
+
+# ------------------------------------------------------------------------------------------------------------------ refusals of the tensors
+def test_refused_tensors(cuda):
+    k = kernels()
+    st = Store(torch.Generator("cuda").manual_seed(8), 2, 1, 2, 16, True)
+    q = torch.zeros((2, 1, 4, HD), device="cuda")
+    with pytest.raises(ValueError):
+        k.KVCache(st.k, st.v, None, None, 2, 16, st.plane)
+    with pytest.raises(ValueError):
+        k.KVCache(st.k, st.v, st.ks[:1], st.vs, 2, 16, st.plane)
+    ok = (q, q, st.args(), ints([0, 0]), None, None, 0, 4, 2, 1, None)
+    k.attention_tree(*ok)
+    for i, bad in ((0, q[:1]), (0, q.half()), (1, q.transpose(0, 2)), (3, torch.zeros(2, device="cuda")), (3, torch.zeros(2, dtype=torch.int32)), (4, ints([0, 0])),
+                   (8, 3)):
+        with pytest.raises(ValueError):
+            k.attention_tree(*ok[:i], bad, *ok[i + 1:])
+    with pytest.raises(k.KernelError):
+        k.attention_tree(q, q, st.args(), ints([0, 0]), None, None, 0, 3, 2, 1, None)
+    with pytest.raises(ValueError):
+        k.kv_reorder(st.args(), ints([0, 0, 0]), None, ints([4]), 3, 1, 1, st.plane)
