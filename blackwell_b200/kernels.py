@@ -316,7 +316,7 @@ class KVCache:
             raise ValueError("contiguous tensors of one device")
         if k.numel() != v.numel() or (coded and any(s.dtype != torch.float32 or s.numel() * 128 != k.numel() for s in (k_scale, v_scale))):
             raise ValueError("k, v and their scales (fp32, one per row of 128) have the same rows")
-        self.tensors, self.device, self.rows = tuple(sides), k.device, k.numel() // 128
+        self.tensors, self.index, self.rows = tuple(sides), k.get_device(), k.numel() // 128
         self.kv_heads, self.max_seq, self.batch_elems, self.layer_elems = kv_heads, max_seq, batch_elems, layer_elems
         self._args = _KVCacheArgs(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if coded else None, v_scale.data_ptr() if coded else None,
                                   kv_heads, max_seq, batch_elems, layer_elems)
@@ -327,25 +327,26 @@ class KVCache:
         last = (sequences - 1) * self.batch_elems + self.layer_elems + (layers - 1) * layer_stride
         if sequences < 1 or layers < 1 or last // 128 + self.kv_heads * self.max_seq > self.rows:
             raise ValueError(f"{name}: the cache has {self.rows} rows; {sequences} sequences and {layers} layers reach past them")
-        if self.device.index != torch.cuda.current_device():
-            raise ValueError(f"{name}: the cache is on {self.device}, not on the current device")
+        if self.index != torch.cuda.current_device():
+            raise ValueError(f"{name}: the cache is on device {self.index}, not on the current one")
 
 
-def _t(name, t, device, count, *dtypes):
-    """Pointer of an optional tensor of at least ``count`` elements on the call's device."""
+def _t(name, t, device, count, dtype, other=None):
+    """Pointer of an optional tensor of at least ``count`` elements on CUDA device number ``device``."""
     if t is None:
         return None
-    if t.dtype not in dtypes or t.device != device or t.numel() < count or not t.is_contiguous():
-        raise ValueError(f"{name}: wants a contiguous tensor of {count} x {dtypes[0]} on {device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
-    return t.data_ptr()
+    if (t.dtype is dtype or t.dtype is other) and t.get_device() == device and t.numel() >= count and t.is_contiguous():
+        return t.data_ptr()
+    raise ValueError(f"{name}: wants a contiguous tensor of {count} x {dtype} on device {device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
 
 
-def _q(stream):
-    return (torch.cuda.current_stream() if stream is None else stream).cuda_stream
+def _q(device, stream):
+    """The stream's handle, or that of the device's current stream (without the object that torch makes of it)."""
+    return torch._C._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream
 
 
 _ACT = (torch.float32, torch.bfloat16)
-_FLAG = (torch.uint8, torch.bool)
+_I32, _F32, _U8 = torch.int32, torch.float32, torch.uint8
 _vp, _i, _sz = C.c_void_p, C.c_int, C.c_size_t
 _L.bw_qk_norm_rope_kv_rows.argtypes = [_vp] * 8 + [_i] * 3 + [C.c_float] * 2 + [_i, _vp]
 _L.bw_attention_tree.argtypes = [_vp] * 6 + [_i] * 5 + [_vp, _sz, _vp]
@@ -358,28 +359,28 @@ _L.bw_kv_keep_rows.argtypes = [_vp] * 4 + [_i] * 3 + [_sz, _vp]
 
 def qk_norm_rope_kv_rows(q_out, cache, qkv, q_norm_w, k_norm_w, d_first_row, d_offset, d_count, num_q_heads, M, T, eps, rope_base, stream=None):
     """Head norm, rotation and (quantised) cache rows of T tokens or tree nodes of each sequence (bw_qk_norm_rope_kv_rows)."""
-    name, dev, act = "qk_norm_rope_kv_rows", cache.device, qkv.dtype
+    name, dev, act = "qk_norm_rope_kv_rows", cache.index, qkv.dtype
     if act not in _ACT:
         raise ValueError(f"{name}: activations are float32 or bfloat16")
     cache._check(name, M)
     _chk(name, _L.bw_qk_norm_rope_kv_rows(
         _t(name, q_out, dev, M * T * num_q_heads * 128, act), cache._ref, _t(name, qkv, dev, M * T * (num_q_heads + 2 * cache.kv_heads) * 128, act),
-        _t(name, q_norm_w, dev, 128, torch.float32), _t(name, k_norm_w, dev, 128, torch.float32), _t(name, d_first_row, dev, M, torch.int32),
-        _t(name, d_offset, dev, M * T, torch.int32), _t(name, d_count, dev, M, torch.int32), num_q_heads, M, T, eps, rope_base,
-        act == torch.bfloat16, _q(stream)))
+        _t(name, q_norm_w, dev, 128, _F32), _t(name, k_norm_w, dev, 128, _F32), _t(name, d_first_row, dev, M, _I32),
+        _t(name, d_offset, dev, M * T, _I32), _t(name, d_count, dev, M, _I32), num_q_heads, M, T, eps, rope_base,
+        act == torch.bfloat16, _q(dev, stream)))
 
 
 def attention_tree(out, q, cache, d_first_row, d_mask, d_count, ctx_hint, num_q_heads, M, T, scratch, stream=None):
     """Attention of single tokens (T == 1) or tree nodes over a binary16 or e4m3 cache (bw_attention_tree); ``d_mask`` int64 or uint64 [M][T]."""
-    name, dev, act = "attention_tree", cache.device, q.dtype
+    name, dev, act = "attention_tree", cache.index, q.dtype
     if act not in _ACT:
         raise ValueError(f"{name}: activations are float32 or bfloat16")
     cache._check(name, M)
     n = M * T * num_q_heads * 128
     _chk(name, _L.bw_attention_tree(
-        _t(name, out, dev, n, act), _t(name, q, dev, n, act), cache._ref, _t(name, d_first_row, dev, M, torch.int32),
-        _t(name, d_mask, dev, M * T, torch.int64, torch.uint64), _t(name, d_count, dev, M, torch.int32), ctx_hint, num_q_heads, M, T,
-        act == torch.bfloat16, _t(name, scratch, dev, 0, torch.uint8), scratch.numel() if scratch is not None else 0, _q(stream)))
+        _t(name, out, dev, n, act), _t(name, q, dev, n, act), cache._ref, _t(name, d_first_row, dev, M, _I32),
+        _t(name, d_mask, dev, M * T, torch.int64, torch.uint64), _t(name, d_count, dev, M, _I32), ctx_hint, num_q_heads, M, T,
+        act == torch.bfloat16, _t(name, scratch, dev, 0, _U8), scratch.numel() if scratch is not None else 0, _q(dev, stream)))
 
 
 def attention_tree_scratch_bytes(M, T, num_q_heads, num_kv_heads, max_context) -> int:
@@ -388,14 +389,12 @@ def attention_tree_scratch_bytes(M, T, num_q_heads, num_kv_heads, max_context) -
 
 def beam_select(parent_out, token_out, score_out, ended_out, logits, row_stride, vocab, score, ended, eos_id, beams, keep, M, scratch, stream=None):
     """The best ``keep`` continuations of each request's beams (bw_beam_select)."""
-    name, dev, n, rows = "beam_select", logits.device, M * keep, M * beams
-    if dev.index != torch.cuda.current_device():
-        raise ValueError(f"{name}: the logits are on {dev}, not on the current device")
+    name, dev, n, rows = "beam_select", torch.cuda.current_device(), M * keep, M * beams
     _chk(name, _L.bw_beam_select(
-        _t(name, parent_out, dev, n, torch.int32), _t(name, token_out, dev, n, torch.int32), _t(name, score_out, dev, n, torch.float32),
-        _t(name, ended_out, dev, n, *_FLAG), _t(name, logits, dev, (rows - 1) * row_stride + vocab, torch.float32), row_stride, vocab,
-        _t(name, score, dev, rows, torch.float32), _t(name, ended, dev, rows, *_FLAG), eos_id, beams, keep, M,
-        _t(name, scratch, dev, 0, torch.uint8), scratch.numel() if scratch is not None else 0, _q(stream)))
+        _t(name, parent_out, dev, n, _I32), _t(name, token_out, dev, n, _I32), _t(name, score_out, dev, n, _F32),
+        _t(name, ended_out, dev, n, _U8, torch.bool), _t(name, logits, dev, (rows - 1) * row_stride + vocab, _F32), row_stride, vocab,
+        _t(name, score, dev, rows, _F32), _t(name, ended, dev, rows, _U8, torch.bool), eos_id, beams, keep, M,
+        _t(name, scratch, dev, 0, _U8), scratch.numel() if scratch is not None else 0, _q(dev, stream)))
 
 
 def beam_select_scratch_bytes(vocab, beams, keep, M) -> int:
@@ -404,15 +403,15 @@ def beam_select_scratch_bytes(vocab, beams, keep, M) -> int:
 
 def kv_reorder(cache, d_parent, d_from, d_to, beams, M, layers, layer_stride_elems, stream=None):
     """Rows [from, to) of each beam from its parent, in place (bw_kv_reorder)."""
-    name, dev = "kv_reorder", cache.device
+    name, dev = "kv_reorder", cache.index
     cache._check(name, M * beams, layers, layer_stride_elems)
-    _chk(name, _L.bw_kv_reorder(cache._ref, _t(name, d_parent, dev, M * beams, torch.int32), _t(name, d_from, dev, M, torch.int32),
-                                _t(name, d_to, dev, M, torch.int32), beams, M, layers, layer_stride_elems, _q(stream)))
+    _chk(name, _L.bw_kv_reorder(cache._ref, _t(name, d_parent, dev, M * beams, _I32), _t(name, d_from, dev, M, _I32),
+                                _t(name, d_to, dev, M, _I32), beams, M, layers, layer_stride_elems, _q(dev, stream)))
 
 
 def kv_keep_rows(cache, d_first_row, d_path, d_count, M, T, layers, layer_stride_elems, stream=None):
     """Accepted nodes of a tree moved together, in place (bw_kv_keep_rows)."""
-    name, dev = "kv_keep_rows", cache.device
+    name, dev = "kv_keep_rows", cache.index
     cache._check(name, M, layers, layer_stride_elems)
-    _chk(name, _L.bw_kv_keep_rows(cache._ref, _t(name, d_first_row, dev, M, torch.int32), _t(name, d_path, dev, M * T, torch.int32),
-                                  _t(name, d_count, dev, M, torch.int32), M, T, layers, layer_stride_elems, _q(stream)))
+    _chk(name, _L.bw_kv_keep_rows(cache._ref, _t(name, d_first_row, dev, M, _I32), _t(name, d_path, dev, M * T, _I32),
+                                  _t(name, d_count, dev, M, _I32), M, T, layers, layer_stride_elems, _q(dev, stream)))
