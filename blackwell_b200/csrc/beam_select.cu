@@ -1,25 +1,35 @@
 // Beam search's selection: of the candidates  score[b] + log_softmax(logits[b])[v]  of a request's beams the best few.
 //
-// Two launches.  The first reads the logits once, a chunk of a row per block: the chunk's maximum and sum of exponentials, and its
-// `keep` largest logits (within a row the order of the candidates is that of the logits).  The second, a block per request, forms the
-// rows' log-sums and compares the chunks' candidates across the beams.  Log-sums, scores and comparisons are in 64 bits: two beams'
-// candidates may lie closer to each other than 32 bits tell apart.
-//
-// Both find the best K of n values without sorting: the n values are dealt to K or more groups of threads, and the smallest of the
-// groups' maxima has at least K values at or above it.  Some K (ln K + 1) values pass that bar; they are gathered and ranked by
-// counting.  Where more pass than the list holds (many equal values), K rounds of a block-wide maximum take over.
+// Two launches.  The first reads the logits once, a stretch of a row per block, 4,096 values at a time with the next ones in flight.  A
+// warp works by itself: running maxima and sums of exponentials per lane, and a list of the values that may be among the `keep` largest of
+// the stretch (within a row the order of the candidates is that of the logits).  What enters the list is at or above a bar: the
+// smallest of the running maxima of `keep` or more groups of the block's threads.  At least `keep` values lie there, of the first n some keep *
+// (ln keep + 1), so that after the first turns hardly a warp has one.  The maxima only grow, so that warps share them without waiting for
+// each other: a stale one lowers the bar.  A list that has grown is cut to its best.  The second launch, a block per request, forms the rows' log-sums and ranks the
+// stretches' candidates across the beams, scores in 64 bits: two beams' candidates may lie closer to each other than 32 bits tell apart.
+// The exponentials are 32-bit, taken of differences that are exact where they matter; their roundings average out in the sum.  64-bit exp
+// and log are avoided: a chain of some 300 64-bit instructions took the merge 5 us.
 #include <float.h>
 
 #include "common.cuh"
 #include "host_util.h"
 #include "kv_cache.cuh"
+#include "lm_device.cuh"
 
 namespace bw {
 namespace beam {
 
+using lm::exp2_fast;
+
+constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kMaxKeep = 64, kMaxBeams = 64;
-constexpr int kList = 512;              // candidates that are ranked at once
+constexpr int kVec = 4;                       // 16-byte vectors of a thread in flight
+constexpr int kTurn = kThreads * kVec;        // vectors a block takes at once
+constexpr int kGrown = 128;                   // entries from which a warp's list is cut to the best
+constexpr int kList = kGrown + 32 * 4 * kVec; // ... and one turn that enters whole
+constexpr int kStaged = 4096;                 // candidates of a request that the merge holds in shared memory
+constexpr int kMaxLists = 64 * kWarps;        // stretches of a request's beams, at most: two per lane of the merge's warps
 
 struct Args {
     int *parent, *token;
@@ -30,7 +40,7 @@ struct Args {
     int vocab;
     const float* score;
     const unsigned char* ended;
-    int eos, beams, keep, M, chunks, chunk;
+    int eos, beams, keep, M, chunks, chunk;     // stretches of a row, their length in vectors
     float2* sums;                       // [M * beams][chunks] maximum, sum of exponentials relative to it
     unsigned long long* best;           // [M * beams][chunks][keep] keys, largest first; 0: none
 };
@@ -43,245 +53,323 @@ __device__ __forceinline__ float order32_value(uint32_t k) { return __uint_as_fl
 // Larger value first, then the lower index.
 __device__ __forceinline__ unsigned long long key_of(float v, uint32_t index) { return (unsigned long long)order32(v) << 32 | (0xFFFFFFFFu - index); }
 
+// A candidate of the merge: its score as an integer that orders as the score does (64-bit comparisons of floats have a long latency; ranking
+// is a chain of them), 0: none.
 struct Cand {
-    double score;
+    unsigned long long score;
     uint32_t at;                        // beam * vocab + token
 };
+__device__ __forceinline__ unsigned long long order64(double d) {
+    const unsigned long long b = (unsigned long long)__double_as_longlong(d);
+    return b >> 63 ? ~b : b | 1ull << 63;
+}
+__device__ __forceinline__ double order64_value(unsigned long long k) { return __longlong_as_double((long long)(k >> 63 ? k & ~(1ull << 63) : ~k)); }
 __device__ __forceinline__ bool before(const Cand& a, const Cand& b) { return a.score > b.score || (a.score == b.score && a.at < b.at); }
 
-// Groups of 2^s neighbouring threads, at least `keep` of them: how many threads a group has.
-__device__ __forceinline__ int group_size(int keep) {
-    int n = kThreads;
-    while (kThreads / n < keep) n >>= 1;
-    return n;
+__device__ __forceinline__ unsigned long long pair_of(float lo, float hi) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ unsigned long long warp_max_key(unsigned long long k) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const unsigned long long q = __shfl_xor_sync(0xffffffffu, k, o);
+        k = q > k ? q : k;
+    }
+    return k;
+}
+// The best `keep` of the warp's n keys to the front of its list, largest first; zeros where there are fewer.
+__device__ __forceinline__ void cut_list(unsigned long long* list, int n, int keep, int lane) {
+    unsigned long long last = ~0ull, mine[2] = {0, 0};
+    __syncwarp();
+    for (int r = 0; r < keep; ++r) {
+        unsigned long long k = 0;
+        for (int i = lane; i < n; i += 32) {
+            const unsigned long long q = list[i];
+            if (q < last && q > k) k = q;
+        }
+        last = warp_max_key(k);
+        if ((r & 31) == lane) mine[r >> 5] = last;
+        if (last == 0) break;
+    }
+    __syncwarp();
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+        if (lane + 32 * e < keep) list[lane + 32 * e] = mine[e];
+    __syncwarp();
 }
 
-// PER values of a thread in registers.
-template <int PER>
-__global__ void __launch_bounds__(kThreads) chunk_kernel(const Args a) {
-    __shared__ float s_f[kWarps];
-    __shared__ float s_max[kWarps];
-    __shared__ unsigned long long s_list[kList];
-    __shared__ int s_n;
+// Sum of exp(v - to) over a thread's values, two at a time.
+__device__ __forceinline__ float exponentials(const float4 (&v)[kVec], float to) {
+    unsigned long long part[2];
+    const unsigned long long minus = pair_of(-to, -to), scale = pair_of(kLog2e, kLog2e);
+#pragma unroll
+    for (int j = 0; j < kVec; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            unsigned long long d;
+            asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(e ? pair_of(v[j].z, v[j].w) : pair_of(v[j].x, v[j].y)), "l"(minus));
+            asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(d) : "l"(scale));
+            float lo, hi;
+            asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(d));
+            const unsigned long long x = pair_of(exp2_fast(lo), exp2_fast(hi));
+            if (j == 0) part[e] = x;
+            else asm("add.rn.f32x2 %0, %0, %1;" : "+l"(part[e]) : "l"(x));
+        }
+    float p[4];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) asm("mov.b64 {%0, %1}, %2;" : "=f"(p[2 * e]), "=f"(p[2 * e + 1]) : "l"(part[e]));
+    return (p[0] + p[1]) + (p[2] + p[3]);
+}
+
+__global__ void __launch_bounds__(kThreads, 3) chunk_kernel(const Args a) {
+    __shared__ unsigned long long s_list[kWarps][kList], s_all[kWarps * kMaxKeep];
+    __shared__ float s_f[kWarps], s_g[kWarps];
+    __shared__ uint32_t s_group[64];
+    __shared__ int s_n[kWarps];
+    const int c = blockIdx.x, row = blockIdx.y, t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const float* x = a.logits + (size_t)row * a.row_stride;
+    const int skew = (int)(reinterpret_cast<uintptr_t>(x) >> 2 & 3);     // vector q: elements 4 q - skew ...
+    const int q0 = c * a.chunk, q1 = min(q0 + a.chunk, (a.vocab + skew + 3) / 4);
     pdl_trigger();
     pdl_wait();
-    const int c = blockIdx.x, row = blockIdx.y, t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    const int v0 = c * a.chunk, n = min(a.vocab - v0, a.chunk);
-    const float* x = a.logits + (size_t)row * a.row_stride + v0;
-    if (t == 0) s_n = 0;
-    float v[PER];
+    auto load = [&](int base, float4 (&v)[kVec]) {
+        if (4 * base >= skew && 4 * (base + kTurn) - skew <= a.vocab && base + kTurn <= q1) {
+            const float4* p = reinterpret_cast<const float4*>(x - skew) + base + t;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-        const int i = t + kThreads * j;
-        v[j] = i < n ? fmaxf(x[i], -INFINITY) : -INFINITY;     // (NaN: -inf)
-    }
-    float top = -INFINITY;
+            for (int j = 0; j < kVec; ++j) v[j] = p[kThreads * j];
+            return;
+        }
 #pragma unroll
-    for (int j = 0; j < PER; ++j) top = fmaxf(top, v[j]);
-    // the bar: the least of the groups' maxima
-    const int gs = group_size(a.keep);
-    float gm = top;
-    for (int o = 1; o < min(gs, 32); o <<= 1) gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, o));
-    float wmax = warp_max(top), wmin = -warp_max(-gm);
-    if (lane == 0) { s_max[warp] = wmax; s_f[warp] = wmin; }
+        for (int j = 0; j < kVec; ++j) {                                 // a row's ends
+            const int q = base + kThreads * j + t, i = 4 * q - skew;
+            float e[4];
+#pragma unroll
+            for (int d = 0; d < 4; ++d) e[d] = q < q1 && i + d >= 0 && i + d < a.vocab ? x[i + d] : -INFINITY;
+            v[j] = make_float4(e[0], e[1], e[2], e[3]);
+        }
+    };
+    float4 next[kVec];
+    load(q0, next);
+    if (t < 64) s_group[t] = 0;                                          // (below every value)
+    if (t < kWarps) s_n[t] = 0;
     __syncthreads();
-    float bmax = s_max[0], bar = INFINITY;
+    unsigned long long* list = s_list[warp];
+    float m[2] = {-INFINITY, -INFINITY}, sum = 0.f, ground = -FLT_MAX;     // maxima of the lane's even and odd vectors
+    int groups = 1;
+    while (groups < a.keep) groups <<= 1;
+    for (int base = q0; base < q1; base += kTurn) {
+        float4 v[kVec];
 #pragma unroll
-    for (int w = 1; w < kWarps; ++w) bmax = fmaxf(bmax, s_max[w]);
-    if (gs <= 32) {
+        for (int j = 0; j < kVec; ++j) v[j] = next[j];
+        if (base + kTurn < q1) load(base + kTurn, next);
+        const float old = fmaxf(m[0], m[1]);
+        float top[2] = {-INFINITY, -INFINITY};                           // (a NaN is no maximum)
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) bar = fminf(bar, s_f[w]);
-    } else {
-        for (int w = 0; w < kWarps; w += gs / 32) {
-            float g = s_max[w];
-            for (int e = 1; e < gs / 32; ++e) g = fmaxf(g, s_max[w + e]);
-            bar = fminf(bar, g);
+        for (int j = 0; j < kVec; ++j) top[j & 1] = fmaxf(top[j & 1], fmaxf(fmaxf(v[j].x, v[j].y), fmaxf(v[j].z, v[j].w)));
+        m[0] = fmaxf(m[0], top[0]);
+        m[1] = fmaxf(m[1], top[1]);
+        const float to = fmaxf(m[0], m[1]), best = fmaxf(top[0], top[1]);
+        if (to > -INFINITY) {
+            const float kept = sum * exp2_fast((old - to) * kLog2e);
+            sum = kept + exponentials(v, to);
+            if (sum != sum) {                                            // a NaN counts as -inf (and +inf leaves NaN here)
+#pragma unroll
+                for (int j = 0; j < kVec; ++j)
+                    v[j] = make_float4(fmaxf(v[j].x, -INFINITY), fmaxf(v[j].y, -INFINITY), fmaxf(v[j].z, -INFINITY), fmaxf(v[j].w, -INFINITY));
+                sum = kept + exponentials(v, to);
+            }
+        }
+        // group (thread mod G), or with G = 64 (lane) and (32 + lane) of the lanes' two maxima
+        uint32_t low;
+        if (groups > 32) {
+            const uint32_t g0 = atomicMax(&s_group[lane], order32(m[0])), g1 = atomicMax(&s_group[32 + lane], order32(m[1]));
+            low = min(max(g0, order32(m[0])), max(g1, order32(m[1])));
+        } else {
+            float g = to;
+            for (int o = 16; o >= groups; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+            low = order32(g);
+            if (lane < groups) low = max(low, atomicMax(&s_group[lane], low));
+        }
+        const float bar = order32_value(__reduce_min_sync(0xffffffffu, groups > 32 || lane < groups ? low : 0xFFFFFFFFu));
+        const float in = fmaxf(bar, ground);
+        if (__any_sync(0xffffffffu, best >= in)) {
+            const uint32_t i0 = (uint32_t)(4 * (base + t) - skew);
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) {
+                const float e[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+#pragma unroll
+                for (int d = 0; d < 4; ++d)
+                    if (e[d] >= in) list[atomicAdd(&s_n[warp], 1)] = key_of(e[d], i0 + 4 * kThreads * j + d);
+            }
+            __syncwarp();
+            const int n = *reinterpret_cast<volatile int*>(&s_n[warp]);
+            __syncwarp();
+            if (n > kGrown) {
+                cut_list(list, n, a.keep, lane);
+                ground = order32_value((uint32_t)(list[a.keep - 1] >> 32) + 1);   // the next float: what equals the last one comes too late
+                if (lane == 0) s_n[warp] = a.keep;
+                __syncwarp();
+            }
         }
     }
-    __syncthreads();
-    float sum = 0.f;
-    if (bmax > -INFINITY) {
-#pragma unroll
-        for (int j = 0; j < PER; ++j) sum += __expf(v[j] - bmax);
+    // the block's maximum and sum, and the best of the warps' lists
+    const float mine = fmaxf(m[0], m[1]), wm = warp_max(mine);
+    if (lane == 0) s_g[warp] = wm;
+    __syncwarp();
+    int n = s_n[warp];
+    if (__syncthreads_or(n > kMaxKeep)) {
+        if (n > a.keep) cut_list(list, n, a.keep, lane);
+        n = min(n, a.keep);
+        if (lane == 0) s_n[warp] = n;
+        __syncthreads();
     }
-    sum = warp_sum(sum);
+    float top = s_g[0];
+    int all = 0, at = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        top = fmaxf(top, s_g[w]);
+        at = w == warp ? all : at;
+        all += s_n[w];
+    }
+    sum = warp_sum(mine > -INFINITY ? sum * exp2_fast((mine - top) * kLog2e) : 0.f);
     if (lane == 0) s_f[warp] = sum;
-    // what passes the bar
-#pragma unroll
-    for (int j = 0; j < PER; ++j)
-        if (v[j] >= bar && v[j] > -INFINITY) {
-            const int k = atomicAdd(&s_n, 1);
-            if (k < kList) s_list[k] = key_of(v[j], v0 + t + kThreads * j);
-        }
+    for (int i = lane; i < n; i += 32) s_all[at + i] = list[i];
     __syncthreads();
     const size_t rec = (size_t)row * a.chunks + c;
-    if (t == 0) {
-        float all = 0.f;
-        for (int w = 0; w < kWarps; ++w) all += s_f[w];
-        a.sums[rec] = make_float2(bmax, all);
-    }
     unsigned long long* out = a.best + rec * a.keep;
-    const int got = s_n;
-    if (got <= kList) {
-        for (int i = t; i < got; i += kThreads) {
-            const unsigned long long k = s_list[i];
-            int rank = 0;
-            for (int j = 0; j < got; ++j) rank += s_list[j] > k;
-            if (rank < a.keep) out[rank] = k;
-        }
-        for (int i = got + t; i < a.keep; i += kThreads) out[i] = 0;
-        return;
+    for (int i = t; i < all; i += kThreads) {
+        const unsigned long long k = s_all[i];
+        int rank = 0;
+#pragma unroll 4
+        for (int j = 0; j < all; ++j) rank += s_all[j] > k;
+        if (rank < a.keep) out[rank] = k;
     }
-    unsigned long long last = ~0ull;
-    for (int r = 0; r < a.keep; ++r) {
-        unsigned long long k = 0;
+    if (t >= all && t < a.keep) out[t] = 0;
+    if (t == 0) {
+        float whole = 0.f;
 #pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const unsigned long long q = key_of(v[j], v0 + t + kThreads * j);
-            if (v[j] > -INFINITY && q < last && q > k) k = q;
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const unsigned long long q = __shfl_xor_sync(0xffffffffu, k, o);
-            k = q > k ? q : k;
-        }
-        __syncthreads();
-        if (lane == 0) s_list[warp] = k;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) k = s_list[w] > k ? s_list[w] : k;
-        if (t == 0) out[r] = k;
-        last = k;                                              // (0 once there are no more)
+        for (int w = 0; w < kWarps; ++w) whole += s_f[w];
+        a.sums[rec] = make_float2(top, whole);
     }
+}
+
+// The best of up to 64 sorted lists, two per lane, one after the other: head(l, i) is entry i of list l (score 0: none), emit(r, cand)
+// takes the r-th best, by the lane that holds it.  A round is three warp-wide integer reductions; only the winner's list moves on.
+template <typename Head, typename Emit>
+__device__ __forceinline__ void tournament(int lists, int keep, int lane, const Head& head, const Emit& emit) {
+    Cand x[2];
+    int i[2] = {0, 0};
+#pragma unroll
+    for (int e = 0; e < 2; ++e) x[e] = lane + 32 * e < lists ? head(lane + 32 * e, 0) : Cand{0, 0};
+    for (int r = 0; r < keep; ++r) {
+        const int e = before(x[1], x[0]);
+        const Cand y = e ? x[1] : x[0];
+        const uint32_t hi = (uint32_t)(y.score >> 32), lo = (uint32_t)y.score;
+        const uint32_t mhi = __reduce_max_sync(0xffffffffu, hi);
+        const uint32_t mlo = __reduce_max_sync(0xffffffffu, hi == mhi ? lo : 0u);
+        const bool tied = hi == mhi && lo == mlo;
+        const uint32_t at = __reduce_min_sync(0xffffffffu, tied ? y.at : 0xFFFFFFFFu);
+        if (mhi == 0 && mlo == 0) {
+            if (lane == 0)
+                for (; r < keep; ++r) emit(r, Cand{0, 0});
+            break;
+        }
+        if (tied && y.at == at) {
+            emit(r, y);
+            if (e) x[1] = ++i[1] < keep ? head(lane + 32, i[1]) : Cand{0, 0};
+            else x[0] = ++i[0] < keep ? head(lane, i[0]) : Cand{0, 0};
+        }
+    }
+    __syncwarp();
 }
 
 __global__ void __launch_bounds__(kThreads) merge_kernel(const Args a) {
     __shared__ double s_lse[kMaxBeams];
     __shared__ float s_score[kMaxBeams];
     __shared__ unsigned char s_ended[kMaxBeams];
-    __shared__ Cand s_list[kList];
-    __shared__ Cand s_w[kWarps];
-    __shared__ double s_max[kWarps], s_min[kWarps];
-    __shared__ int s_n;
+    __shared__ unsigned long long s_key[kStaged];
+    __shared__ Cand s_best[kWarps][kMaxKeep];
+    const int m = blockIdx.x, t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const int lists = a.beams * a.chunks, total = lists * a.keep;
+    const unsigned long long* best = a.best + (size_t)m * total;
     pdl_trigger();
     pdl_wait();
-    const int m = blockIdx.x, t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    if (t == 0) s_n = 0;
+    const bool staged = total <= kStaged;
+    if (staged)
+        for (int i = t; i < total; i += kThreads) s_key[i] = best[i];
     for (int b = warp; b < a.beams; b += kWarps) {
         const float2* rec = a.sums + ((size_t)m * a.beams + b) * a.chunks;
-        float mx = -INFINITY;
-        for (int c = lane; c < a.chunks; c += 32) mx = fmaxf(mx, rec[c].x);
+        const float2 one = lane < a.chunks ? rec[lane] : make_float2(-INFINITY, 0.f);
+        float mx = one.x;
+        for (int c = lane + 32; c < a.chunks; c += 32) mx = fmaxf(mx, rec[c].x);
         mx = warp_max(mx);
-        double sum = 0.0;
-        for (int c = lane; c < a.chunks; c += 32) {
+        float sum = one.x > -INFINITY ? one.y * exp2f((one.x - mx) * kLog2e) : 0.f;
+        for (int c = lane + 32; c < a.chunks; c += 32) {
             const float2 r = rec[c];
-            if (r.x > -INFINITY) sum += (double)r.y * exp((double)r.x - (double)mx);
+            if (r.x > -INFINITY) sum += r.y * exp2f((r.x - mx) * kLog2e);
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        sum = warp_sum(sum);
         if (lane == 0) {
-            s_lse[b] = (double)mx + log(sum);
+            // log sum = k ln 2 + log of what is left, which lies in [1, 2): its 32-bit rounding is under 2^-24
+            int k = 0;
+            float left = sum;
+            if (sum >= 1.f && sum < INFINITY) {
+                k = (int)(__float_as_uint(sum) >> 23) - 127;
+                left = __uint_as_float((__float_as_uint(sum) & 0x7FFFFFu) | 0x3F800000u);
+            }
+            s_lse[b] = (double)mx + fma((double)k, 0.6931471805599453, (double)logf(left));
             s_score[b] = a.score[m * a.beams + b];
             s_ended[b] = a.ended ? a.ended[m * a.beams + b] : 0;
         }
     }
     __syncthreads();
-    const int per_beam = a.chunks * a.keep, total = a.beams * per_beam;
-    const unsigned long long* best = a.best + (size_t)m * total;
-    // Candidate number i; score -inf: none.
-    auto cand = [&](int i) {
-        const int b = i / per_beam;
-        Cand x{-INFINITY, 0xFFFFFFFFu};
+    // Entry i of list l (a beam's stretch); an ended beam has one, its first stretch's.
+    auto head = [&](int l, int i) {
+        const int b = l / a.chunks;
+        Cand x{0, 0};
         if (s_ended[b]) {
-            if (i == b * per_beam && s_score[b] > -INFINITY) x = Cand{(double)s_score[b], (uint32_t)b * a.vocab + a.eos};
+            if (l == b * a.chunks && i == 0 && s_score[b] > -INFINITY) x = Cand{order64((double)s_score[b]), (uint32_t)b * a.vocab + a.eos};
             return x;
         }
-        const unsigned long long k = best[i];
+        const unsigned long long k = staged ? s_key[l * a.keep + i] : best[(size_t)l * a.keep + i];
         if (k == 0) return x;
         const double s = (double)s_score[b] + ((double)order32_value((uint32_t)(k >> 32)) - s_lse[b]);
-        if (s > -INFINITY) x = Cand{s, (uint32_t)b * a.vocab + (0xFFFFFFFFu - (uint32_t)k)};
+        if (s > -INFINITY) x = Cand{order64(s), (uint32_t)b * a.vocab + (0xFFFFFFFFu - (uint32_t)k)};
         return x;
     };
-    double top = -INFINITY;
-    for (int i = t; i < total; i += kThreads) top = fmax(top, cand(i).score);
-    const int gs = group_size(a.keep);
-    double gm = top, wmax = top;
-    for (int o = 1; o < min(gs, 32); o <<= 1) gm = fmax(gm, __shfl_xor_sync(0xffffffffu, gm, o));
-    double wmin = gm;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        wmax = fmax(wmax, __shfl_xor_sync(0xffffffffu, wmax, o));
-        wmin = fmin(wmin, __shfl_xor_sync(0xffffffffu, wmin, o));
-    }
-    if (lane == 0) { s_max[warp] = wmax; s_min[warp] = wmin; }
-    __syncthreads();
-    double bar = INFINITY;
-    if (gs <= 32) {
-        for (int w = 0; w < kWarps; ++w) bar = fmin(bar, s_min[w]);
-    } else {
-        for (int w = 0; w < kWarps; w += gs / 32) {
-            double g = s_max[w];
-            for (int e = 1; e < gs / 32; ++e) g = fmax(g, s_max[w + e]);
-            bar = fmin(bar, g);
-        }
-    }
-    for (int i = t; i < total; i += kThreads) {
-        const Cand x = cand(i);
-        if (x.score >= bar && x.score > -INFINITY) {
-            const int k = atomicAdd(&s_n, 1);
-            if (k < kList) s_list[k] = x;
-        }
-    }
-    __syncthreads();
-    const int got = s_n;
-    auto emit = [&](int r, const Cand& x) {
+    auto out = [&](int r, const Cand& x) {
         const size_t o = (size_t)m * a.keep + r;
-        const bool some = x.score > -INFINITY;
+        const bool some = x.score != 0;
         const int b = some ? (int)(x.at / (uint32_t)a.vocab) : -1, v = some ? (int)(x.at - (uint32_t)b * a.vocab) : -1;
         a.parent[o] = b;
         a.token[o] = v;
-        a.score_out[o] = (float)x.score;
+        a.score_out[o] = some ? (float)order64_value(x.score) : -INFINITY;
         if (a.ended_out) a.ended_out[o] = some && (s_ended[b] || v == a.eos);
     };
-    if (got <= kList) {
-        for (int i = t; i < got; i += kThreads) {
-            const Cand x = s_list[i];
-            int rank = 0;
-            for (int j = 0; j < got; ++j) rank += before(s_list[j], x);
-            if (rank < a.keep) emit(rank, x);
-        }
-        for (int i = got + t; i < a.keep; i += kThreads) emit(i, Cand{-INFINITY, 0xFFFFFFFFu});
+    if (lists <= 64) {
+        if (warp == 0) tournament(lists, a.keep, lane, head, out);
         return;
     }
-    Cand last{INFINITY, 0};
-    for (int r = 0; r < a.keep; ++r) {
-        Cand x{-INFINITY, 0xFFFFFFFFu};
-        for (int i = t; i < total; i += kThreads) {
-            const Cand y = cand(i);
-            if ((r == 0 || before(last, y)) && before(y, x)) x = y;
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const Cand y{__shfl_xor_sync(0xffffffffu, x.score, o), __shfl_xor_sync(0xffffffffu, x.at, o)};
-            if (before(y, x)) x = y;
-        }
-        __syncthreads();
-        if (lane == 0) s_w[warp] = x;
-        __syncthreads();
-        for (int w = 0; w < kWarps; ++w)
-            if (before(s_w[w], x)) x = s_w[w];
-        if (t == 0) emit(r, x);
-        last = x;
-    }
+    const int per = (lists + kWarps - 1) / kWarps, l0 = min(warp * per, lists);
+    tournament(min(per, lists - l0), a.keep, lane, [&](int l, int i) { return head(l0 + l, i); }, [&](int r, const Cand& x) { s_best[warp][r] = x; });
+    __syncthreads();
+    if (warp == 0) tournament(kWarps, a.keep, lane, [&](int l, int i) { return s_best[l][i]; }, out);
 }
 
-// Values of a chunk: 2,048 (eight a thread) where that leaves a few blocks per SM at most, else 8,192.
-static int chunk_of(int vocab, long rows) {
-    return rows * ((vocab + 2047) / 2048) <= 8L * sm_count(current_device()) ? 2048 : 8192;
+// Stretches of a row: whole turns, three blocks per SM where that many are to be had.
+static void stretches(int vocab, int beams, long rows, int sms, Args* a) {
+    const int turns = (vocab + 3 + 3) / 4 / kTurn + 1;
+    long n = 3L * sms / rows;
+    n = n > kMaxLists / beams ? kMaxLists / beams : n;
+    n = n < 1 ? 1 : n > turns ? turns : n;
+    a->chunk = (int)((turns + n - 1) / n) * kTurn;
+    a->chunks = ((vocab + 6) / 4 + a->chunk - 1) / a->chunk;
 }
 static size_t round16(size_t n) { return (n + 15) & ~(size_t)15; }
-static size_t bytes_of(long rows, int chunks, int keep) {
-    return round16((size_t)rows * chunks * sizeof(float2)) + (size_t)rows * chunks * keep * sizeof(unsigned long long);
+static size_t bytes_of(long records, int keep) {
+    return round16((size_t)records * sizeof(float2)) + (size_t)records * keep * sizeof(unsigned long long);
 }
 static bool sizes_ok(int vocab, int beams, int keep, int M) {
     return vocab >= 1 && beams >= 1 && beams <= kMaxBeams && keep >= 1 && keep <= kMaxKeep && M >= 1 && (long)M * beams <= 65535 &&
@@ -295,7 +383,8 @@ using namespace bw;
 
 extern "C" size_t bw_beam_select_scratch_bytes(int vocab, int beams, int keep, int M) {
     if (!beam::sizes_ok(vocab, beams, keep, M)) return 0;
-    return beam::bytes_of((long)M * beams, (vocab + 2047) / 2048, keep);
+    const long rows = (long)M * beams, most = 3L * sm_count(current_device());   // (records of any smaller call too)
+    return beam::bytes_of(rows > most ? rows : most, keep);
 }
 
 extern "C" int bw_beam_select(int* parent_out, int* token_out, float* score_out, unsigned char* ended_out_or_null, const float* logits,
@@ -305,9 +394,8 @@ extern "C" int bw_beam_select(int* parent_out, int* token_out, float* score_out,
     if (row_stride < vocab || (ended_or_null && (eos_id < 0 || eos_id >= vocab)) || !kv::aligned(scratch, 16)) return cudaErrorInvalidValue;
     const long rows = (long)M * beams;
     beam::Args a{};
-    a.chunk = beam::chunk_of(vocab, rows);
-    a.chunks = (vocab + a.chunk - 1) / a.chunk;
-    if (scratch_bytes < beam::bytes_of(rows, a.chunks, keep)) return cudaErrorInvalidValue;
+    beam::stretches(vocab, beams, rows, sm_count(current_device()), &a);
+    if (scratch_bytes < beam::bytes_of(rows * a.chunks, keep)) return cudaErrorInvalidValue;
     a.parent = parent_out; a.token = token_out; a.score_out = score_out; a.ended_out = ended_out_or_null;
     a.logits = logits; a.row_stride = row_stride; a.vocab = vocab; a.score = score; a.ended = ended_or_null;
     a.eos = eos_id; a.beams = beams; a.keep = keep; a.M = M;
@@ -315,8 +403,7 @@ extern "C" int bw_beam_select(int* parent_out, int* token_out, float* score_out,
     a.best = reinterpret_cast<unsigned long long*>(static_cast<unsigned char*>(scratch) + beam::round16((size_t)rows * a.chunks * sizeof(float2)));
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const dim3 grid((unsigned)a.chunks, (unsigned)rows);
-    cudaError_t e = a.chunk == 2048 ? launch_pdl(beam::chunk_kernel<8>, grid, dim3(beam::kThreads), 0, st, a)
-                                    : launch_pdl(beam::chunk_kernel<32>, grid, dim3(beam::kThreads), 0, st, a);
+    cudaError_t e = launch_pdl(beam::chunk_kernel, grid, dim3(beam::kThreads), 0, st, a);
     if (e == cudaSuccess) e = launch_pdl(beam::merge_kernel, dim3((unsigned)M), dim3(beam::kThreads), 0, st, a);
     count_launch(2);
     return e != cudaSuccess ? e : cudaPeekAtLastError();
