@@ -40,7 +40,11 @@ struct Args {
     const unsigned long long* mask;     // [M * T] or NULL: node j <= i
     int nq, M, T, group, rows, tiles;   // rows = T * group query rows per kv head, in `tiles` blocks of 8 * NT
     int nsplit;
-    float* part;                        // [M][heads][rows][nsplit][kPart] where nsplit > 1
+    float* part;                        // [M][heads][rows][nsplit][kPart] where nsplit > 1; tcgen05 kernel: [2 * blocks][rec_rows][kPart]
+    // tcgen05 kernel
+    int flat, blocks, groups, group_rows, rec_rows;   // work in a line; row groups of 128 or 256 rows
+    int* cum;                           // tiles before each sequence; from kPlanned on, [blocks + 1], where each block's stretch starts
+    int* status;
 };
 
 template <int NT, bool kCoded>
@@ -76,6 +80,11 @@ __device__ __forceinline__ float2 load_q2(const float* p) { return *reinterpret_
 __device__ __forceinline__ float2 load_q2(const __nv_bfloat16* p) {
     const uint32_t u = *reinterpret_cast<const uint32_t*>(p);
     return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
+}
+__device__ __forceinline__ float4 load_q4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float4 load_q4(const __nv_bfloat16* p) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u), __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xFFFF0000u));
 }
 __device__ __forceinline__ void store_o4(float* p, const float4& v) { *reinterpret_cast<float4*>(p) = v; }
 __device__ __forceinline__ void store_o4(__nv_bfloat16* p, const float4& v) {

@@ -23,6 +23,7 @@ cudaError_t attn_reserve_scratch(size_t bytes);
 size_t attn_scratch_bytes(int M, int nqh, int nkv, int ctx);
 namespace peer { void set_two_step_min_kb(int kb); void set_wait_limit_ms(int ms); }  // peer_allreduce.cu
 namespace lm { void set_linear_stream_max(int rows); }  // linear_bf16.cu
+namespace tree { void set_route(int kernel); }          // attention_tree.cu
 
 namespace tc {  // tensor-core path, gemm_w4a8_tc.cu
 bool eligible(const GemvArgs& a, int M);
@@ -747,6 +748,7 @@ extern "C" int bw_set_tuning(int key, int value) {
         case 21: g_tune_prep_min_swiglu = value; return 0;
         case 22: set_attn_slots_pct(value); return 0;
         case 24: wide::set_force(value); return 0;
+        case 25: tree::set_route(value); return 0;
         case 23: lm::set_linear_stream_max(value); return 0;
         default: return cudaErrorInvalidValue;
     }

@@ -157,7 +157,19 @@ def words(masks):
     return torch.tensor([[b - (1 << 64) if b >> 63 else b for b in row] for row in masks], dtype=torch.int64, device="cuda")
 
 
-def check_attention(M, T, nq, nkv, first, max_seq, coded, act, masks=None, count=None, hint=0, layers=1, layer=0, q_size=1.5, v_size=1.0, seed=0,
+def check_attention(*a, **kw):
+    """By both kernels, then by the one that the sizes choose."""
+    k = kernels()
+    try:
+        for route in (1, 2):
+            k.set_tuning(25, route)
+            one_attention(*a, **kw)
+    finally:
+        k.set_tuning(25, 0)
+    return one_attention(*a, **kw)
+
+
+def one_attention(M, T, nq, nkv, first, max_seq, coded, act, masks=None, count=None, hint=0, layers=1, layer=0, q_size=1.5, v_size=1.0, seed=0,
                     store=None, clean=True, stream=None, call=None):
     g = torch.Generator("cuda").manual_seed(seed)
     st = store or Store(g, M, layers, nkv, max_seq, coded, v_size=v_size)
@@ -213,7 +225,8 @@ def check_attention(M, T, nq, nkv, first, max_seq, coded, act, masks=None, count
         bar = (2 * ds + 2 * fine + steps * 2.0 ** -23).reshape(n[m], nq, 1) * torch.einsum("ihgt,htd->ihgd", p, vv[m].abs()).reshape(n[m], nq, HD).amax(-1, keepdim=True)
         if act == torch.bfloat16:
             bar = bar + want.abs() * 2.0 ** -8
-        assert ((got - want).abs() <= bar).all(), (m, ((got - want).abs() / bar).max())
+        off = float(((got - want).abs() / bar).nan_to_num(0).max())   # (a bar of zero: nothing but zeros)
+        assert off <= 1 and (got[(bar == 0).expand_as(got)] == 0).all(), (m, off)
     return out
 
 
