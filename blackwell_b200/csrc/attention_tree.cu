@@ -8,28 +8,59 @@
 namespace bw {
 namespace tree {
 
-constexpr int kMaxSplits = 64;
-
 // Rows of a block, in tiles of eight.
 static int tiles_of_eight(int rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
 
-// One wave of two blocks per SM, no split shorter than 256 positions.
-static int choose_splits(long blocks, int ctx, int sms) {
-    long n = 2L * sms / blocks;
-    if (n > ctx / 256) n = ctx / 256;
-    if (n > kMaxSplits) n = kMaxSplits;
+constexpr int kFewRows = 32;            // query rows of a head that the mma.sync kernel takes
+constexpr int kMaxCluster = 8;
+// Blocks that share a context of a (sequence, head, row tile).  Few of those: one wave of two blocks per SM, but two tiles of 16 positions
+// for each warp or more.  Many: a block has a context whole.  In any case about 512 positions for a warp at most, because its sums are
+// cut, not rounded, at 24 bits.  Measured (us, 32 / 8 heads, 8 bits, fp32): 1 x 2,048 positions 9.7 in 16 shares, 8.8 in 8; 32 x 4,096 to
+// 8,192 positions 123 in 8 shares, 95 in 4, 90 in 2.  Clusters of 16 need 16 free SMs next to each other: 1 x 2,048 positions with 64
+// rows 27 us, as two clusters of 8 and a merge 20.
+static int choose_splits(long pairs, int ctx, int slots, int warps) {
+    long n = slots / pairs;
+    if (n > ctx / (32 * warps)) n = ctx / (32 * warps);
+    if (n < ctx / (512 * warps)) n = ctx / (512 * warps);
+    const long most = 2L * slots / pairs;               // (more than a cluster leave records: not of many rows)
+    if (n > kMaxCluster && n > most) n = most > kMaxCluster ? most : kMaxCluster;
     return n < 1 ? 1 : (int)n;
 }
 
 template <int NT, bool kCoded, typename A>
-static cudaError_t launch(const Args& a, cudaStream_t st) {
+static cudaError_t launch(Args a, int ctx, void* scratch, size_t scratch_bytes, cudaStream_t st) {
+    using Sh = Shape<NT, kCoded>;
     auto kern = attend_kernel<NT, kCoded, A>;
-    constexpr int smem = Shape<NT, kCoded>::kSmem;
     static std::once_flag once[kMaxDevices];
-    std::call_once(once[current_device()], [&] { cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
-    cudaError_t e = launch_pdl(kern, dim3(a.nsplit, a.c.heads * a.tiles, a.M), dim3(kWarps * 32), smem, st, a);
+    const int dev = current_device();
+    std::call_once(once[dev], [&] {
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem);
+        cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    });
+    a.nsplit = choose_splits((long)a.M * a.c.heads * a.tiles, ctx, 2 * sm_count(dev), Sh::kWarps);
+    a.cluster = a.nsplit <= kMaxCluster ? a.nsplit : kMaxCluster;
+    const int groups = a.nsplit / a.cluster;
+    a.nsplit = groups * a.cluster;
+    if (groups > 1) {
+        if (!scratch || scratch_bytes < (size_t)a.M * a.c.heads * a.rows * groups * kPart * sizeof(float)) return cudaErrorInvalidValue;
+        a.part = static_cast<float*>(scratch);
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a.nsplit, a.c.heads * a.tiles, a.M);
+    cfg.blockDim = dim3(Sh::kWarps * 32);
+    cfg.dynamicSmemBytes = Sh::kSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = a.cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = a.cluster > 1 ? 2 : 1;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a);
     count_launch(1);
-    if (e == cudaSuccess && a.nsplit > 1) {
+    if (e == cudaSuccess && groups > 1) {
         const long rows = (long)a.M * a.c.heads * a.rows;
         e = launch_pdl(attend_merge_kernel<A>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, st, a);
         count_launch(1);
@@ -37,8 +68,9 @@ static cudaError_t launch(const Args& a, cudaStream_t st) {
     return e != cudaSuccess ? e : cudaPeekAtLastError();
 }
 template <bool kCoded, typename A>
-static cudaError_t launch_rows(const Args& a, int nt, cudaStream_t st) {
-    return nt == 1 ? launch<1, kCoded, A>(a, st) : nt == 2 ? launch<2, kCoded, A>(a, st) : launch<4, kCoded, A>(a, st);
+static cudaError_t launch_rows(const Args& a, int nt, int ctx, void* scratch, size_t bytes, cudaStream_t st) {
+    return nt == 1 ? launch<1, kCoded, A>(a, ctx, scratch, bytes, st) : nt == 2 ? launch<2, kCoded, A>(a, ctx, scratch, bytes, st)
+                                                                                : launch<4, kCoded, A>(a, ctx, scratch, bytes, st);
 }
 
 template <bool kTall, bool kCoded, typename A>
@@ -50,8 +82,7 @@ static cudaError_t launch_tc(const Args& a, cudaStream_t st) {
     cudaError_t e = launch_pdl(kern, dim3(a.blocks), dim3(kTcThreads), smem, st, a);
     count_launch(1);
     if (e == cudaSuccess && a.flat) {
-        const long rows = (long)a.M * a.c.heads * a.rows;
-        e = launch_pdl(attend_tc_merge_kernel<A>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, st, a);
+        e = launch_pdl(attend_tc_merge_kernel<A>, dim3((a.rows + 31) / 32, a.c.heads, a.M), dim3(256), 0, st, a);
         count_launch(1);
     }
     return e != cudaSuccess ? e : cudaPeekAtLastError();
@@ -61,6 +92,16 @@ static cudaError_t launch_tc_rows(const Args& a, cudaStream_t st) {
     return a.group_rows > 128 ? launch_tc<true, kCoded, A>(a, st) : launch_tc<false, kCoded, A>(a, st);
 }
 
+// Which kernel.  The tcgen05 kernel takes some 20 us before it pays (queries into shared memory, the pipeline's start, records and their merge); a
+// tile of the mma.sync kernel (32 rows, 16 positions) takes a block 0.5 us.  So: by the tiles that an SM gets, and not for one or two row
+// tiles, which leave the 128 lanes of an accumulator half empty, unless there is much of it.  Measured (us, mma.sync / tcgen05; 32 / 8 heads, fp32): 64 nodes,
+// 8 x 2,048 positions 108 / 66, 4 x 1,000 39 / 36, 4 x 300 21 / 31; 24 nodes, 8 x 2,048 62 / 44, 4 x 1,000 22 / 27, 32 x 100 38 / 24; 16 nodes,
+// 32 x 1,000 62 / 71, 32 x 8,192 383 / 346.
+static bool many_rows(long heads, int rows, int ctx, int sms) {
+    if (rows <= kFewRows) return false;
+    const double tiles = (double)heads * ((rows + 31) / 32) * ((ctx + 15) / 16) / sms;
+    return tiles >= (rows <= 64 ? 600 : ctx <= 128 ? 40 : 80);
+}
 static int g_route = 0;   // experiments: 1 mma.sync, 2 tcgen05
 void set_route(int v) { g_route = v; }
 
@@ -69,11 +110,21 @@ void set_route(int v) { g_route = v; }
 
 using namespace bw;
 
-// At most two records per SM of a block's rows, whatever the call's sizes, and the line of work.
+namespace bw {
+namespace tree {
+// Scratch of the tcgen05 kernel: the line of work, two records per block, the sums that fp32 activations keep.
+constexpr size_t kLineBytes = 4096;
+static size_t record_bytes(long blocks, int rows) { return (size_t)2 * blocks * rows * kPart * sizeof(float); }
+static size_t kept_bytes(long blocks) { return (size_t)blocks * 2 * kHd * 128 * sizeof(float); }
+}  // namespace tree
+}  // namespace bw
+
+// Bounds for any smaller call too: the blocks are at most as many as SMs (mma.sync kernel: records of 32 rows of two waves at most).
 extern "C" size_t bw_attention_tree_scratch_bytes(int M, int T, int num_q_heads, int num_kv_heads, int max_context) {
     if (M < 1 || T < 1 || T > tree::kMaxNodes || num_kv_heads < 1 || num_q_heads < 1 || num_q_heads % num_kv_heads || max_context < 1) return 0;
-    const int rows = T * (num_q_heads / num_kv_heads), rec = rows < 32 ? 32 : rows < 256 ? rows : 256;
-    return (size_t)2 * sm_count(current_device()) * rec * tree::kPart * sizeof(float) + 4096;
+    const int sms = sm_count(current_device()), rows = T * (num_q_heads / num_kv_heads);
+    if (rows <= tree::kFewRows) return tree::record_bytes(sms, 32);
+    return tree::kLineBytes + tree::record_bytes(sms, rows < 256 ? rows : 256) + tree::kept_bytes(sms);
 }
 
 extern "C" int bw_attention_tree(void* out, const void* q, const bw_kv_cache* cache, const int* d_first_row,
@@ -90,31 +141,30 @@ extern "C" int bw_attention_tree(void* out, const void* q, const bw_kv_cache* ca
     a.rows = a.group * T;
     const int ctx = ctx_hint > 0 && ctx_hint < a.c.max_seq ? ctx_hint : a.c.max_seq, sms = sm_count(current_device());
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (tree::g_route == 2 || (tree::g_route == 0 && a.rows > 32)) {
+    if (tree::g_route == 2 || (tree::g_route == 0 && tree::many_rows((long)M * a.c.heads, a.rows, ctx, sms))) {
         a.group_rows = a.rows > 128 ? 256 : 128;
         a.groups = (a.rows + a.group_rows - 1) / a.group_rows;
         a.rec_rows = a.rows < a.group_rows ? a.rows : a.group_rows;
         const long pairs = (long)M * a.c.heads * a.groups, tiles = (ctx + tree::kTcKeys - 1) / tree::kTcKeys;
-        if (pairs > 0x7FFFFFFFL) return cudaErrorInvalidValue;
+        if (pairs > (1L << 30) || a.c.heads > 65535) return cudaErrorInvalidValue;
+        // In a line, unless every head's context is short or heads are many times the blocks.
+        a.pairs = (int)pairs;
+        a.flat = M <= tree::kPlanned && pairs < 4L * sms && tiles > 2 && pairs * (a.c.max_seq / tree::kTcKeys + 1) < (1L << 30);
+        const long work = a.flat ? pairs * tiles / 2 : pairs;    // (two tiles for a block or more)
+        a.blocks = (int)(work < sms ? work : sms);
+        const size_t records = a.flat ? tree::kLineBytes + tree::record_bytes(a.blocks, a.rec_rows) : 0;
+        if ((a.flat || !bf16) && (!scratch || scratch_bytes < records + (bf16 ? 0 : tree::kept_bytes(a.blocks)))) return cudaErrorInvalidValue;
+        a.cum = static_cast<int*>(scratch);
+        a.part = reinterpret_cast<float*>(static_cast<unsigned char*>(scratch) + tree::kLineBytes);
+        a.kept = reinterpret_cast<float*>(static_cast<unsigned char*>(scratch) + records);
         a.status = status_word_ptr();
-        a.flat = M <= tree::kPlanned && pairs < 4L * sms && tiles > 2 && pairs * (a.c.max_seq / tree::kTcKeys + 1) < 0x7FFFFFFFL;
-        a.blocks = (int)(!a.flat ? pairs : pairs * tiles < sms ? pairs * tiles : sms);
-        if (a.flat) {
-            if (!scratch || scratch_bytes < 4096 + (size_t)2 * a.blocks * a.rec_rows * tree::kPart * sizeof(float)) return cudaErrorInvalidValue;
-            a.cum = static_cast<int*>(scratch);
-            a.part = reinterpret_cast<float*>(static_cast<unsigned char*>(scratch) + 4096);
-        }
         if (a.c.coded()) return bf16 ? tree::launch_tc_rows<true, __nv_bfloat16>(a, st) : tree::launch_tc_rows<true, float>(a, st);
         return bf16 ? tree::launch_tc_rows<false, __nv_bfloat16>(a, st) : tree::launch_tc_rows<false, float>(a, st);
     }
     const int nt = tree::tiles_of_eight(a.rows);
     a.tiles = (a.rows + 8 * nt - 1) / (8 * nt);
     if ((long)a.c.heads * a.tiles > 65535) return cudaErrorInvalidValue;
-    a.nsplit = tree::choose_splits((long)M * a.c.heads * a.tiles, ctx, sms);
-    if (a.nsplit > 1) {
-        if (!scratch || scratch_bytes < (size_t)M * a.c.heads * a.rows * a.nsplit * tree::kPart * sizeof(float)) return cudaErrorInvalidValue;
-        a.part = static_cast<float*>(scratch);
-    }
-    if (a.c.coded()) return bf16 ? tree::launch_rows<true, __nv_bfloat16>(a, nt, st) : tree::launch_rows<true, float>(a, nt, st);
-    return bf16 ? tree::launch_rows<false, __nv_bfloat16>(a, nt, st) : tree::launch_rows<false, float>(a, nt, st);
+    if (a.c.coded())
+        return bf16 ? tree::launch_rows<true, __nv_bfloat16>(a, nt, ctx, scratch, scratch_bytes, st) : tree::launch_rows<true, float>(a, nt, ctx, scratch, scratch_bytes, st);
+    return bf16 ? tree::launch_rows<false, __nv_bfloat16>(a, nt, ctx, scratch, scratch_bytes, st) : tree::launch_rows<false, float>(a, nt, ctx, scratch, scratch_bytes, st);
 }

@@ -27,7 +27,6 @@ namespace tree {
 
 using kv::kHd;
 constexpr int kMaxNodes = 64;
-constexpr int kWarps = 4;
 constexpr int kTile = 16;               // positions a warp takes at once
 constexpr int kPart = kHd + 4;          // floats of a partial record: outputs, maximum, sum, padding
 constexpr float kHead = 6.f, kSlack = 14.f;   // P up to 2^6 when the maximum is new, 2^14 before it is moved
@@ -39,31 +38,32 @@ struct Args {
     const int *first, *count;
     const unsigned long long* mask;     // [M * T] or NULL: node j <= i
     int nq, M, T, group, rows, tiles;   // rows = T * group query rows per kv head, in `tiles` blocks of 8 * NT
-    int nsplit;
-    float* part;                        // [M][heads][rows][nsplit][kPart] where nsplit > 1; tcgen05 kernel: [2 * blocks][rec_rows][kPart]
+    int nsplit, cluster;                // blocks that share a context; those that join as a cluster
+    float* part;                        // [M][heads][rows][nsplit / cluster][kPart] where there are several; tcgen05 kernel: [2 * blocks][rec_rows][kPart]
     // tcgen05 kernel
-    int flat, blocks, groups, group_rows, rec_rows;   // work in a line; row groups of 128 or 256 rows
+    int flat, blocks, pairs, groups, group_rows, rec_rows;   // work in a line; heads and row groups of 128 or 256 rows in all
     int* cum;                           // tiles before each sequence; from kPlanned on, [blocks + 1], where each block's stretch starts
+    float* kept;                        // fp32: [blocks][2][128][128]
     int* status;
 };
 
 template <int NT, bool kCoded>
 struct Shape {
     static constexpr int kRows = 8 * NT;
-    static constexpr int kStages = kCoded ? 4 : 3;
+    static constexpr int kStages = NT > 2 && !kCoded ? 2 : 3;              // (two blocks fit an SM)
+    static constexpr int kWarps = NT == 1 && kCoded ? 8 : 4;               // two blocks per SM, as many warps as the registers allow
     static constexpr int kSide = kTile * kHd * (kCoded ? 1 : 2);           // bytes of 16 K or V rows
-    static constexpr int kStage = 2 * kSide + (kCoded ? 2 * kTile * 4 : 0); // and their scales
-    static constexpr int kWarp = kStages * kStage;
+    static constexpr int kStage = 2 * kSide;
+    static constexpr int kRing = kStages * kStage;
     static constexpr int kO = kRows * kHd * 4;                             // a warp's O, over its stages once they have drained
-    static constexpr int kPerWarp = kWarp > kO ? kWarp : kO;
-    static constexpr int kSmem = kWarps * kPerWarp;
+    static constexpr int kPerWarp = kRing > kO ? kRing : kO;
+    static constexpr int kQ = NT > 2 ? 8 * NT * 32 * 16 : 0;               // the query operand where it does not fit in registers
+    static constexpr int kSmem = kWarps * kPerWarp + kQ;
 };
 
-// f16 pair of two e4m3 codes (exact).
-__device__ __forceinline__ uint32_t codes_f16x2(uint32_t two) {
-    uint32_t r;
-    asm("{\n\t.reg .b16 c;\n\tcvt.u16.u32 c, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, c;\n\t}" : "=r"(r) : "r"(two));
-    return r;
+// f16 pairs of two e4m3 codes each (exact): the low and the high half of a word.
+__device__ __forceinline__ void codes_f16(uint32_t four, uint32_t& lo, uint32_t& hi) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(four));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     uint32_t r;
@@ -75,6 +75,13 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float4 ld_dsmem4(uint32_t addr, uint32_t rank) {
+    uint32_t ra;
+    float4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"(addr), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(ra) : "memory");
+    return v;
 }
 __device__ __forceinline__ float2 load_q2(const float* p) { return *reinterpret_cast<const float2*>(p); }
 __device__ __forceinline__ float2 load_q2(const __nv_bfloat16* p) {
@@ -97,11 +104,7 @@ __device__ __forceinline__ float2 binade(float x) {
     return make_float2(__uint_as_float(e << 23), __uint_as_float((254 - e) << 23));
 }
 
-// What a sequence's rows see: positions [0, ctx) all of them, node j (position ctx + j, j < nodes) by its mask bit.
-struct Seen {
-    int ctx, end;                       // end: positions in all
-    unsigned long long any;             // nodes that some row of the sequence sees
-};
+// What a sequence's rows see: positions [0, first) all of them, node j (position first + j) by bit j of a row's mask.
 __device__ __forceinline__ unsigned long long low_bits(int n) { return n >= 64 ? ~0ull : (1ull << n) - 1; }
 __device__ __forceinline__ int node_count(const Args& a, int m) { return a.count ? max(0, min(a.count[m], a.T)) : a.T; }
 __device__ __forceinline__ unsigned long long mask_of(const Args& a, int m, int node, int nodes) {
@@ -109,56 +112,70 @@ __device__ __forceinline__ unsigned long long mask_of(const Args& a, int m, int 
 }
 
 template <int NT, bool kCoded, typename A>
-__global__ void __launch_bounds__(kWarps * 32) attend_kernel(const Args a) {
+__global__ void __launch_bounds__(Shape<NT, kCoded>::kWarps * 32, 2) attend_kernel(const Args a) {
     using Sh = Shape<NT, kCoded>;
+    constexpr int kWarps = Sh::kWarps;
     constexpr bool kSplit = sizeof(A) == 4;             // fp32 activations: two products
     extern __shared__ __align__(128) unsigned char dsm[];
-    __shared__ unsigned long long s_mask[Sh::kRows], s_any;
-    __shared__ float s_m[kWarps][Sh::kRows], s_l[kWarps][Sh::kRows];
-    __shared__ uint4 s_q[NT > 2 ? 8 * NT * 32 : 1];     // query operand where it does not fit in registers
+    __shared__ unsigned long long s_mask[Sh::kRows];
+    __shared__ float s_m[kWarps][Sh::kRows], s_l[kWarps][Sh::kRows], s_unit[Sh::kRows];
+    __shared__ float2 s_ml[Sh::kRows];                  // this block's maximum and sum, for the cluster
+    uint4* s_q = reinterpret_cast<uint4*>(dsm + kWarps * Sh::kPerWarp);
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31, g = lane >> 2, tq = lane & 3;
     const int split = blockIdx.x, head = blockIdx.y / a.tiles, r0 = (blockIdx.y - head * a.tiles) * Sh::kRows, m = blockIdx.z;
     pdl_trigger();
     pdl_wait();
     const int first = a.first[m], nodes = node_count(a, m);
-    if (first < 0 || r0 >= nodes * a.group) return;
-    // masks: this block's rows, and of all nodes
-    if (t == 0) s_any = 0;
-    __syncthreads();
-    if (t < nodes) atomicOr(&s_any, mask_of(a, m, t, nodes));
-    for (int r = t; r < Sh::kRows; r += kWarps * 32) s_mask[r] = (r0 + r) < nodes * a.group ? mask_of(a, m, (r0 + r) / a.group, nodes) : 0;
-    __syncthreads();
-    Seen see;
-    see.ctx = min(first, a.c.max_seq);
-    see.end = (int)min((long)first + nodes, (long)a.c.max_seq);
-    see.any = s_any;
-    const int ntile = (see.end + kTile - 1) / kTile;
+    if (first < 0 || r0 >= nodes * a.group) return;     // (all blocks of the cluster)
+    const int ctx = min(first, a.c.max_seq), end = (int)min((long)first + nodes, (long)a.c.max_seq);
+    const int ntile = (end + kTile - 1) / kTile;
     const int tile0 = (int)((long)ntile * split / a.nsplit), tile1 = (int)((long)ntile * (split + 1) / a.nsplit);
 
     const size_t row0 = a.c.row(m, head, 0);
-    constexpr int kRowBytes = kCoded ? kHd : 2 * kHd, kChunks = kRowBytes / 16;
+    constexpr int kRowBytes = kCoded ? kHd : 2 * kHd, kChunks = kRowBytes / 16, kStep = 32 / kChunks;
     const unsigned char *Kb = a.c.k + row0 * kRowBytes, *Vb = a.c.v + row0 * kRowBytes;
     const uint32_t stage0 = smem_u32(dsm + warp * Sh::kPerWarp);
-    // 16 rows of K and V (and their scales) to a stage; rows that nobody sees become zeros, whatever lies there
+    // masks of all nodes, for what nobody sees; only where this block comes to the nodes
+    unsigned long long any = 0;
+    const bool comes = tile1 * kTile > ctx;
+    if (comes) {
+        const unsigned long long mine = (lane < nodes ? mask_of(a, m, lane, nodes) : 0) | (lane + 32 < nodes ? mask_of(a, m, lane + 32, nodes) : 0);
+        any = (unsigned long long)__reduce_or_sync(0xffffffffu, (uint32_t)(mine >> 32)) << 32 | __reduce_or_sync(0xffffffffu, (uint32_t)mine);
+        for (int r = t; r < Sh::kRows; r += kWarps * 32) s_mask[r] = r0 + r < nodes * a.group ? mask_of(a, m, (r0 + r) / a.group, nodes) : 0;
+    }
+    auto there = [&](int p) { return p < ctx || (p < end && (any >> (p - ctx) & 1)); };
+    // 16 rows of K and V to a stage: piece c of rows rr, rr + kStep, ...; rows that nobody sees become zeros, whatever lies there
+    const int c = lane % kChunks, rr = lane / kChunks;
+    const uint32_t off = rr * kRowBytes + ((c ^ (rr & 7)) << 4);
     auto issue = [&](int tile, int stage) {
         const int p0 = tile * kTile;
         const uint32_t to = stage0 + stage * Sh::kStage;
-        const bool all = p0 + kTile <= see.ctx;
+        const unsigned char *k = Kb + (size_t)(p0 + rr) * kRowBytes + c * 16, *v = Vb + (size_t)(p0 + rr) * kRowBytes + c * 16;
+        if (p0 + kTile <= ctx) {
 #pragma unroll
-        for (int i = 0; i < kTile * kChunks / 32; ++i) {
-            const int idx = i * 32 + lane, r = idx / kChunks, c = idx % kChunks, p = p0 + r;
-            const bool there = all || p < see.ctx || (p < see.end && (see.any >> (p - see.ctx) & 1));
-            const size_t from = (size_t)(there ? p : 0) * kRowBytes + c * 16;
-            const uint32_t at = to + r * kRowBytes + ((c ^ (r & 7)) << 4);
-            lm::cp_async16z(at, Kb + from, there);
-            lm::cp_async16z(at + Sh::kSide, Vb + from, there);
+            for (int i = 0; i < kTile / kStep; ++i) {
+                // the row's low bits: rr + kStep * i, of which kStep * i flips whole bits above rr's
+                const uint32_t at = to + (off ^ (((kStep * i) & 7) << 4)) + kStep * i * kRowBytes;
+                amma::cp_async16(at, k + i * kStep * kRowBytes);
+                amma::cp_async16(at + Sh::kSide, v + i * kStep * kRowBytes);
+            }
+        } else {
+#pragma unroll 1
+            for (int i = 0; i < kTile / kStep; ++i) {
+                const bool in = there(p0 + rr + kStep * i);
+                const uint32_t at = to + (off ^ (((kStep * i) & 7) << 4)) + kStep * i * kRowBytes;
+                lm::cp_async16z(at, in ? k + i * kStep * kRowBytes : Kb, in);
+                lm::cp_async16z(at + Sh::kSide, in ? v + i * kStep * kRowBytes : Vb, in);
+            }
         }
-        if (kCoded) {
-            const int r = lane & 15, p = p0 + r;
-            const bool there = all || p < see.ctx || (p < see.end && (see.any >> (p - see.ctx) & 1));
-            const float* s = (lane < 16 ? a.c.ks : a.c.vs) + row0 + (there ? p : 0);
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + 2 * Sh::kSide + lane * 4), "l"(s), "r"(there ? 4 : 0) : "memory");
-        }
+    };
+    // key and value scales of this thread's positions g, g + 8 of a tile
+    auto scales_of = [&](int tile, float (&s)[4]) {
+        const int p = tile * kTile + g;
+        const bool a0 = there(p), a1 = there(p + 8);
+        const size_t i0 = row0 + p;
+        s[0] = a0 ? a.c.ks[i0] : 0.f; s[1] = a1 ? a.c.ks[i0 + 8] : 0.f;
+        s[2] = a0 ? a.c.vs[i0] : 0.f; s[3] = a1 ? a.c.vs[i0 + 8] : 0.f;
     };
     int next = tile0 + warp;
 #pragma unroll
@@ -167,56 +184,69 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const Args a) {
         lm::cp_async_commit();
         next += kWarps;
     }
+    float sc[4] = {1.f, 1.f, 1.f, 1.f};
+    if (kCoded && tile0 + warp < tile1) scales_of(tile0 + warp, sc);
 
     // The query operand: column n of tile j is row r0 + 8 j + n.  Coded keys: a thread's four dimensions of k-step s are 32 tq + 4 s ...,
-    // as it finds them in 16 bytes of a key row; otherwise 16 s + 2 tq, + 1, + 8, + 9.
+    // as it finds them in 16 bytes of a key row; otherwise 16 s + 2 tq, + 1, + 8, + 9.  NT > 2: warp j prepares tile j for all.
     constexpr int kRegs = NT > 2 ? 1 : NT;
     uint32_t qh[kRegs][8][2], ql[kSplit ? kRegs : 1][8][2];
     float qf[NT][2];                                    // factor of the scores of columns 2 tq, 2 tq + 1, base 2
-    {
-        float2 unit[NT];
+    constexpr float kScore = 0.08838834764831845f * 1.4426950408889634f;
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            const int r = r0 + 8 * j + g, node = r / a.group;
-            const bool there = node < nodes;
-            const A* q = static_cast<const A*>(a.q) + (((size_t)m * a.T + (there ? node : 0)) * a.nq + head * a.group + (there ? r - node * a.group : 0)) * kHd;
-            float2 x[8][2];
-            float top = 0.f;
+    for (int jj = 0; jj < kRegs; ++jj) {
+        const int j = NT > 2 ? warp : jj;
+        if (NT > 2 && warp >= NT) break;
+        const int r = r0 + 8 * j + g, node = r / a.group;
+        const bool in = node < nodes;
+        const A* q = static_cast<const A*>(a.q) + (((size_t)m * a.T + (in ? node : 0)) * a.nq + head * a.group + (in ? r - node * a.group : 0)) * kHd;
+        float2 x[8][2];
+        float top = 0.f;
 #pragma unroll
-            for (int s = 0; s < 8; ++s)
+        for (int s = 0; s < 8; ++s)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    x[s][e] = there ? load_q2(q + (kCoded ? 32 * tq + 4 * s + 2 * e : 16 * s + 2 * tq + 8 * e)) : make_float2(0.f, 0.f);
-                    top = fmaxf(top, fmaxf(fabsf(x[s][e].x), fabsf(x[s][e].y)));
-                }
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            unit[j] = binade(top);
+            for (int e = 0; e < 2; ++e) x[s][e] = in ? load_q2(q + (kCoded ? 32 * tq + 4 * s + 2 * e : 16 * s + 2 * tq + 8 * e)) : make_float2(0.f, 0.f);
 #pragma unroll
-            for (int s = 0; s < 8; ++s) {
-                uint32_t h[2], l[2] = {0, 0};
+        for (int s = 0; s < 8; ++s)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    if (kSplit) {
-                        amma::split_hi_lo(x[s][e].x * unit[j].y, x[s][e].y * unit[j].y, h[e], l[e]);
-                    } else {
-                        const __half2 v = __floats2half2_rn(x[s][e].x * unit[j].y, x[s][e].y * unit[j].y);
-                        h[e] = *reinterpret_cast<const uint32_t*>(&v);
-                    }
-                }
-                if (NT > 2) {
-                    if (j % kWarps == warp) s_q[(s * NT + j) * 32 + lane] = make_uint4(h[0], h[1], l[0], l[1]);
+            for (int e = 0; e < 2; ++e) top = fmaxf(top, fmaxf(fabsf(x[s][e].x), fabsf(x[s][e].y)));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float2 unit = binade(top);
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+            uint32_t h[2], l[2] = {0, 0};
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                if (kSplit) {
+                    amma::split_hi_lo(x[s][e].x * unit.y, x[s][e].y * unit.y, h[e], l[e]);
                 } else {
-                    qh[NT > 2 ? 0 : j][s][0] = h[0]; qh[NT > 2 ? 0 : j][s][1] = h[1];
-                    if (kSplit) { ql[NT > 2 ? 0 : j][s][0] = l[0]; ql[NT > 2 ? 0 : j][s][1] = l[1]; }
+                    const __half2 v = __floats2half2_rn(x[s][e].x * unit.y, x[s][e].y * unit.y);
+                    h[e] = *reinterpret_cast<const uint32_t*>(&v);
                 }
             }
+            if (NT > 2) {
+                s_q[(s * NT + j) * 32 + lane] = make_uint4(h[0], h[1], l[0], l[1]);
+            } else {
+                qh[NT > 2 ? 0 : jj][s][0] = h[0]; qh[NT > 2 ? 0 : jj][s][1] = h[1];
+                if (kSplit) { ql[NT > 2 ? 0 : jj][s][0] = l[0]; ql[NT > 2 ? 0 : jj][s][1] = l[1]; }
+            }
+        }
+        if (NT > 2) {
+            if (tq == 0) s_unit[8 * j + g] = unit.x;
+        } else {
 #pragma unroll
             for (int e = 0; e < 2; ++e)                 // (column 2 tq + e is lane group 2 tq + e's row)
-                qf[j][e] = __shfl_sync(0xffffffffu, unit[j].x, (2 * tq + e) * 4) * (0.08838834764831845f * 1.4426950408889634f);
+                qf[jj][e] = __shfl_sync(0xffffffffu, unit.x, (2 * tq + e) * 4) * kScore;
         }
     }
-    if (NT > 2) __syncthreads();
+    __syncthreads();                                    // masks, queries
+    if (NT > 2) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) qf[j][e] = s_unit[8 * j + 2 * tq + e] * kScore;
+    }
 
     float o[NT][8][4], mx[NT][2], l[NT][2], vref = __uint_as_float(2u << 23);
 #pragma unroll
@@ -232,10 +262,11 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const Args a) {
         if (next < tile1) issue(next, stage == 0 ? Sh::kStages - 1 : stage - 1);
         lm::cp_async_commit();
         next += kWarps;
+        float sc_next[4] = {1.f, 1.f, 1.f, 1.f};
+        if (kCoded && tile + kWarps < tile1) scales_of(tile + kWarps, sc_next);
         lm::cp_async_wait<Sh::kStages - 1>();
         __syncwarp();
         const uint32_t ks = stage0 + stage * Sh::kStage, vs = ks + Sh::kSide;
-        const float* scales = reinterpret_cast<const float*>(dsm + warp * Sh::kPerWarp + stage * Sh::kStage + 2 * Sh::kSide);
 
         // ---- S^T: rows g, g + 8 of the tile's positions, columns 2 tq, 2 tq + 1 of each query tile
         float s[NT][4], s2[kSplit ? NT : 1][4];
@@ -267,27 +298,22 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const Args a) {
                 const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const uint32_t k[4] = {codes_f16x2(wl[e]), codes_f16x2(wh[e]), codes_f16x2(wl[e] >> 16), codes_f16x2(wh[e] >> 16)};
+                    uint32_t k[4];
+                    codes_f16(wl[e], k[0], k[2]);
+                    codes_f16(wh[e], k[1], k[3]);
                     key_step(4 * hf + e, k);
                 }
             }
         } else {
-            const int mi = lane >> 3, rr = lane & 7;
+            const int mi = lane >> 3, r8 = lane & 7;
 #pragma unroll
             for (int st = 0; st < 8; ++st) {
                 uint32_t k[4];
-                amma::ldmatrix_x4(ks + ((mi & 1) * 8 + rr) * 2 * kHd + (((2 * st + (mi >> 1)) ^ rr) << 4), k[0], k[1], k[2], k[3]);
+                amma::ldmatrix_x4(ks + ((mi & 1) * 8 + r8) * 2 * kHd + (((2 * st + (mi >> 1)) ^ r8) << 4), k[0], k[1], k[2], k[3]);
                 key_step(st, k);
             }
         }
         // ---- scores in base 2; masks where the tile reaches the nodes
-        float vsc[2] = {1.f, 1.f};
-        float ksc[2] = {1.f, 1.f};
-        if (kCoded) {
-            ksc[0] = scales[g]; ksc[1] = scales[g + 8];
-            vsc[0] = scales[16 + g]; vsc[1] = scales[16 + g + 8];
-        }
-        bool move = false;
         const int p0 = tile * kTile;
 #pragma unroll
         for (int j = 0; j < NT; ++j)
@@ -296,26 +322,27 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const Args a) {
                 float x = s[j][e];
                 if (kSplit) x += s2[kSplit ? j : 0][e];
                 x *= qf[j][e & 1];
-                if (kCoded) x *= ksc[e >> 1];
+                if (kCoded) x *= sc[e >> 1];
                 s[j][e] = x;
             }
-        if (p0 + kTile > see.ctx) {
+        if (p0 + kTile > ctx) {
 #pragma unroll
             for (int j = 0; j < NT; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int p = p0 + g + 8 * (e >> 1);
-                    const bool yes = p < see.ctx || (p < see.end && (s_mask[8 * j + 2 * tq + (e & 1)] >> (p - see.ctx) & 1));
+                    const bool yes = p < ctx || (p < end && (s_mask[8 * j + 2 * tq + (e & 1)] >> (p - ctx) & 1));
                     s[j][e] = yes ? s[j][e] : -INFINITY;
                 }
         }
+        bool move = false;
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
             for (int e = 0; e < 2; ++e) move |= fmaxf(s[j][e], s[j][e + 2]) > mx[j][e] + kSlack;
         float vtop = vref;
         if (kCoded) {
-            vtop = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fabsf(vsc[0]), fabsf(vsc[1])))));
+            vtop = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fabsf(sc[2]), fabsf(sc[3])))));
             move |= vtop > vref;
         }
         if (__any_sync(0xffffffffu, move)) {
@@ -334,10 +361,10 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const Args a) {
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                    const float to = fmaxf(mx[j][e], top - kHead), c = lm::exp2_fast(mx[j][e] - to);
+                    const float to = fmaxf(mx[j][e], top - kHead), cc = lm::exp2_fast(mx[j][e] - to);
                     mx[j][e] = to;
-                    l[j][e] *= c;
-                    f[e] = c * fv;
+                    l[j][e] *= cc;
+                    f[e] = cc * fv;
                 }
 #pragma unroll
                 for (int d = 0; d < 8; ++d) {
@@ -348,7 +375,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const Args a) {
         }
         // ---- P^T, and to the operand layout
         const float vdiv = kCoded ? __uint_as_float((254u << 23) - __float_as_uint(vref)) : 1.f;
-        const float vr[2] = {vsc[0] * vdiv, vsc[1] * vdiv};
+        const float vr[2] = {sc[2] * vdiv, sc[3] * vdiv};
         uint32_t ph[NT][2], pl[kSplit ? NT : 1][2];
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
@@ -394,22 +421,25 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const Args a) {
                                        d < 2 ? w[2].x : d < 4 ? w[2].y : d < 6 ? w[2].z : w[2].w, d < 2 ? w[3].x : d < 4 ? w[3].y : d < 6 ? w[3].z : w[3].w};
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {           // bytes 2 e, 2 e + 1 of two positions: b0 b0' b1 b1'
-                    const uint32_t lo = prmt(x[0], x[1], e ? 0x7362 : 0x5140), hi = prmt(x[2], x[3], e ? 0x7362 : 0x5140);
-                    const uint32_t v[4] = {codes_f16x2(lo), codes_f16x2(lo >> 16), codes_f16x2(hi), codes_f16x2(hi >> 16)};
+                    uint32_t v[4];
+                    codes_f16(prmt(x[0], x[1], e ? 0x7362 : 0x5140), v[0], v[1]);
+                    codes_f16(prmt(x[2], x[3], e ? 0x7362 : 0x5140), v[2], v[3]);
                     value_step(d + e, v);
                 }
             }
         } else {
-            const int mi = lane >> 3, rr = lane & 7;
+            const int mi = lane >> 3, r8 = lane & 7;
 #pragma unroll
             for (int d = 0; d < 8; ++d) {
                 uint32_t v[4];
-                amma::ldmatrix_x4_trans(vs + ((mi >> 1) * 8 + rr) * 2 * kHd + (((2 * d + (mi & 1)) ^ rr) << 4), v[0], v[1], v[2], v[3]);
+                amma::ldmatrix_x4_trans(vs + ((mi >> 1) * 8 + r8) * 2 * kHd + (((2 * d + (mi & 1)) ^ r8) << 4), v[0], v[1], v[2], v[3]);
                 value_step(d, v);
             }
         }
         __syncwarp();                                   // the stage is filled again in the next turn
         stage = stage == Sh::kStages - 1 ? 0 : stage + 1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[i] = sc_next[i];
     }
     lm::cp_async_wait<0>();
     __syncwarp();
@@ -438,33 +468,61 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const Args a) {
             }
         }
     __syncthreads();
-    for (int r = warp; r < Sh::kRows; r += kWarps) {    // a warp per row, four dimensions a lane
+    // ---- and together: a warp per row, four dimensions a lane; over the first warp's where a cluster goes on with them
+    const int groups = a.nsplit / a.cluster, grp = split / a.cluster;
+    auto emit = [&](int r, const float4& acc, float top, float sum) {
         const int row = r0 + r, node = row / a.group;
-        if (node >= nodes) break;
+        if (groups == 1) {
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;   // a row that sees nothing: 0
+            A* out = static_cast<A*>(a.out) + (((size_t)m * a.T + node) * a.nq + head * a.group + row - node * a.group) * kHd + 4 * lane;
+            store_o4(out, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+        } else {
+            float* rec = a.part + ((((size_t)m * a.c.heads + head) * a.rows + row) * groups + grp) * kPart;
+            *reinterpret_cast<float4*>(rec + 4 * lane) = acc;
+            if (lane == 0) *reinterpret_cast<float2*>(rec + kHd) = make_float2(top, sum);
+        }
+    };
+    const int rows = min(Sh::kRows, nodes * a.group - r0);
+    for (int r = warp; r < rows; r += kWarps) {
         float top = -FLT_MAX, sum = 0.f;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_m[w][r]);
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-            const float c = lm::exp2_fast(s_m[w][r] - top);
+            const float cc = lm::exp2_fast(s_m[w][r] - top);
             const float4 v = *reinterpret_cast<const float4*>(dsm + w * Sh::kPerWarp + (r * kHd + 4 * lane) * 4);
-            sum = fmaf(s_l[w][r], c, sum);
-            acc.x = fmaf(v.x, c, acc.x); acc.y = fmaf(v.y, c, acc.y); acc.z = fmaf(v.z, c, acc.z); acc.w = fmaf(v.w, c, acc.w);
+            sum = fmaf(s_l[w][r], cc, sum);
+            acc.x = fmaf(v.x, cc, acc.x); acc.y = fmaf(v.y, cc, acc.y); acc.z = fmaf(v.z, cc, acc.z); acc.w = fmaf(v.w, cc, acc.w);
         }
-        if (a.nsplit == 1) {
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;   // a row that sees nothing: 0
-            A* out = static_cast<A*>(a.out) + (((size_t)m * a.T + node) * a.nq + head * a.group + row - node * a.group) * kHd + 4 * lane;
-            store_o4(out, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+        if (a.cluster == 1) {
+            emit(r, acc, top, sum);
         } else {
-            float* rec = a.part + ((((size_t)m * a.c.heads + head) * a.rows + row) * a.nsplit + split) * kPart;
-            *reinterpret_cast<float4*>(rec + 4 * lane) = acc;
-            if (lane == 0) *reinterpret_cast<float2*>(rec + kHd) = make_float2(top, sum);
+            *reinterpret_cast<float4*>(dsm + (r * kHd + 4 * lane) * 4) = acc;   // (this lane alone reads and writes there)
+            if (lane == 0) s_ml[r] = make_float2(top, sum);
         }
     }
+    if (a.cluster == 1) return;
+    cluster_sync_all();                                 // every block's record is in its shared memory
+    const int rank = split - grp * a.cluster;
+    for (int r = rank + warp * a.cluster; r < rows; r += kWarps * a.cluster) {
+        const uint32_t ml = smem_u32(&s_ml[r]), ov = smem_u32(dsm) + (r * kHd + 4 * lane) * 4;
+        const bool has = lane < a.cluster;
+        const float tb = has ? ld_dsmem(ml, lane) : -FLT_MAX, lb = has ? ld_dsmem(ml + 4, lane) : 0.f;
+        const float top = warp_max(tb), wgt = lm::exp2_fast(tb - top), sum = warp_sum(lb * wgt);
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int b = 0; b < a.cluster; ++b) {
+            const float cc = __shfl_sync(0xffffffffu, wgt, b);
+            const float4 v = ld_dsmem4(ov, b);
+            acc.x = fmaf(v.x, cc, acc.x); acc.y = fmaf(v.y, cc, acc.y); acc.z = fmaf(v.z, cc, acc.z); acc.w = fmaf(v.w, cc, acc.w);
+        }
+        emit(r, acc, top, sum);
+    }
+    cluster_sync_all();                                 // nobody leaves while its record may still be read
 }
 
-// The splits' records of a row, a warp each.
+// The clusters' records of a row, a warp each.
 template <typename A>
 __global__ void __launch_bounds__(128) attend_merge_kernel(const Args a) {
     pdl_trigger();
@@ -474,12 +532,14 @@ __global__ void __launch_bounds__(128) attend_merge_kernel(const Args a) {
     if (at >= (long)a.M * a.c.heads * a.rows) return;
     const int row = (int)(at % a.rows), mh = (int)(at / a.rows), m = mh / a.c.heads, head = mh - m * a.c.heads, node = row / a.group;
     if (a.first[m] < 0 || node >= node_count(a, m)) return;
-    const float* rec = a.part + (size_t)at * a.nsplit * kPart;
+    const int parts = a.nsplit / a.cluster;
+    const float* rec = a.part + (size_t)at * parts * kPart;
     float top = -FLT_MAX, sum = 0.f;
-    for (int s = lane; s < a.nsplit; s += 32) top = fmaxf(top, rec[(size_t)s * kPart + kHd]);
+    for (int s = lane; s < parts; s += 32) top = fmaxf(top, rec[(size_t)s * kPart + kHd]);
     top = warp_max(top);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < a.nsplit; ++s) {
+#pragma unroll 4
+    for (int s = 0; s < parts; ++s) {
         const float2 ml = *reinterpret_cast<const float2*>(rec + (size_t)s * kPart + kHd);
         const float4 v = *reinterpret_cast<const float4*>(rec + (size_t)s * kPart + 4 * lane);
         const float c = lm::exp2_fast(ml.x - top);

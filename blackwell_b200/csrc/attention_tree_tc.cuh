@@ -3,13 +3,13 @@
 // One block of 512 threads per SM.  Query rows (node, query head of the group) are the 128 lanes of an accumulator; two accumulator sets
 // ("streams") keep the tensor cores busy while the softmax of one runs:
 //   kTall   more than 128 rows: each stream has 128 rows, both take every 64 positions of the context
-//   else    each stream has all rows and takes every other 64 positions; stream 1 hands its result to stream 0 at the end
+//   else    each stream has all rows and takes every other 64 positions; at the end they join what they have, half of the columns each
 // Warps 0-3 and 4-7: softmax of a stream, a thread per row.  Warps 8-11: the cache; binary16 rows go to their swizzled place by cp.async, codes
-// come raw, become f16 (exact) and are stored there.  Warp 12 issues the products:
+// come raw, become f16 (exact) and are stored there.  Warps 12 and 13 issue a stream's products each:
 //   S = Q K^T    two S buffers of 64 columns per stream, the next scores are on their way while the softmax has these
 //   O += P V     P over the scores' columns as the f16 A operand, V from shared memory as it lies there ([position][column])
 // fp32 activations: Q and P as f16 high parts and remainders, multiplied one after the other.  The accumulator's sums are cut, not rounded, at
-// 24 bits, which adds up over a long context: there O is taken to registers every eight tiles and starts afresh.
+// 24 bits, which adds up over a long context: there O is added to a sum in the scratch memory (L2) every eight tiles and starts afresh.
 // Scales and the moving maximum as in attention_tree.cuh; a warp brings its rows of O to a new maximum by itself.
 // Work is shared out in tiles of 64 positions: all sequences' tiles, heads and row groups in one line, an equal stretch of it per block; what
 // a block has of a head's context that it does not have whole goes to a record that the merge kernel joins.
@@ -25,36 +25,79 @@ constexpr int kTcKeys = 64, kTcPanel = kTcKeys * 128, kTcThreads = 512;   // pos
 constexpr int kTcStage = 4 * kTcPanel;                                    // K and V of a tile
 constexpr int kTcRaw = 2 * kTcKeys * kHd + 2 * kTcKeys * 4;               // codes and scales of a tile
 constexpr int kFlush = 8;
-constexpr int kPlanned = 512;                                              // sequences whose work is laid out in a line
+constexpr int kPlanned = 448;                                              // sequences whose work is laid out in a line
 
 template <bool kTall, bool kCoded, bool kSplit>
 struct TcShape {
     static constexpr int kQTile = 4 * kTcPanel;                                      // 128 rows x 128
-    static constexpr int kQ = (kTall ? 2 : 1) * (kSplit || !kTall ? 2 : 1) * kQTile; // (64 KB at least where it serves the hand-over too)
+    static constexpr int kQ = (kTall ? 2 : 1) * (kSplit ? 2 : 1) * kQTile;
     static constexpr int kStages = kTall && kSplit ? 2 : kCoded ? 3 : 4;
-    static constexpr int kRaws = !kCoded ? 0 : kTall && kSplit ? 1 : 3;
-    static constexpr int kHead = 4096;                                               // barriers, the line of work, what stream 1 hands over
-    static constexpr int kScales = (kStages * 2 * kTcKeys * 4 + 1023) / 1024 * 1024;
+    static constexpr int kRaws = !kCoded ? 0 : kTall && kSplit ? 1 : kTall || kSplit ? 3 : 4;
+    static constexpr int kHead = 14848;                                              // barriers, the line of work, what stream 1 hands over
+    static constexpr int kScales = (kHead + kStages * 2 * kTcKeys * 4 + 1023) / 1024 * 1024 - kHead;
     static constexpr int kSmem = 1024 + kHead + kScales + kQ + kStages * kTcStage + kRaws * kTcRaw;
     static_assert(kSmem <= 232448, "shared memory of a block");
     // registers per thread: 256 softmax threads, 256 others; 65,536 together, what 512 threads of 128 start with
-    static constexpr int kRegsSoftmax = kSplit ? 208 : 152, kRegsOther = 256 - kRegsSoftmax;
-    static constexpr int kPiece = kSplit ? 16 : 32;                                  // columns of scores that a thread holds at once
+    static constexpr int kRegsSoftmax = 168, kRegsOther = 256 - kRegsSoftmax;
     // barriers
-    static constexpr int kFullQ = 0, kFullS = 1, kFullP = 5, kDoneO = 9, kDrain = 13, kGive = 14, kGiven = 15, kTaken = 16, kFullKV = 17,
+    static constexpr int kFullQ = 0, kFullS = 1, kFullP = 5, kDoneO = 9, kDrain = 13, kGive = 14, kTaken = 15, kFullKV = 16,
                          kEmptyKV = kFullKV + kStages, kBars = kEmptyKV + kStages;
 };
 
 // ------------------------------------------------------------------------------------------------------------------ work in a line
+struct Seq {
+    int first, nodes, tiles, groups;    // tiles of 64 positions, row groups; none: 0
+};
+__device__ __forceinline__ Seq seq_of(const Args& a, int m) {
+    Seq s{a.first[m], node_count(a, m), 0, 0};
+    if (s.first >= 0 && s.nodes > 0) {
+        s.tiles = ((int)min((long)s.first + s.nodes, (long)a.c.max_seq) + kTcKeys - 1) / kTcKeys;
+        s.groups = (s.nodes * a.group + a.group_rows - 1) / a.group_rows;
+    }
+    return s;
+}
 struct Part {
     int m, head, group, t0, t1, slot;   // slot < 0: the head's whole context
+    int first, nodes;
 };
-__device__ __forceinline__ int seq_end(const Args& a, int m, int nodes) { return (int)min((long)a.first[m] + nodes, (long)a.c.max_seq); }
-__device__ __forceinline__ int seq_tiles(const Args& a, int m, int* groups) {
-    const int nodes = node_count(a, m);
-    *groups = (nodes * a.group + a.group_rows - 1) / a.group_rows;
-    if (a.first[m] < 0 || nodes == 0) { *groups = 0; return 0; }
-    return (seq_end(a, m, nodes) + kTcKeys - 1) / kTcKeys;
+
+// (x, y) *= (fx, fy), as one instruction.
+__device__ __forceinline__ void mul2(float& x, float& y, float fx, float fy) {
+    asm("{\n\t.reg .b64 v, f;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 f, {%2, %3};\n\tmul.rn.f32x2 v, v, f;\n\tmov.b64 {%0, %1}, v;\n\t}" : "+f"(x), "+f"(y) : "f"(fx), "f"(fy));
+}
+// (x, y) = (x, y) * f + c and (x, y) += (a, b), as one instruction each.
+__device__ __forceinline__ void fma2(float& x, float& y, float f, float c) {
+    asm("{\n\t.reg .b64 v, f, c;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 f, {%2, %2};\n\tmov.b64 c, {%3, %3};\n\tfma.rn.f32x2 v, v, f, c;\n\tmov.b64 {%0, %1}, v;\n\t}"
+        : "+f"(x), "+f"(y) : "f"(f), "f"(c));
+}
+__device__ __forceinline__ void add2(float& x, float& y, float a, float b) {
+    asm("{\n\t.reg .b64 v, f;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 f, {%2, %3};\n\tadd.rn.f32x2 v, v, f;\n\tmov.b64 {%0, %1}, v;\n\t}" : "+f"(x), "+f"(y) : "f"(a), "f"(b));
+}
+// f16 high parts and remainders of a pair.
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    add2(x, y, -f.x, -f.y);
+    const __half2 l = __floats2half2_rn(x, y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+__device__ __forceinline__ void mul2(uint32_t& x, uint32_t& y, float fx, float fy) {
+    float a = __uint_as_float(x), b = __uint_as_float(y);
+    mul2(a, b, fx, fy);
+    x = __float_as_uint(a);
+    y = __float_as_uint(b);
+}
+
+__device__ __forceinline__ void store_o16(float* p, const float (&v)[16]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) reinterpret_cast<float4*>(p)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+}
+__device__ __forceinline__ void store_o16(__nv_bfloat16* p, const float (&v)[16]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        reinterpret_cast<uint4*>(p)[i] = make_uint4(lm::pack_bf16(v[8 * i], v[8 * i + 1]), lm::pack_bf16(v[8 * i + 2], v[8 * i + 3]),
+                                                    lm::pack_bf16(v[8 * i + 4], v[8 * i + 5]), lm::pack_bf16(v[8 * i + 6], v[8 * i + 7]));
 }
 
 template <bool kTall, bool kCoded, typename A>
@@ -68,10 +111,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
     static_assert((Sh::kHead + Sh::kScales) % 1024 == 0, "swizzled tiles start at 1,024 bytes");
     const uint32_t sq = smem_u32(q_area), skv = sq + Sh::kQ, sraw = skv + NS * kTcStage, bar0 = smem_u32(smem), flag = bar0 + 516;
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + 516);
-    int* s_cum = reinterpret_cast<int*>(smem + 768);               // [kPlanned + 1]
-    float2* s_ml = reinterpret_cast<float2*>(smem + 3072);         // [128]
+    int* s_cum = reinterpret_cast<int*>(smem + 768);               // [kPlanned]: tiles of all sequences before
+    Seq* s_seq = reinterpret_cast<Seq*>(smem + 2560);              // [kPlanned]
+    float4* s_ml = reinterpret_cast<float4*>(smem + 9728);         // [2][128] maximum, sum, scales that a stream shows the other
+    float* s_qf = reinterpret_cast<float*>(smem + 13824);          // [128] factors of the rows that both streams have
+    static_assert(768 + kPlanned * 4 <= 2560 && 2560 + kPlanned * sizeof(Seq) <= 9728 && 9728 + 4096 <= 13824 && 13824 + 512 <= Sh::kHead, "layout");
     float* s_scale = reinterpret_cast<float*>(smem + Sh::kHead);   // [stage][K 64, V 64]
-    float* s_vtop = reinterpret_cast<float*>(smem + 520);          // [stage][2]
+    float* s_vref = reinterpret_cast<float*>(smem + 520);          // [stage]: what the values' scales are relative to
     const int t = threadIdx.x, warp = __shfl_sync(0xffffffffu, t >> 5, 0), lane = t & 31;
     auto bar = [&](int i) { return bar0 + 8 * i; };
     auto wait = [&](int i, uint32_t parity) { mbar_wait_or_abort(bar(i), parity, flag); };
@@ -82,13 +128,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
             mbar_init(bar(Sh::kFullP + i), 4);
             mbar_init(bar(Sh::kDoneO + i), 1);
         }
-        mbar_init(bar(Sh::kDrain), 1);
-        mbar_init(bar(Sh::kGive), 128);
-        mbar_init(bar(Sh::kGiven), 128);
-        mbar_init(bar(Sh::kTaken), 128);
+        mbar_init(bar(Sh::kDrain), 2);
+        mbar_init(bar(Sh::kGive), 256);
+        mbar_init(bar(Sh::kTaken), 256);
         for (int i = 0; i < NS; ++i) {
             mbar_init(bar(Sh::kFullKV + i), 128);
-            mbar_init(bar(Sh::kEmptyKV + i), 1);
+            mbar_init(bar(Sh::kEmptyKV + i), kTall ? 2 : 1);
         }
         *abort_flag = 0;
         mbar_fence_init();
@@ -103,10 +148,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
     int line = 0;
     if (a.flat) {
         int* s_warp = reinterpret_cast<int*>(smem + 640);          // [16]
-        int groups, v = 0;
+        int v = 0;
         if (t < a.M) {
-            v = seq_tiles(a, t, &groups);
-            v *= groups * a.c.heads;
+            const Seq q = seq_of(a, t);
+            s_seq[t] = q;
+            v = q.tiles * q.groups * a.c.heads;
         }
         int sum = v;
 #pragma unroll
@@ -117,12 +163,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
         if (lane == 31) s_warp[warp] = sum;
         __syncthreads();
         int before = 0;
+#pragma unroll
         for (int w = 0; w < 16; ++w) {
-            before += w < warp ? s_warp[w] : 0;
-            line += s_warp[w];
+            const int u = s_warp[w];
+            before += w < warp ? u : 0;
+            line += u;
         }
         if (t < a.M) s_cum[t] = before + sum - v;
-        if (t == 0) s_cum[a.M] = line;
         if (blockIdx.x == 0) {                                     // for the merge
             if (t < a.M) a.cum[t] = before + sum - v;
             if (t <= a.blocks) a.cum[kPlanned + t] = (int)((long)line * t / a.blocks);
@@ -132,8 +179,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
     __syncthreads();
     tc::tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *reinterpret_cast<volatile uint32_t*>(smem + 512), 0);
-    const int c = blockIdx.x, x_first = a.flat ? (int)((long)line * c / gridDim.x) : 0, x_end = a.flat ? (int)((long)line * (c + 1) / gridDim.x) : 1;
-    // Part number 0, 1, ... of this block: false after the last.  x: where it starts in the line, moved on.
+    const int c = blockIdx.x, x_first = a.flat ? (int)((long)line * c / a.blocks) : c, x_end = a.flat ? (int)((long)line * (c + 1) / a.blocks) : a.pairs;
+    // Part number 0, 1, ... of this block: false after the last.  x: where it starts in the line, moved on; without a line, the number of a
+    // sequence's head and row group, every blocks-th of which is this block's, whole.
     auto next_part = [&](int& x, Part& p) {
         if (x >= x_end) return false;
         if (a.flat) {
@@ -142,47 +190,66 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
                 const int mid = (lo + hi + 1) >> 1;
                 if (s_cum[mid] <= x) lo = mid; else hi = mid - 1;
             }
+            const Seq q = s_seq[lo];
+            const uint32_t rel = x - s_cum[lo], pair = rel / (uint32_t)q.tiles;
             p.m = lo;
-            int groups;
-            const int tiles = seq_tiles(a, p.m, &groups), rel = x - s_cum[lo], pair = rel / tiles;
-            p.head = pair / groups;
-            p.group = pair - p.head * groups;
-            p.t0 = rel - pair * tiles;
-            p.t1 = min(tiles, p.t0 + x_end - x);
-            p.slot = p.t0 == 0 && p.t1 == tiles ? -1 : 2 * c + (x == x_first ? 0 : 1);
+            p.first = q.first;
+            p.nodes = q.nodes;
+            p.head = q.groups == 1 ? pair : pair / (uint32_t)q.groups;
+            p.group = pair - p.head * q.groups;
+            p.t0 = rel - pair * q.tiles;
+            p.t1 = min(q.tiles, p.t0 + x_end - x);
+            p.slot = p.t0 == 0 && p.t1 == q.tiles ? -1 : 2 * c + (x == x_first ? 0 : 1);
             x += p.t1 - p.t0;
             return true;
         }
-        x = 1;
-        int groups;
-        p.group = blockIdx.x % a.groups;
-        p.head = blockIdx.x / a.groups % a.c.heads;
-        p.m = blockIdx.x / a.groups / a.c.heads;
-        p.t0 = 0;
-        p.t1 = seq_tiles(a, p.m, &groups);
-        p.slot = -1;
-        return p.group < groups;
+        for (; x < x_end; x += a.blocks) {
+            const uint32_t mh = x / (uint32_t)a.groups;
+            p.group = x - mh * a.groups;
+            p.m = mh / (uint32_t)a.c.heads;
+            p.head = mh - p.m * a.c.heads;
+            const Seq q = seq_of(a, p.m);
+            if (p.group >= q.groups) continue;
+            p.first = q.first;
+            p.nodes = q.nodes;
+            p.t0 = 0;
+            p.t1 = q.tiles;
+            p.slot = -1;
+            x += a.blocks;
+            return true;
+        }
+        return false;
     };
-    // Jobs of a part: job n is tile n / 2 (kTall) or n and stream n & 1; job k of stream w is n = 2 k + w.
-    auto jobs_of = [&](const Part& p) { return (p.t1 - p.t0) * (kTall ? 2 : 1); };
+    // Jobs of a part for stream w: all its tiles (kTall), else tiles w, w + 2, ...
 
     if (warp >= 12) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Sh::kRegsOther));
-        if (warp == 12) {
-            // The whole warp walks the loop, one elected lane issues.
+        if (warp < 14) {
+            // A warp per stream; the whole warp walks the loop, one elected lane issues.  The scores of the next tile go out before this
+            // tile's second product.
             constexpr uint32_t id_s = tc::idesc_f16(kTcKeys), id_o = tc::idesc_f16(kHd, true);
             const bool elected = tc::elect_one();
-            int x = x_first, it0 = 0, kb[2] = {0, 0}, nth = 0;
+            const int w = warp - 12;
+            const uint32_t acc = tmem + w * 256, q = sq + (kTall ? w : 0) * (kSplit ? 2 : 1) * Sh::kQTile;
+            int x = x_first, kb = 0, nth = 0, st_s = 0, st_o = 0;  // stages of the next scores, of the next second product
+            uint32_t lap = 0;                                      // parity of the next scores' stage
             Part p;
+            auto walk = [&](int by) {
+                st_s += by;
+                if (st_s >= NS) {
+                    st_s -= NS;
+                    lap ^= 1;
+                }
+            };
             for (; next_part(x, p) && !*abort_flag; ++nth) {
-                const int jobs = jobs_of(p);
-                auto scores = [&](int n) {
-                    const int w = n & 1, kk = kb[w] + (n >> 1), b = kk & 1, it = it0 + (kTall ? n >> 1 : n), st = it % NS;
+                const int tiles = p.t1 - p.t0, jobs = kTall ? tiles : (tiles + 1 - w) >> 1;
+                auto scores = [&](int k) {
+                    const int kk = kb + k, b = kk & 1;
                     if (kk > 1) wait(Sh::kDoneO + 2 * w + b, ((kk - 2) >> 1) & 1);   // the P that lay there has been multiplied
-                    wait(Sh::kFullKV + st, (it / NS) & 1);
+                    wait(Sh::kFullKV + st_s, lap);
                     tc::tc_fence_after();
                     if (elected) {
-                        const uint32_t d = tmem + w * 256 + b * 64, q = sq + (kTall ? w : 0) * (kSplit ? 2 : 1) * Sh::kQTile, k = skv + st * kTcStage;
+                        const uint32_t d = acc + b * 64, kt = skv + st_s * kTcStage;
 #pragma unroll
                         for (int part = 0; part < (kSplit ? 2 : 1); ++part)
 #pragma unroll
@@ -190,22 +257,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
 #pragma unroll
                                 for (int e = 0; e < 4; ++e)   // 16 dimensions = 32 bytes further inside the swizzle atom
                                     tc::tc_mma_bf16(d, tc::flash_desc(q + part * Sh::kQTile + pan * 2 * kTcPanel, 16, 1024) + 2 * e,
-                                                    tc::flash_desc(k + pan * kTcPanel, 16, 1024) + 2 * e, id_s, part + pan + e > 0 ? 1u : 0u);
+                                                    tc::flash_desc(kt + pan * kTcPanel, 16, 1024) + 2 * e, id_s, part + pan + e > 0 ? 1u : 0u);
                         tc::tc_commit(bar(Sh::kFullS + 2 * w + b));
                     }
                     __syncwarp();
+                    walk(kTall ? 1 : 2);
                 };
+                if (!kTall && w == 1) walk(1);
+                st_o = st_s;
                 wait(Sh::kFullQ, nth & 1);
                 tc::tc_fence_after();
-                scores(0);
-                if (jobs > 1) scores(1);
-                for (int n = 0; n < jobs && !*abort_flag; ++n) {
-                    if (n + 2 < jobs) scores(n + 2);
-                    const int w = n & 1, k = n >> 1, kk = kb[w] + k, b = kk & 1, it = it0 + (kTall ? n >> 1 : n), st = it % NS;
+                if (jobs > 0) scores(0);
+                for (int k = 0; k < jobs && !*abort_flag; ++k) {
+                    if (k + 1 < jobs) scores(k + 1);
+                    const int kk = kb + k, b = kk & 1;
                     wait(Sh::kFullP + 2 * w + b, (kk >> 1) & 1);
                     tc::tc_fence_after();
                     if (elected) {
-                        const uint32_t pa = tmem + w * 256 + b * 64, o = tmem + w * 256 + 128, v = skv + st * kTcStage + 2 * kTcPanel;
+                        const uint32_t pa = acc + b * 64, o = acc + 128, v = skv + st_o * kTcStage + 2 * kTcPanel;
                         const bool fresh = kSplit ? k % kFlush == 0 : k == 0;
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {   // 16 positions: two 8-row groups
@@ -215,13 +284,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
                             if (kSplit) tc::tc_mma_bf16_ta(o, at + 8, vd, id_o, 1u);
                         }
                         tc::tc_commit(bar(Sh::kDoneO + 2 * w + b));
-                        if (!kTall || w == 1) tc::tc_commit(bar(Sh::kEmptyKV + st));
+                        tc::tc_commit(bar(Sh::kEmptyKV + st_o));
                     }
                     __syncwarp();
+                    st_o += kTall ? 1 : 2;
+                    if (st_o >= NS) st_o -= NS;
                 }
-                it0 += p.t1 - p.t0;
-                kb[0] += (jobs + 1) >> 1;
-                kb[1] += jobs >> 1;
+                // to the first stage after the part: a stream's scores stand behind its last tile and the next but one
+                if (!kTall && jobs > 0 && ((tiles ^ w) & 1) == 1) {   // one too far
+                    if (st_s == 0) lap ^= 1;
+                    st_s = st_s == 0 ? NS - 1 : st_s - 1;
+                }
+                kb += jobs;
             }
             if (elected) tc::tc_commit(bar(Sh::kDrain));   // whatever became of the others: no MMA in flight when the tensor memory is freed
             __syncwarp();
@@ -236,53 +310,73 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
         // that leaves may be asked for ahead of it.
         constexpr int kAhead = kCoded ? Sh::kRaws : kTall ? NS - 1 : NS - 2;
         static_assert(NS >= (kTall ? 2 : 3) && kAhead >= 1, "stages");
-        int xi = x_first, xo = x_first, it_in = 0, it_out = 0;
+        int xi = x_first, xo = x_first, it_in = 0, it_out = 0, st_in = 0, st_out = 0, raw_in = 0, raw_out = 0;
+        uint32_t lap_in = 1, lap_out = 1;                          // parity of the stages' next release
         Part in{}, out{};
-        int in_tile = 0, out_tile = 0;
         bool in_more = next_part(xi, in), out_more = next_part(xo, out);
-        in_tile = in.t0;
-        out_tile = out.t0;
-        int ctx = 0, end = 0;
+        int in_tile = in.t0, out_tile = out.t0, ctx = 0, end = 0;
         unsigned long long any = 0;
-        const unsigned char *kp = nullptr, *vp = nullptr;
+        const unsigned char *kp = nullptr, *vp = nullptr;          // this thread's piece of the part's first row
         size_t row0 = 0;
         auto open_part = [&]() {                                   // what the sequence's rows see
-            const int nodes = node_count(a, in.m);
-            ctx = min(a.first[in.m], a.c.max_seq);
-            end = seq_end(a, in.m, nodes);
-            const unsigned long long mine = (lane < nodes ? mask_of(a, in.m, lane, nodes) : 0) | (lane + 32 < nodes ? mask_of(a, in.m, lane + 32, nodes) : 0);
-            any = (unsigned long long)__reduce_or_sync(0xffffffffu, (uint32_t)(mine >> 32)) << 32 | __reduce_or_sync(0xffffffffu, (uint32_t)mine);
+            const int nodes = in.nodes;
+            ctx = min(in.first, a.c.max_seq);
+            end = (int)min((long)in.first + nodes, (long)a.c.max_seq);
+            any = 0;
+            if (in.t1 * kTcKeys > ctx) {
+                const unsigned long long mine = (lane < nodes ? mask_of(a, in.m, lane, nodes) : 0) | (lane + 32 < nodes ? mask_of(a, in.m, lane + 32, nodes) : 0);
+                any = (unsigned long long)__reduce_or_sync(0xffffffffu, (uint32_t)(mine >> 32)) << 32 | __reduce_or_sync(0xffffffffu, (uint32_t)mine);
+            }
             row0 = a.c.row(in.m, in.head, 0);
-            kp = a.c.k + row0 * kRowBytes;
-            vp = a.c.v + row0 * kRowBytes;
+            kp = a.c.k + (row0 + r0) * kRowBytes + pc * 16;
+            vp = a.c.v + (row0 + r0) * kRowBytes + pc * 16;
         };
+        // where this thread's piece of row r0 goes; the others are kStep rows on (binary16: swizzled, kStep = 8 keeps a row's low bits)
+        const uint32_t place = kCoded ? r0 * kHd + pc * 16 : (pc >> 3) * kTcPanel + r0 * 128 + (((pc & 7) ^ (r0 & 7)) << 4);
+        constexpr uint32_t kSideOff = kCoded ? kTcKeys * kHd : 2 * kTcPanel, kRowOff = kStep * 128;
         auto issue = [&]() {                                       // the next tile on its way
             if (in_more) {
                 if (in_tile == in.t0) open_part();
                 const int p0 = in_tile * kTcKeys;
-                const bool all = p0 + kTcKeys <= ctx;
-                if (!kCoded) wait(Sh::kEmptyKV + it_in % NS, (it_in / NS & 1) ^ 1);
-                const uint32_t to = kCoded ? sraw + it_in % max(Sh::kRaws, 1) * kTcRaw : skv + it_in % NS * kTcStage;
+                if (!kCoded) wait(Sh::kEmptyKV + st_in, lap_in);
+                const uint32_t to = kCoded ? sraw + raw_in * kTcRaw : skv + st_in * kTcStage;
+                const unsigned char *k = kp + (size_t)p0 * kRowBytes, *v = vp + (size_t)p0 * kRowBytes;
+                if (p0 + kTcKeys <= ctx) {
 #pragma unroll
-                for (int i = 0; i < kRows; ++i) {
-                    const int r = r0 + kStep * i, p = p0 + r;
-                    const bool there = all || p < ctx || (p < end && (any >> (p - ctx) & 1));
-                    const size_t from = (size_t)(there ? p : 0) * kRowBytes + pc * 16;
-                    if (kCoded) {
-                        lm::cp_async16z(to + r * kHd + pc * 16, kp + from, there);
-                        lm::cp_async16z(to + kTcKeys * kHd + r * kHd + pc * 16, vp + from, there);
-                    } else {
-                        const uint32_t at = to + (pc >> 3) * kTcPanel + r * 128 + (((pc & 7) ^ (r & 7)) << 4);
-                        lm::cp_async16z(at, kp + from, there);
-                        lm::cp_async16z(at + 2 * kTcPanel, vp + from, there);
+                    for (int i = 0; i < kRows; ++i) {
+                        amma::cp_async16(to + place + i * kRowOff, k + i * kStep * kRowBytes);
+                        amma::cp_async16(to + place + kSideOff + i * kRowOff, v + i * kStep * kRowBytes);
+                    }
+                    if (kCoded && (warp & 1) == 0) {               // warp 8 the keys' scales, warp 10 the values'
+                        const float* f = (warp == 8 ? a.c.ks : a.c.vs) + row0 + p0 + lane;
+                        tc::cp_async4(to + 2 * kTcKeys * kHd + (warp - 8) * 128 + lane * 4, f, 4);
+                        tc::cp_async4(to + 2 * kTcKeys * kHd + (warp - 8) * 128 + 128 + lane * 4, f + 32, 4);
+                    }
+                } else {
+                    auto there = [&](int p) { return p < ctx || (p < end && (any >> (p - ctx) & 1)); };
+#pragma unroll 1
+                    for (int i = 0; i < kRows; ++i) {
+                        const bool in_seq = there(p0 + r0 + kStep * i);
+                        lm::cp_async16z(to + place + i * kRowOff, in_seq ? k + i * kStep * kRowBytes : kp, in_seq);
+                        lm::cp_async16z(to + place + kSideOff + i * kRowOff, in_seq ? v + i * kStep * kRowBytes : vp, in_seq);
+                    }
+                    if (kCoded && (warp & 1) == 0) {
+#pragma unroll 1
+                        for (int i = 0; i < 2; ++i) {
+                            const int p = p0 + lane + 32 * i;
+                            const bool in_seq = there(p);
+                            tc::cp_async4(to + 2 * kTcKeys * kHd + (warp - 8) * 128 + 128 * i + lane * 4,
+                                          (warp == 8 ? a.c.ks : a.c.vs) + row0 + (in_seq ? p : 0), in_seq ? 4 : 0);
+                        }
                     }
                 }
-                if (kCoded) {
-                    const int p = p0 + (u & 63);
-                    const bool there = all || p < ctx || (p < end && (any >> (p - ctx) & 1));
-                    tc::cp_async4(to + 2 * kTcKeys * kHd + u * 4, (u < 64 ? a.c.ks : a.c.vs) + row0 + (there ? p : 0), there ? 4 : 0);
-                }
                 ++it_in;
+                if (kCoded) {
+                    raw_in = raw_in == Sh::kRaws - 1 ? 0 : raw_in + 1;
+                } else if (++st_in == NS) {
+                    st_in = 0;
+                    lap_in ^= 1;
+                }
                 if (++in_tile == in.t1) {
                     in_more = next_part(xi, in);
                     in_tile = in.t0;
@@ -290,43 +384,60 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
             }
             lm::cp_async_commit();
         };
+        float vref = 0.f;                                          // warp 10: the largest value scale of the part so far, a power of two
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) issue();
         while (out_more && !*abort_flag) {
-            const int st = it_out % NS;
+            const int st = st_out;
             lm::cp_async_wait<kAhead - 1>();
             if (kCoded) {
-                wait(Sh::kEmptyKV + st, (it_out / NS & 1) ^ 1);
-                const uint32_t from = sraw + it_out % max(Sh::kRaws, 1) * kTcRaw, to = skv + st * kTcStage;
-                const float* fs = reinterpret_cast<const float*>(smem + (from - bar0) + 2 * kTcKeys * kHd);
-                const float sc = fs[u];
-                s_scale[st * 2 * kTcKeys + u] = sc;
-                if (warp >= 10) {
-                    const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(sc)));
-                    if (lane == 0) s_vtop[2 * st + warp - 10] = __uint_as_float(top);
+                wait(Sh::kEmptyKV + st, lap_out);
+                const uint32_t from = sraw + raw_out * kTcRaw, to = skv + st * kTcStage;
+                if ((warp & 1) == 0) {
+                    // The scales, by whom copied them.  A value's is given relative to the largest one met so far in the part.
+                    const float* fs = reinterpret_cast<const float*>(smem + (from - bar0) + 2 * kTcKeys * kHd) + (warp - 8) * 32 + lane;
+                    float s0 = fs[0], s1 = fs[32];
+                    if (warp == 10) {
+                        if (out_tile == out.t0) vref = __uint_as_float(2u << 23);
+                        const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fabsf(s0), fabsf(s1)))));
+                        if (top > vref) vref = __uint_as_float(min((__float_as_uint(top) + 0x7FFFFFu) & 0x7F800000u, 252u << 23));
+                        const float inv = __uint_as_float((254u << 23) - __float_as_uint(vref));
+                        s0 *= inv;
+                        s1 *= inv;
+                        if (lane == 0) s_vref[st] = vref;
+                    }
+                    s_scale[st * 2 * kTcKeys + (warp - 8) * 32 + lane] = s0;
+                    s_scale[st * 2 * kTcKeys + (warp - 8) * 32 + lane + 32] = s1;
                 }
+                // dimensions 16 pc ...: pieces 2 (pc & 3), + 1 of panel pc / 4; the second panel's threads store the odd one first (banks)
+                const int odd = pc >> 2;
+                const uint32_t base = to + odd * kTcPanel + r0 * 128;
+                const uint32_t c0 = base + (((2 * (pc & 3) + odd) ^ (r0 & 7)) << 4), c1 = base + (((2 * (pc & 3) + 1 - odd) ^ (r0 & 7)) << 4);
 #pragma unroll
                 for (int side = 0; side < 2; ++side)
 #pragma unroll
-                    for (int i = 0; i < kRows; ++i) {
-                        const int r = r0 + kStep * i;
-                        uint4 w;
+                    for (int i = 0; i < kRows; ++i) {              // rows r0 + 16 i: the same low bits
+                        uint4 w, lo, hi;
                         asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
-                                     : "r"(from + side * kTcKeys * kHd + r * kHd + pc * 16));
-                        uint4 lo = make_uint4(codes_f16x2(w.x), codes_f16x2(w.x >> 16), codes_f16x2(w.y), codes_f16x2(w.y >> 16));
-                        uint4 hi = make_uint4(codes_f16x2(w.z), codes_f16x2(w.z >> 16), codes_f16x2(w.w), codes_f16x2(w.w >> 16));
-                        // dimensions 16 pc ...: pieces 2 (pc & 3), + 1 of panel pc / 4; the second panel's threads store the odd one first (banks)
-                        const uint32_t base = to + side * 2 * kTcPanel + (pc >> 2) * kTcPanel + r * 128;
-                        const int odd = pc >> 2;
-                        const uint32_t c0 = base + (((2 * (pc & 3) + odd) ^ (r & 7)) << 4), c1 = base + (((2 * (pc & 3) + 1 - odd) ^ (r & 7)) << 4);
+                                     : "r"(from + place + side * kSideOff + i * kRowOff));
+                        codes_f16(w.x, lo.x, lo.y);
+                        codes_f16(w.y, lo.z, lo.w);
+                        codes_f16(w.z, hi.x, hi.y);
+                        codes_f16(w.w, hi.z, hi.w);
                         const uint4 first = odd ? hi : lo, second = odd ? lo : hi;
-                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(c0), "r"(first.x), "r"(first.y), "r"(first.z), "r"(first.w) : "memory");
-                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(c1), "r"(second.x), "r"(second.y), "r"(second.z), "r"(second.w) : "memory");
+                        const uint32_t at = side * 2 * kTcPanel + i * kRowOff;
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(c0 + at), "r"(first.x), "r"(first.y), "r"(first.z), "r"(first.w) : "memory");
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(c1 + at), "r"(second.x), "r"(second.y), "r"(second.z), "r"(second.w) : "memory");
                     }
+                raw_out = raw_out == Sh::kRaws - 1 ? 0 : raw_out + 1;
             }
             fence_proxy_async();
             mbar_arrive(bar(Sh::kFullKV + st));
             ++it_out;
+            if (++st_out == NS) {
+                st_out = 0;
+                lap_out ^= 1;
+            }
             if (++out_tile == out.t1) {
                 out_more = next_part(xo, out);
                 out_tile = out.t0;
@@ -339,163 +450,205 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
         // ---- softmax, a thread per row of the stream's accumulator
         const int w = warp >> 2, rt = t & 127;
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16) + w * 256;
-        int x = x_first, it0 = 0, kb = 0, nth = 0;
+        // fp32: O of the tiles before, [column][row], relative to the maximum and scale that it had then
+        float* kept = kSplit ? a.kept + ((size_t)c * 2 + w) * kHd * 128 + rt : nullptr;
+        int x = x_first, st = 0, kb = 0, nth = 0;
+        uint32_t lap = 0;
         Part p;
         for (; next_part(x, p) && !*abort_flag; ++nth) {
-            const int nodes = node_count(a, p.m), ctx = min(a.first[p.m], a.c.max_seq);
-            const int rows = nodes * a.group - p.group * a.group_rows - (kTall ? w * 128 : 0);   // of this stream, from its first lane on
-            const bool active = (warp & 3) * 32 < rows, mine = rt < rows;
-            const int row = p.group * a.group_rows + (kTall ? w * 128 : 0) + rt, node = mine ? row / a.group : 0;
-            const unsigned long long mask = mine ? mask_of(a, p.m, node, nodes) & low_bits(seq_end(a, p.m, nodes) - ctx) : 0;
-            // ---- the warp's query rows, the largest element of each brought to 1 .. 2: a row at a time, four dimensions a lane.  kTall: the
-            // stream's own rows, else panel w of the rows that both streams have.
+            const int ctx = min(p.first, a.c.max_seq), r0 = (warp & 3) * 32;
+            const int grow = p.group * a.group_rows + (kTall ? w * 128 : 0) + r0;      // the warp's first row, of the head's
+            const int nn = min(32, p.nodes * a.group - grow);                          // and how many it has
+            const bool active = nn > 0;
+            // ---- the query rows, the largest element of each brought to 1 .. 2.  A warp copies its 32 rows, whole lines at a time, to where the
+            // operand will lie (a row of bf16 takes the place of its f16, one of fp32 that of high parts and remainders); then a thread takes a
+            // row.  kTall: each stream its own rows, else stream 0 those of both.
             float qf = 0.f;
-            if (!kTall && nth > 0) wait(Sh::kTaken, (nth - 1) & 1);   // all rows of the hand-over have been read
-            if (active) {
-                const uint32_t tile = sq + (kTall ? w : 0) * (kSplit ? 2 : 1) * Sh::kQTile + (lane >> 4) * 2 * kTcPanel + (lane & 1) * 8;
-                const int r0 = (warp & 3) * 32, grow = p.group * a.group_rows + (kTall ? w * 128 : 0) + r0;
-                const A* q = static_cast<const A*>(a.q) + ((size_t)p.m * a.T * a.nq + p.head * a.group) * kHd + 4 * lane;
-                const int nn = min(32, rows - r0);
-                int nd = grow / a.group, hd = grow - nd * a.group;        // node and head of row i, walked along
-#pragma unroll 1
-                for (int i0 = 0; i0 < 32; i0 += 8) {
-                    float4 v[8];
+            unsigned long long mask = 0;
+            const bool mine = lane < nn;
+            const uint32_t node = (uint32_t)(grow + lane) / (uint32_t)a.group;
+            const size_t at_row = (((size_t)p.m * a.T + node) * a.nq + p.head * a.group + grow + lane - node * a.group) * kHd;
+            if (!kTall && nth > 0) wait(Sh::kTaken, (nth - 1) & 1);   // O of both streams has been read
+            if (mine) mask = mask_of(a, p.m, node, p.nodes) & low_bits((int)min((long)p.first + p.nodes, (long)a.c.max_seq) - ctx);
+            if (active && (kTall || w == 0)) {
+                constexpr int kLanes = kHd * (int)sizeof(A) / 16, kAtOnce = 32 / kLanes;   // lanes of a row, rows at once
+                const uint32_t tile = sq + (kTall ? w : 0) * (kSplit ? 2 : 1) * Sh::kQTile + r0 * 128;
+                // piece j of row i: 1,024 bytes apart are rows 8 apart, 16 KB panels; within a row's 128 bytes swizzled
+                auto place = [&](int i, int j) { return tile + (j >> 3) * 2 * kTcPanel + i * 128 + (((j & 7) ^ (i & 7)) << 4); };
+                const int piece = lane % kLanes;
+                int row = lane / kLanes, nd = (uint32_t)(grow + row) / (uint32_t)a.group, hd = grow + row - nd * a.group;
+                const A* q = static_cast<const A*>(a.q) + (((size_t)p.m * a.T + nd) * a.nq + p.head * a.group + hd) * kHd + piece * (16 / (int)sizeof(A));
+                const size_t skip = (size_t)(a.nq - a.group) * kHd;
+#pragma unroll 4
+                for (; row < nn; row += kAtOnce) {
+                    amma::cp_async16(place(row, piece), q);
+                    q += kAtOnce * kHd;
+                    for (hd += kAtOnce; hd >= a.group; hd -= a.group) q += skip;
+                }
+                lm::cp_async_commit();
+                lm::cp_async_wait<0>();
+                __syncwarp();
+                if (mine) {
+                    uint4 raw[kLanes];
+                    float mx[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        v[i] = i0 + i < nn ? load_q4(q + ((size_t)nd * a.nq + hd) * kHd) : make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (++hd == a.group) { hd = 0; ++nd; }
+                    for (int j = 0; j < kLanes; ++j) {
+                        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(raw[j].x), "=r"(raw[j].y), "=r"(raw[j].z), "=r"(raw[j].w) : "r"(place(lane, j)));
+                        const uint32_t u[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            mx[e] = kSplit ? fmaxf(mx[e], fabsf(__uint_as_float(u[e])))
+                                           : fmaxf(fmaxf(mx[e], fabsf(__uint_as_float(u[e] << 16))), fabsf(__uint_as_float(u[e] & 0xFFFF0000u)));
                     }
+                    const float2 unit = binade(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+                    qf = unit.x * (0.08838834764831845f * 1.4426950408889634f);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float top = fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w)));
-                        const float2 unit = binade(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top))));
-                        if (lane == i0 + i) qf = unit.x * (0.08838834764831845f * 1.4426950408889634f);
-                        uint32_t h[2], l[2];
-                        amma::split_hi_lo(v[i].x * unit.y, v[i].y * unit.y, h[0], l[0]);
-                        amma::split_hi_lo(v[i].z * unit.y, v[i].w * unit.y, h[1], l[1]);
-                        const int r = r0 + i0 + i;
-                        const uint32_t to = tile + r * 128 + (((lane >> 1 & 7) ^ (r & 7)) << 4);
-                        if (kTall || lane >> 4 == w) {
-                            asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to), "r"(h[0]), "r"(h[1]) : "memory");
-                            if (kSplit) asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to + Sh::kQTile), "r"(l[0]), "r"(l[1]) : "memory");
+                    for (int ch = 0; ch < 16; ++ch) {              // eight dimensions
+                        float v[8];
+                        if (kSplit) {
+                            const uint4 x = raw[(2 * ch) % kLanes], y = raw[(2 * ch + 1) % kLanes];
+                            v[0] = __uint_as_float(x.x); v[1] = __uint_as_float(x.y); v[2] = __uint_as_float(x.z); v[3] = __uint_as_float(x.w);
+                            v[4] = __uint_as_float(y.x); v[5] = __uint_as_float(y.y); v[6] = __uint_as_float(y.z); v[7] = __uint_as_float(y.w);
+                        } else {
+                            const uint4 x = raw[ch % kLanes];
+                            const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                v[2 * e] = __uint_as_float(u[e] << 16);
+                                v[2 * e + 1] = __uint_as_float(u[e] & 0xFFFF0000u);
+                            }
                         }
+                        uint32_t h[4], l[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            mul2(v[2 * e], v[2 * e + 1], unit.y, unit.y);
+                            if (kSplit) {
+                                amma::split_hi_lo(v[2 * e], v[2 * e + 1], h[e], l[e]);
+                            } else {
+                                const __half2 f = __floats2half2_rn(v[2 * e], v[2 * e + 1]);
+                                h[e] = *reinterpret_cast<const uint32_t*>(&f);
+                            }
+                        }
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(place(lane, ch)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+                        if (kSplit)
+                            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(place(lane, ch) + Sh::kQTile), "r"(l[0]), "r"(l[1]), "r"(l[2]), "r"(l[3]) : "memory");
                     }
                 }
+                if (!kTall) s_qf[rt] = qf;
             }
             fence_proxy_async();
             mbar_arrive(bar(Sh::kFullQ));
-            float m = -FLT_MAX, l = 0.f, vref = __uint_as_float(2u << 23);
-            float kept[kSplit ? kHd : 1];
-            if (kSplit) {
-#pragma unroll
-                for (int i = 0; i < (kSplit ? kHd : 1); ++i) kept[i] = 0.f;
+            if (!kTall && w == 1) {
+                wait(Sh::kFullQ, nth & 1);
+                if (mine) qf = s_qf[rt];
             }
-            const int jobs = (jobs_of(p) + 1 - w) >> 1;
+            float m = -FLT_MAX, l = 0.f, vref = 1.f, m_kept = -FLT_MAX, v_kept = 1.f;
+            bool has_kept = false;
+            const int tiles = p.t1 - p.t0, jobs = kTall ? tiles : (tiles + 1 - w) >> 1;
+            auto walk = [&]() {                               // a tile on in the ring of stages
+                if (++st == NS) {
+                    st = 0;
+                    lap ^= 1;
+                }
+            };
+            if (!kTall && w == 1) walk();
             for (int k = 0; k < jobs && !*abort_flag; ++k) {
-                const int kk = kb + k, b = kk & 1, rel = kTall ? k : 2 * k + w, it = it0 + rel, st = it % NS, p0 = (p.t0 + rel) * kTcKeys;
+                const int kk = kb + k, b = kk & 1, p0 = (p.t0 + (kTall ? k : 2 * k + w)) * kTcKeys;
                 const uint32_t at = lanes + b * 64;
                 wait(Sh::kFullS + 2 * w + b, (kk >> 1) & 1);
                 if (kk > 1) wait(Sh::kDoneO + 2 * w + b, ((kk - 2) >> 1) & 1);   // long done; no phase of it goes by unseen
-                if (kCoded) wait(Sh::kFullKV + st, (it / NS) & 1);               // (long full: the scales)
+                if (kCoded) wait(Sh::kFullKV + st, lap);                         // (long full: the scales)
                 tc::tc_fence_after();
-                if (kSplit && k > 0 && k % kFlush == 0 && active) {             // O so far to registers; the next product starts afresh
-                    wait(Sh::kDoneO + 2 * w + (b ^ 1), ((kk - 1) >> 1) & 1);
-                    tc::tc_fence_after();
-#pragma unroll
-                    for (int d = 0; d < (kSplit ? kHd : 0); d += 32) {
-                        uint32_t o[32];
-                        tc::tmem_ld32(lanes + 128 + d, o);
-                        tc::tmem_wait_ld();
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) kept[d + i] += __uint_as_float(o[i]);
-                    }
-                }
                 if (active) {
+                    uint32_t r[64];
+                    tc::tmem_ld32(at, r);
+                    tc::tmem_ld32(at + 32, r + 32);
+                    if (kSplit && k > 0 && k % kFlush == 0) {                    // O so far to the sum; the next product starts afresh
+                        wait(Sh::kDoneO + 2 * w + (b ^ 1), ((kk - 1) >> 1) & 1);
+                        tc::tc_fence_after();
+                        const float f = has_kept ? lm::exp2_fast(m_kept - m) * (v_kept * __uint_as_float((254u << 23) - __float_as_uint(vref))) : 0.f;
+#pragma unroll 1
+                        for (int d = 0; d < kHd; d += 16) {
+                            uint32_t o[16];
+                            float old[16];
+                            tc::tmem_ld16(lanes + 128 + d, o);
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) old[i] = has_kept ? kept[(d + i) * 128] : 0.f;
+                            tc::tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) kept[(d + i) * 128] = fmaf(old[i], f, __uint_as_float(o[i]));
+                        }
+                        has_kept = true;
+                        m_kept = m;
+                        v_kept = vref;
+                    }
+                    tc::tmem_wait_ld();
                     const float* ks = s_scale + st * 2 * kTcKeys;
                     const float* vs = ks + kTcKeys;
-                    const bool tail = p0 + kTcKeys > ctx;
-                    unsigned long long vis = ~0ull;
-                    if (tail) vis = p0 >= ctx ? (p0 - ctx < 64 ? mask >> (p0 - ctx) : 0) : low_bits(ctx - p0) | mask << (ctx - p0);
-                    constexpr int kPiece = Sh::kPiece;
-                    auto scores = [&](int i0, float (&s)[kPiece]) {      // of positions i0 ..., times the keys' scales
-                        uint32_t r[kPiece];
-                        if constexpr (kPiece == 32) tc::tmem_ld32(at + i0, r);
-                        else tc::tmem_ld16(at + i0, r);
-                        tc::tmem_wait_ld();
+                    if (kCoded) {
 #pragma unroll
-                        for (int i = 0; i < kPiece; i += 4) {
-                            float4 f = make_float4(1.f, 1.f, 1.f, 1.f);
-                            if (kCoded) f = *reinterpret_cast<const float4*>(ks + i0 + i);
-                            s[i] = __uint_as_float(r[i]); s[i + 1] = __uint_as_float(r[i + 1]);
-                            s[i + 2] = __uint_as_float(r[i + 2]); s[i + 3] = __uint_as_float(r[i + 3]);
-                            if (kCoded) { s[i] *= f.x; s[i + 1] *= f.y; s[i + 2] *= f.z; s[i + 3] *= f.w; }
+                        for (int i = 0; i < 64; i += 4) {
+                            const float4 f = *reinterpret_cast<const float4*>(ks + i);
+                            mul2(r[i], r[i + 1], f.x, f.y);
+                            mul2(r[i + 2], r[i + 3], f.z, f.w);
                         }
-                        if (tail) {
-                            const uint32_t bits = (uint32_t)(vis >> i0);
-#pragma unroll
-                            for (int i = 0; i < kPiece; ++i)
-                                if (!(bits >> i & 1)) s[i] = -INFINITY;
-                        }
-                    };
-                    float s[kPiece], mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                    for (int i0 = 0; i0 < kTcKeys; i0 += kPiece) {
-                        scores(i0, s);
-#pragma unroll
-                        for (int i = 0; i < kPiece; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
                     }
-                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * qf;
-                    float vtop = vref;
-                    if (kCoded) vtop = fmaxf(s_vtop[2 * st], s_vtop[2 * st + 1]);
-                    if (__any_sync(0xffffffffu, top > m + kSlack || vtop > vref)) {
-                        float f = 1.f;
-                        if (kCoded && vtop > vref) {
-                            const float to = __uint_as_float(min((__float_as_uint(vtop) + 0x7FFFFFu) & 0x7F800000u, 252u << 23));
-                            f = vref * __uint_as_float((254u << 23) - __float_as_uint(to));
-                            vref = to;
-                        }
-                        const float to = fmaxf(m, top - kHead), e = lm::exp2_fast(m - to);
-                        m = to;
-                        l *= e;
-                        f *= e;
-                        if (kSplit) {
+                    if (p0 + kTcKeys > ctx) {                                    // masks where the tile reaches the nodes
+                        const unsigned long long vis = p0 >= ctx ? (p0 - ctx < 64 ? mask >> (p0 - ctx) : 0) : low_bits(ctx - p0) | mask << (ctx - p0);
 #pragma unroll
-                            for (int i = 0; i < (kSplit ? kHd : 1); ++i) kept[i] *= f;
-                        }
+                        for (int i = 0; i < 64; ++i)
+                            if (!(vis >> i & 1)) r[i] = 0xFF800000u;
+                    }
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int i = 0; i < 64; i += 8)
+#pragma unroll
+                        for (int d = 0; d < 4; ++d) mx[d] = fmaxf(fmaxf(mx[d], __uint_as_float(r[i + d])), __uint_as_float(r[i + 4 + d]));
+                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * qf;
+                    const float vnew = kCoded ? s_vref[st] : 1.f;
+                    if (__any_sync(0xffffffffu, top > m + kSlack || vnew != vref)) {
+                        const float to = fmaxf(m, top - kHead), e = lm::exp2_fast(m - to);
+                        const float f = kCoded && vnew != vref ? e * vref * __uint_as_float((254u << 23) - __float_as_uint(vnew)) : e;
+                        m = to;
+                        vref = vnew;
+                        l *= e;
                         if (kSplit ? k % kFlush != 0 : k > 0) {
                             wait(Sh::kDoneO + 2 * w + (b ^ 1), ((kk - 1) >> 1) & 1);   // O is complete up to the tile before
                             tc::tc_fence_after();
-#pragma unroll
-                            for (int d = 0; d < kHd; d += 32) {
-                                uint32_t o[32];
-                                tc::tmem_ld32(lanes + 128 + d, o);
+#pragma unroll 1
+                            for (int d = 0; d < kHd; d += 16) {
+                                uint32_t o[16];
+                                tc::tmem_ld16(lanes + 128 + d, o);
                                 tc::tmem_wait_ld();
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                                tc::tmem_st32(lanes + 128 + d, o);
+                                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                                tc::tmem_st16(lanes + 128 + d, o);
                             }
                         }
                     }
-                    const float vdiv = kCoded ? __uint_as_float((254u << 23) - __float_as_uint(vref)) : 1.f;
                     float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int i0 = 0; i0 < kTcKeys; i0 += kPiece) {       // P over the same columns, 16 of them: high parts, then (fp32) remainders
-                        scores(i0, s);
+                    for (int i0 = 0; i0 < 64; i0 += kSplit ? 16 : 32) {  // P over the columns of 16 (fp32: then its remainders) or 32 positions
                         uint32_t h[16];
 #pragma unroll
-                        for (int i = 0; i < kPiece; i += 4) {
-                            float4 f = make_float4(1.f, 1.f, 1.f, 1.f);
-                            if (kCoded) f = *reinterpret_cast<const float4*>(vs + i0 + i);
+                        for (int i = 0; i < (kSplit ? 16 : 32); i += 4) {
                             float e[4];
 #pragma unroll
-                            for (int d = 0; d < 4; ++d) {
-                                e[d] = lm::exp2_fast(fmaf(s[i + d], qf, -m));
-                                sum[d] += e[d];
+                            for (int d = 0; d < 4; ++d) e[d] = __uint_as_float(r[i0 + i + d]);
+                            fma2(e[0], e[1], qf, -m);
+                            fma2(e[2], e[3], qf, -m);
+#pragma unroll
+                            for (int d = 0; d < 4; ++d) e[d] = lm::exp2_fast(e[d]);
+                            add2(sum[0], sum[1], e[0], e[1]);
+                            add2(sum[2], sum[3], e[2], e[3]);
+                            if (kCoded) {
+                                const float4 f = *reinterpret_cast<const float4*>(vs + i0 + i);
+                                mul2(e[0], e[1], f.x, f.y);
+                                mul2(e[2], e[3], f.z, f.w);
                             }
-                            if (kCoded) { e[0] *= f.x * vdiv; e[1] *= f.y * vdiv; e[2] *= f.z * vdiv; e[3] *= f.w * vdiv; }
                             if (kSplit) {
-                                amma::split_hi_lo(e[0], e[1], h[i / 2], h[(8 + i / 2) & 15]);
-                                amma::split_hi_lo(e[2], e[3], h[i / 2 + 1], h[(9 + i / 2) & 15]);
+                                split2(e[0], e[1], h[i / 2], h[(8 + i / 2) & 15]);
+                                split2(e[2], e[3], h[i / 2 + 1], h[(9 + i / 2) & 15]);
                             } else {
                                 const __half2 h0 = __floats2half2_rn(e[0], e[1]), h1 = __floats2half2_rn(e[2], e[3]);
                                 h[i / 2] = *reinterpret_cast<const uint32_t*>(&h0);
@@ -510,74 +663,78 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
                 tc::tc_fence_before();
                 __syncwarp();
                 mbar_arrive_by(lane == 0, bar(Sh::kFullP + 2 * w + b));
+                walk();
+                if (!kTall && (k + 1 < jobs || (w == 0 && tiles % 2 == 0))) walk();
             }
+            if (!kTall && w == 1 && jobs > 0 && tiles % 2 == 1) walk();
             // ---- the part's end
             const int last = kb + jobs - 1;
             if (jobs > 0) wait(Sh::kDoneO + 2 * w + (last & 1), (last >> 1) & 1);
             tc::tc_fence_after();
-            // Each warp's 16 KB of the queries' place: what stream 1 has, [column][row]; then, 32 columns at a time, [row][column] with the
-            // 16-byte pieces swizzled, from where rows go out whole lines at a time.
-            float* hand = reinterpret_cast<float*>(q_area + (kTall ? w * (kSplit ? 2 : 1) * Sh::kQTile + (warp & 3) * 4096 : (warp & 3) * 16384));
-            float top = m, c0 = 1.f, c1 = 0.f;
+            // kTall: a stream has its rows' results.  Otherwise both have a share of the same rows, O in the same lanes of tensor memory: with
+            // the other's maximum, sum and scale, each joins half of the columns.
+            float top = m, c0 = kCoded ? vref : 1.f, c1 = 0.f, f0 = has_kept ? lm::exp2_fast(m_kept - m) * v_kept : 0.f, f1 = 0.f;
+            const bool other = ((tiles + w) >> 1) > 0;               // the other stream had a tile
             if (!kTall) {
-                if (w == 0) {
-                    mbar_arrive(bar(Sh::kGive));              // both streams' scores are done: the queries' place is free
-                    wait(Sh::kGiven, nth & 1);
-                    const float2 ml = s_ml[rt];
-                    top = fmaxf(m, ml.x);
-                    c0 = lm::exp2_fast(m - top);
-                    c1 = lm::exp2_fast(ml.x - top);
-                    l = fmaf(l, c0, ml.y * c1);
-                } else {
-                    wait(Sh::kGive, nth & 1);
-                    s_ml[rt] = make_float2(m, l);
-                }
+                s_ml[w * 128 + rt] = make_float4(m, l, c0, f0);
+                mbar_arrive(bar(Sh::kGive));
+                wait(Sh::kGive, nth & 1);
+                tc::tc_fence_after();
+                const float4 ml = s_ml[(w ^ 1) * 128 + rt];
+                top = fmaxf(m, ml.x);
+                const float e0 = lm::exp2_fast(m - top), e1 = lm::exp2_fast(ml.x - top);
+                l = fmaf(l, e0, ml.y * e1);
+                c0 *= e0;
+                f0 *= e0;
+                c1 = ml.z * e1;
+                f1 = ml.w * e1;
             }
             if (active) {
-                const float vmul = kCoded ? vref : 1.f, inv = l == 0.f ? 0.f : 1.f / l;
                 const bool whole = p.slot < 0;
-                const int r0 = (warp & 3) * 32, nn = min(32, rows - r0), grow = p.group * a.group_rows + (kTall ? w * 128 : 0) + r0;
-                float* rec = whole ? nullptr : a.part + ((size_t)p.slot * a.rec_rows + (kTall ? w * 128 : 0) + r0) * kPart;
-                A* out = static_cast<A*>(a.out) + ((size_t)p.m * a.T * a.nq + p.head * a.group) * kHd;
+                const float inv = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;   // (a row that sees nothing: 0)
+                c0 *= inv; c1 *= inv; f0 *= inv; f1 *= inv;
+                // A record is [column][row], then the rows' maxima and sums: a warp stores 32 rows of a column.
+                float* rec = whole ? nullptr : a.part + (size_t)p.slot * a.rec_rows * kPart + (kTall ? w * 128 : 0) + rt;
+                A* out = static_cast<A*>(a.out) + at_row;
+                const float* kept1 = kSplit ? a.kept + ((size_t)c * 2 + (w ^ 1)) * kHd * 128 + rt : nullptr;
+#pragma unroll 1
+                for (int d = kTall ? 0 : w * 64; d < (kTall ? kHd : w * 64 + 64); d += 16) {
+                    uint32_t o[16], q[16];
+                    tc::tmem_ld16(lanes + 128 + d, o);
+                    if (!kTall) tc::tmem_ld16((lanes ^ 256) + 128 + d, q);
+                    float old[16], old1[16];
+                    if (kSplit) {
 #pragma unroll
-                for (int d = 0; d < kHd; d += 32) {
-                    uint32_t o[32];
-                    if (jobs > 0) {
-                        tc::tmem_ld32(lanes + 128 + d, o);
-                        tc::tmem_wait_ld();
+                        for (int i = 0; i < 16; ++i) {
+                            old[i] = f0 != 0.f ? kept[(d + i) * 128] : 0.f;
+                            old1[i] = !kTall && f1 != 0.f ? kept1[(d + i) * 128] : 0.f;
+                        }
                     }
+                    tc::tmem_wait_ld();
+                    float v[16];
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        float v = jobs > 0 ? __uint_as_float(o[i]) : 0.f;
-                        if (kSplit) v += kept[kSplit ? d + i : 0];
-                        v *= vmul;
-                        if (!kTall && w == 1) hand[(d + i) * 32 + lane] = v;
-                        if (!kTall && w == 0) v = fmaf(v, c0, c1 * hand[(d + i) * 32 + lane]);
-                        o[i] = __float_as_uint(whole ? v * inv : v);
+                    for (int i = 0; i < 16; ++i) {
+                        v[i] = jobs > 0 ? __uint_as_float(o[i]) * c0 : 0.f;
+                        if (!kTall && other) v[i] = fmaf(__uint_as_float(q[i]), c1, v[i]);
+                        if (kSplit) v[i] = fmaf(old[i], f0, v[i]);
+                        if (kSplit && !kTall) v[i] = fmaf(old1[i], f1, v[i]);
                     }
-                    if (!kTall && w == 1) continue;
-                    float* stage = hand + (kTall ? 0 : d * 32);
-                    __syncwarp();
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        *reinterpret_cast<uint4*>(stage + lane * 32 + ((i ^ (lane & 7)) << 2)) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-                    __syncwarp();
-#pragma unroll 2
-                    for (int i = lane >> 3; i < nn; i += 4) {
-                        const float4 v = *reinterpret_cast<const float4*>(stage + i * 32 + (((lane & 7) ^ (i & 7)) << 2));
+                    if (mine) {
                         if (whole) {
-                            const int nd = (grow + i) / a.group;
-                            store_o4(out + ((size_t)nd * a.nq + grow + i - nd * a.group) * kHd + d + 4 * (lane & 7), v);
+                            store_o16(out + d, v);
                         } else {
-                            *reinterpret_cast<float4*>(rec + (size_t)i * kPart + d + 4 * (lane & 7)) = v;
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) rec[(size_t)(d + i) * a.rec_rows] = v[i];
                         }
                     }
                 }
-                if (!whole && mine && (kTall || w == 0)) *reinterpret_cast<float2*>(rec + (size_t)lane * kPart + kHd) = make_float2(top, l);
+                if (!whole && mine && (kTall || w == 0)) {
+                    rec[(size_t)kHd * a.rec_rows] = top;
+                    rec[(size_t)(kHd + 1) * a.rec_rows] = l;
+                }
             }
-            if (!kTall) mbar_arrive(bar(w == 1 ? Sh::kGiven : Sh::kTaken));
+            if (!kTall) mbar_arrive(bar(Sh::kTaken));
             tc::tc_fence_before();
-            it0 += p.t1 - p.t0;
             kb += jobs;
         }
     }
@@ -590,19 +747,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
     if (t == 0 && *abort_flag) atomicExch(a.status, kStatusMbarTimeout);
 }
 
-// Joins the records of contexts that several blocks have, a warp per row.
+// Joins the records of contexts that several blocks have: a block per 32 rows of a head, a lane per row, 16 columns per warp; from
+// shared memory rows go out whole.
 template <typename A>
-__global__ void __launch_bounds__(128) attend_tc_merge_kernel(const Args a) {
+__global__ void __launch_bounds__(256) attend_tc_merge_kernel(const Args a) {
+    __shared__ __align__(16) float s_out[32][kHd + 4];
     pdl_trigger();
     pdl_wait();
-    const int lane = threadIdx.x & 31;
-    const long at = (long)blockIdx.x * 4 + (threadIdx.x >> 5);     // (m, head, row)
-    if (at >= (long)a.M * a.c.heads * a.rows) return;
-    const int row = (int)(at % a.rows), mh = (int)(at / a.rows), m = mh / a.c.heads, head = mh - m * a.c.heads, node = row / a.group;
-    if (a.first[m] < 0 || node >= node_count(a, m)) return;
-    int groups;
-    const int tiles = seq_tiles(a, m, &groups), g = row / a.group_rows;
-    const int x0 = a.cum[m] + (head * groups + g) * tiles, x1 = x0 + tiles;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r0 = blockIdx.x * 32, head = blockIdx.y, m = blockIdx.z;
+    const Seq q = seq_of(a, m);
+    const int rows = q.nodes * a.group;
+    if (q.tiles == 0 || r0 >= rows) return;
+    const int g = r0 >= a.group_rows ? (uint32_t)r0 / (uint32_t)a.group_rows : 0, row = min(r0 + lane, rows - 1);
+    const int x0 = a.cum[m] + (head * q.groups + g) * q.tiles, x1 = x0 + q.tiles;
     const int* starts = a.cum + kPlanned;                          // of the blocks' stretches, in tiles
     const float per = (float)a.blocks / (float)starts[a.blocks];
     auto block_of = [&](int x) {                                   // the block that has tile x
@@ -613,26 +770,50 @@ __global__ void __launch_bounds__(128) attend_tc_merge_kernel(const Args a) {
     };
     const int b0 = block_of(x0), b1 = block_of(x1 - 1);
     if (b0 == b1) return;                                          // one block had it whole
-    const bool late = starts[b0] < x0;                             // the first block has other work before
-    auto record = [&](int c) { return a.part + ((size_t)(2 * c + (c == b0 && late ? 1 : 0)) * a.rec_rows + row - g * a.group_rows) * kPart; };
-    float top = -FLT_MAX, sum = 0.f;
-    for (int c = b0 + lane; c <= b1; c += 32)
-        if (starts[c] < starts[c + 1]) top = fmaxf(top, record(c)[kHd]);
-    top = warp_max(top);
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int c = b0; c <= b1; ++c) {
-        if (starts[c] == starts[c + 1]) continue;
-        const float* rec = record(c);
-        const float2 ml = *reinterpret_cast<const float2*>(rec + kHd);
-        const float4 v = *reinterpret_cast<const float4*>(rec + 4 * lane);
-        const float e = lm::exp2_fast(ml.x - top);
-        sum = fmaf(ml.y, e, sum);
-        acc.x = fmaf(v.x, e, acc.x); acc.y = fmaf(v.y, e, acc.y); acc.z = fmaf(v.z, e, acc.z); acc.w = fmaf(v.w, e, acc.w);
+    const size_t record = (size_t)a.rec_rows * kPart;
+    const float* rec = a.part + row - g * a.group_rows;
+    const size_t late = starts[b0] < x0 ? record : 0;              // (the first block may have other work before)
+    float top = -FLT_MAX, sum = 0.f, acc[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+    for (int c0 = b0; c0 <= b1; c0 += 4) {                         // four records in flight
+        float v[4][16], mt[4], lt[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int c = min(c0 + j, b1);
+            const bool there = c0 + j <= b1 && starts[c] < starts[c + 1];
+            const float* at = rec + 2 * c * record + (c == b0 ? late : 0);
+            mt[j] = there ? at[(size_t)kHd * a.rec_rows] : -FLT_MAX;
+            lt[j] = there ? at[(size_t)(kHd + 1) * a.rec_rows] : 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[j][i] = there ? at[(size_t)(warp * 16 + i) * a.rec_rows] : 0.f;
+        }
+        const float to = fmaxf(top, fmaxf(fmaxf(mt[0], mt[1]), fmaxf(mt[2], mt[3]))), f = lm::exp2_fast(top - to);
+        top = to;
+        sum *= f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[i] *= f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float e = lm::exp2_fast(mt[j] - to);
+            sum = fmaf(lt[j], e, sum);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[i] = fmaf(v[j][i], e, acc[i]);
+        }
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    A* out = static_cast<A*>(a.out) + (((size_t)m * a.T + node) * a.nq + head * a.group + row - node * a.group) * kHd + 4 * lane;
-    store_o4(out, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+#pragma unroll
+    for (int i = 0; i < 16; i += 4)
+        *reinterpret_cast<float4*>(&s_out[lane][warp * 16 + i]) = make_float4(acc[i] * inv, acc[i + 1] * inv, acc[i + 2] * inv, acc[i + 3] * inv);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = r0 + warp + 8 * i;
+        if (r >= rows) break;
+        const uint32_t node = (uint32_t)r / (uint32_t)a.group;
+        store_o4(static_cast<A*>(a.out) + (((size_t)m * a.T + node) * a.nq + head * a.group + r - node * a.group) * kHd + 4 * lane,
+                 *reinterpret_cast<const float4*>(&s_out[r - r0][4 * lane]));
+    }
 }
 
 }  // namespace tree

@@ -194,7 +194,7 @@ def one_attention(M, T, nq, nkv, first, max_seq, coded, act, masks=None, count=N
             for t in (st.ks, st.vs) if coded else ():
                 t[m, layer, :, ~seen[m].any(0)] = math.nan
     k = kernels()
-    scratch = torch.full((k.attention_tree_scratch_bytes(M, T, nq, nkv, max_seq),), 255, dtype=torch.uint8, device="cuda")
+    scratch = torch.full((k.attention_tree_scratch_bytes(M, 64, nq, nkv, max_seq),), 255, dtype=torch.uint8, device="cuda")   # (whatever kernel)
     a = (out, q, st.args(layer), ints(first), None if masks is None else words(masks), None if count is None else ints(count), hint, nq, M, T, scratch)
     (call or k.attention_tree)(*a)
     kk, vv = st.value(layer)
