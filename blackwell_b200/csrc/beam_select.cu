@@ -123,7 +123,7 @@ __device__ __forceinline__ float exponentials(const float4 (&v)[kVec], float to)
     return (p[0] + p[1]) + (p[2] + p[3]);
 }
 
-__global__ void __launch_bounds__(kThreads, 3) chunk_kernel(const Args a) {
+__global__ void __launch_bounds__(kThreads, 4) chunk_kernel(const Args a) {
     __shared__ unsigned long long s_list[kWarps][kList], s_all[kWarps * kMaxKeep];
     __shared__ float s_f[kWarps], s_g[kWarps];
     __shared__ uint32_t s_group[64];
@@ -153,12 +153,17 @@ __global__ void __launch_bounds__(kThreads, 3) chunk_kernel(const Args a) {
     float4 next[kVec];
     load(q0, next);
     if (t < 64) s_group[t] = 0;                                          // (below every value)
-    if (t < kWarps) s_n[t] = 0;
     __syncthreads();
     unsigned long long* list = s_list[warp];
     float m[2] = {-INFINITY, -INFINITY}, sum = 0.f, ground = -FLT_MAX;     // maxima of the lane's even and odd vectors
-    int groups = 1;
+    int n = 0, groups = 1;
     while (groups < a.keep) groups <<= 1;
+    auto bar_of = [&]() {                                                // the smallest of the groups' maxima so far
+        const volatile uint32_t* g = s_group;
+        uint32_t low = lane < groups ? g[lane] : 0xFFFFFFFFu;
+        if (groups > 32) low = min(low, g[32 + lane]);
+        return order32_value(__reduce_min_sync(0xffffffffu, low));
+    };
     for (int base = q0; base < q1; base += kTurn) {
         float4 v[kVec];
 #pragma unroll
@@ -182,34 +187,36 @@ __global__ void __launch_bounds__(kThreads, 3) chunk_kernel(const Args a) {
             }
         }
         // group (thread mod G), or with G = 64 (lane) and (32 + lane) of the lanes' two maxima
-        uint32_t low;
         if (groups > 32) {
-            const uint32_t g0 = atomicMax(&s_group[lane], order32(m[0])), g1 = atomicMax(&s_group[32 + lane], order32(m[1]));
-            low = min(max(g0, order32(m[0])), max(g1, order32(m[1])));
+            atomicMax(&s_group[lane], order32(m[0]));
+            atomicMax(&s_group[32 + lane], order32(m[1]));
         } else {
             float g = to;
             for (int o = 16; o >= groups; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
-            low = order32(g);
-            if (lane < groups) low = max(low, atomicMax(&s_group[lane], low));
+            if (lane < groups) atomicMax(&s_group[lane], order32(g));
         }
-        const float bar = order32_value(__reduce_min_sync(0xffffffffu, groups > 32 || lane < groups ? low : 0xFFFFFFFFu));
-        const float in = fmaxf(bar, ground);
-        if (__any_sync(0xffffffffu, best >= in)) {
+        if (base == q0) __syncthreads();                                 // the first bar is that of the block's values, not of a warp's
+        else __syncwarp();
+        const float bar = bar_of();
+        if (__any_sync(0xffffffffu, best >= fmaxf(bar, ground))) {
             const uint32_t i0 = (uint32_t)(4 * (base + t) - skew);
+            const float least = fmaxf(bar, ground);
 #pragma unroll
             for (int j = 0; j < kVec; ++j) {
                 const float e[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
 #pragma unroll
-                for (int d = 0; d < 4; ++d)
-                    if (e[d] >= in) list[atomicAdd(&s_n[warp], 1)] = key_of(e[d], i0 + 4 * kThreads * j + d);
+                for (int d = 0; d < 4; ++d) {
+                    const uint32_t who = __ballot_sync(0xffffffffu, e[d] >= least);
+                    if (who) {                                           // (hardly ever: a branch costs less than what it skips)
+                        if (e[d] >= least) list[n + __popc(who & ((1u << lane) - 1))] = key_of(e[d], i0 + 4 * kThreads * j + d);
+                        n += __popc(who);
+                    }
+                }
             }
-            __syncwarp();
-            const int n = *reinterpret_cast<volatile int*>(&s_n[warp]);
-            __syncwarp();
             if (n > kGrown) {
                 cut_list(list, n, a.keep, lane);
                 ground = order32_value((uint32_t)(list[a.keep - 1] >> 32) + 1);   // the next float: what equals the last one comes too late
-                if (lane == 0) s_n[warp] = a.keep;
+                n = a.keep;
                 __syncwarp();
             }
         }
@@ -217,8 +224,21 @@ __global__ void __launch_bounds__(kThreads, 3) chunk_kernel(const Args a) {
     // the block's maximum and sum, and the best of the warps' lists
     const float mine = fmaxf(m[0], m[1]), wm = warp_max(mine);
     if (lane == 0) s_g[warp] = wm;
-    __syncwarp();
-    int n = s_n[warp];
+    __syncthreads();
+    {                                                                    // what is at or above the last bar
+        const float bar = fmaxf(bar_of(), -FLT_MAX);
+        int left = 0;
+        for (int i0 = 0; i0 < n; i0 += 32) {
+            const unsigned long long k = i0 + lane < n ? list[i0 + lane] : 0;
+            const bool in = k != 0 && order32_value((uint32_t)(k >> 32)) >= bar;
+            const uint32_t who = __ballot_sync(0xffffffffu, in);         // (all have read before any writes, at or before where it read)
+            if (in) list[left + __popc(who & ((1u << lane) - 1))] = k;
+            left += __popc(who);
+            __syncwarp();
+        }
+        n = left;
+    }
+    if (lane == 0) s_n[warp] = n;
     if (__syncthreads_or(n > kMaxKeep)) {
         if (n > a.keep) cut_list(list, n, a.keep, lane);
         n = min(n, a.keep);
@@ -358,10 +378,10 @@ __global__ void __launch_bounds__(kThreads) merge_kernel(const Args a) {
     if (warp == 0) tournament(kWarps, a.keep, lane, [&](int l, int i) { return s_best[l][i]; }, out);
 }
 
-// Stretches of a row: whole turns, three blocks per SM where that many are to be had.
+// Stretches of a row: whole turns, four blocks per SM where that many are to be had.
 static void stretches(int vocab, int beams, long rows, int sms, Args* a) {
     const int turns = (vocab + 3 + 3) / 4 / kTurn + 1;
-    long n = 3L * sms / rows;
+    long n = 4L * sms / rows;
     n = n > kMaxLists / beams ? kMaxLists / beams : n;
     n = n < 1 ? 1 : n > turns ? turns : n;
     a->chunk = (int)((turns + n - 1) / n) * kTurn;
@@ -383,7 +403,7 @@ using namespace bw;
 
 extern "C" size_t bw_beam_select_scratch_bytes(int vocab, int beams, int keep, int M) {
     if (!beam::sizes_ok(vocab, beams, keep, M)) return 0;
-    const long rows = (long)M * beams, most = 3L * sm_count(current_device());   // (records of any smaller call too)
+    const long rows = (long)M * beams, most = 4L * sm_count(current_device());   // (records of any smaller call too)
     return beam::bytes_of(rows > most ? rows : most, keep);
 }
 

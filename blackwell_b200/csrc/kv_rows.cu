@@ -20,7 +20,6 @@ struct WriteArgs {
     const int *first, *offset, *count;
     int nq, M, T;
     float eps;
-    double ratio;                       // base^(-2/128)
 };
 __device__ __forceinline__ float4 load_act4(const float* p) { return *reinterpret_cast<const float4*>(p); }
 __device__ __forceinline__ float4 load_act4(const __nv_bfloat16* p) {
@@ -31,31 +30,28 @@ __device__ __forceinline__ void store_act4(float* p, const float4& v) { *reinter
 __device__ __forceinline__ void store_act4(__nv_bfloat16* p, const float4& v) {
     *reinterpret_cast<uint2*>(p) = make_uint2(lm::pack_bf16(v.x, v.y), lm::pack_bf16(v.z, v.w));
 }
-// base^(-2i/128) = ratio^i for i = 2 lane, by the bits of lane.  64 bits: a position times a 32-bit frequency is off by position * 2^-24,
-// a visible angle from some thousand positions on.
-__device__ __forceinline__ double even_frequency(double ratio, int lane) {
-    double f = 1.0, s = ratio * ratio;
-#pragma unroll
-    for (int bit = 1; bit < 32; bit <<= 1) {
-        if (lane & bit) f *= s;
-        s *= s;
-    }
-    return f;
-}
-// cos, sin of position * frequency, reduced to a half turn in 64 bits.
-__device__ __forceinline__ float2 turn_of(double position, double frequency) {
-    const double a = position * frequency;
-    const float r = (float)fma(-rint(a * 0.15915494309189535), 6.283185307179586, a);
+// base^(-2i/128) / 2 pi, i = 0..63: turns per position, as fractions of 2^64.  A position times one of them, modulo 2^64, is the angle to 2^-64 turns
+// a position, whatever the position: in 32-bit floating point it would be off by position * 2^-24, visible from some thousand positions on.
+struct Turns {
+    unsigned long long f[kHd / 2];
+};
+// cos, sin of the angle.
+__device__ __forceinline__ float2 turn_of(long long position, unsigned long long per) {
+    const unsigned long long a = (unsigned long long)position * per;
     float s, c;
-    sincosf(r, &s, &c);
+    sincospif((float)(int)(uint32_t)(a >> 32) * 0x1p-31f, &s, &c);
     return make_float2(c, s);
 }
 
 // A warp takes HW heads of one row (token or node), four dimensions of each per lane.  x / sqrt(mean x^2 + eps) * w, then pairs
 // (2i, 2i + 1) turned; a cached row is stored in binary16, or divided by absmax / 448 and rounded to e4m3.
 template <typename A, int HW>
-__global__ void __launch_bounds__(256) write_rows_kernel(const WriteArgs a) {
+__global__ void __launch_bounds__(256) write_rows_kernel(const WriteArgs a, const __grid_constant__ Turns turns) {
+    // (a lane's own entry of the parameters' constant bank costs a pass per lane: once per block)
+    __shared__ __align__(16) unsigned long long s_turns[kHd / 2];
     pdl_trigger();
+    if (threadIdx.x < kHd / 2) s_turns[threadIdx.x] = turns.f[threadIdx.x];
+    __syncthreads();
     pdl_wait();
     const int lane = threadIdx.x & 31, heads = a.nq + 2 * a.c.heads, per_row = (heads + HW - 1) / HW;
     const long gw = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -68,36 +64,46 @@ __global__ void __launch_bounds__(256) write_rows_kernel(const WriteArgs a) {
     float4 v[HW];
 #pragma unroll
     for (int j = 0; j < HW; ++j) v[j] = h0 + j < heads ? load_act4(x + j * kHd) : make_float4(0.f, 0.f, 0.f, 0.f);
-    float2 r0 = make_float2(1.f, 0.f), r1 = r0;
-    if (h0 < a.nq + a.c.heads) {
-        const double p = (double)((long)first + (a.offset ? a.offset[at] : i));
-        const double f = even_frequency(a.ratio, lane);
-        r0 = turn_of(p, f);
-        r1 = turn_of(p, f * a.ratio);
+    const int turned = a.nq + a.c.heads;                // heads that are normed and turned
+    if (h0 < turned) {
+        float4 qw = make_float4(1.f, 1.f, 1.f, 1.f), kw = qw;
+        if (a.q_w && h0 < a.nq) qw = *reinterpret_cast<const float4*>(a.q_w + 4 * lane);
+        if (a.k_w && h0 + HW > a.nq) kw = *reinterpret_cast<const float4*>(a.k_w + 4 * lane);
+        const long long p = (long long)first + (a.offset ? a.offset[at] : i);
+        const ulonglong2 per = *reinterpret_cast<const ulonglong2*>(&s_turns[2 * lane]);
+        const float2 r0 = turn_of(p, per.x), r1 = turn_of(p, per.y);
+        float ss[HW];
+#pragma unroll
+        for (int j = 0; j < HW; ++j) ss[j] = fmaf(v[j].w, v[j].w, fmaf(v[j].z, v[j].z, fmaf(v[j].y, v[j].y, v[j].x * v[j].x)));
+        // a lane ends up with the sum of one of the heads, and gives its root to all
+        const float root = rsqrtf(warp_sum_many<HW>(ss, lane) / 128.0f + a.eps);
+#pragma unroll
+        for (int j = 0; j < HW; ++j) {
+            const int h = h0 + j;
+            if (h >= turned) break;
+            const bool is_q = h < a.nq;
+            float4 y = v[j];
+            if (is_q ? a.q_w != nullptr : a.k_w != nullptr) {
+                const float is = __shfl_sync(0xffffffffu, root, HW == 1 ? 0 : (j >> 1) * 16 + (j & 1) * 8);   // warp_sum_many_index
+                const float4 g = is_q ? qw : kw;
+                y = make_float4(y.x * is * g.x, y.y * is * g.y, y.z * is * g.z, y.w * is * g.w);
+            }
+            v[j] = make_float4(fmaf(y.x, r0.x, -(y.y * r0.y)), fmaf(y.x, r0.y, y.y * r0.x), fmaf(y.z, r1.x, -(y.w * r1.y)),
+                               fmaf(y.z, r1.y, y.w * r1.x));
+        }
     }
     const long row = (long)first + i;
 #pragma unroll
     for (int j = 0; j < HW; ++j) {
         const int h = h0 + j;
         if (h >= heads) break;
-        float4 y = v[j];
-        if (h < a.nq + a.c.heads) {
-            const float* w = h < a.nq ? a.q_w : a.k_w;
-            if (w) {
-                const float ss = warp_sum(fmaf(y.w, y.w, fmaf(y.z, y.z, fmaf(y.y, y.y, y.x * y.x))));
-                const float is = rsqrtf(ss / 128.0f + a.eps);
-                const float4 g = *reinterpret_cast<const float4*>(w + 4 * lane);
-                y = make_float4(y.x * is * g.x, y.y * is * g.y, y.z * is * g.z, y.w * is * g.w);
-            }
-            y = make_float4(fmaf(y.x, r0.x, -(y.y * r0.y)), fmaf(y.x, r0.y, y.y * r0.x), fmaf(y.z, r1.x, -(y.w * r1.y)),
-                            fmaf(y.z, r1.y, y.w * r1.x));
-        }
+        const float4 y = v[j];
         if (h < a.nq) {
             store_act4(static_cast<A*>(a.q_out) + (at * a.nq + h) * kHd + 4 * lane, y);
             continue;
         }
         if (row >= a.c.max_seq) continue;               // a row outside of the cache is never written
-        const bool is_k = h < a.nq + a.c.heads;
+        const bool is_k = h < turned;
         const size_t to = a.c.row(m, h - a.nq - (is_k ? 0 : a.c.heads), row);
         unsigned char* side = is_k ? a.c.k : a.c.v;
         if (!a.c.coded()) {
@@ -105,26 +111,26 @@ __global__ void __launch_bounds__(256) write_rows_kernel(const WriteArgs a) {
             *reinterpret_cast<uint2*>(side + (to * kHd + 4 * lane) * 2) =
                 make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
         } else {
-            const float top = warp_max(fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
+            const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))))));
             const bool tiny = top < kTinyRow;
-            const float up = tiny ? 1.f : kCodeMax / top;
+            const float up = tiny ? 1.f : __fdividef(kCodeMax, top);   // (to 2^-22: which of two codes is nearer changes for one element in a million)
             const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y.x * up, y.y * up), __NV_SATFINITE, __NV_E4M3);
             const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y.z * up, y.w * up), __NV_SATFINITE, __NV_E4M3);
             *reinterpret_cast<uint32_t*>(side + to * kHd + 4 * lane) = lo | hi << 16;
-            if (lane == 0) (is_k ? a.c.ks : a.c.vs)[to] = tiny ? 1.f : top / kCodeMax;
+            if (lane == 0) (is_k ? a.c.ks : a.c.vs)[to] = tiny ? 1.f : top * (1.0f / kCodeMax);
         }
     }
 }
 
 template <typename A>
-static cudaError_t write_launch(const WriteArgs& a, cudaStream_t st) {
+static cudaError_t write_launch(const WriteArgs& a, const Turns& turns, cudaStream_t st) {
     const int heads = a.nq + 2 * a.c.heads;
     const long rows = (long)a.M * a.T;
     // Few rows: a warp per head, everything is latency.  Many: four heads a warp share the angles and keep four loads in flight.
     const bool many = rows * heads > 32L * sm_count(current_device());
     const long warps = rows * (many ? (heads + 3) / 4 : heads), blocks = (warps + 7) / 8;
     if (blocks > 0x7FFFFFFFL) return cudaErrorInvalidValue;
-    const cudaError_t e = launch_pdl(many ? write_rows_kernel<A, 4> : write_rows_kernel<A, 1>, dim3((unsigned)blocks), dim3(256), 0, st, a);
+    const cudaError_t e = launch_pdl(many ? write_rows_kernel<A, 4> : write_rows_kernel<A, 1>, dim3((unsigned)blocks), dim3(256), 0, st, a, turns);
     count_launch(1);
     return e != cudaSuccess ? e : cudaPeekAtLastError();
 }
@@ -183,44 +189,85 @@ __global__ void __launch_bounds__(256) reorder_kernel(const MoveArgs a) {
     }
 }
 
-// Row first + i takes row first + path[i], i < count: a block reads all rows of a plane (one side of a head in a layer), then writes.
+// Row first + i takes row first + path[i], i < count: a warp has a plane (one side of a head in a layer).  Each step reads 128 pieces of 16
+// bytes before it writes them.  An ascending path (path[i] >= i, each larger than the one before: the nodes of a tree in order) can go on so, because
+// a later step reads behind all that is written; any other one is read whole first, through local memory.
+__device__ __forceinline__ void keep_plane(const MoveArgs& a, uint4* data, float* scale, size_t base, const int* path, int first, int n, int lane) {
+    const int shift = scale ? 3 : 4, cols = 1 << shift;  // pieces of a row: 8 or 16
+    auto source = [&](int i) {                           // path[i], or -1 where row i stays as it is
+        if (i >= n) return -1;
+        const int p = path[i];
+        return p >= 0 && p < a.n && p != i && (long)first + max(p, i) < a.c.max_seq ? p : -1;
+    };
+    bool ascending = true;
+    if (n * cols > 128) {
+        const int lo = lane < n ? path[lane] : 1 << 20, hi = lane + 32 < n ? path[lane + 32] : 1 << 20;
+        const int lo_next = __shfl_down_sync(0xffffffffu, lo, 1), hi_next = __shfl_down_sync(0xffffffffu, hi, 1), hi_first = __shfl_sync(0xffffffffu, hi, 0);
+        const bool fine = (lane >= n || (lo >= lane && lo < (lane < 31 ? lo_next : hi_first))) &&
+                          (lane + 32 >= n || (hi >= lane + 32 && (lane == 31 || hi < hi_next)));
+        ascending = __all_sync(0xffffffffu, fine);
+    }
+    if (ascending) {
+        for (int u0 = 0; u0 < n * cols; u0 += 128) {
+            uint4 x[4];
+            float s[4];
+            int p[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) p[j] = source((u0 + lane + 32 * j) >> shift);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int col = (lane + 32 * j) & (cols - 1);
+                if (p[j] >= 0) {
+                    x[j] = data[((base + p[j]) << shift) + col];
+                    if (scale && col == 0) s[j] = scale[base + p[j]];
+                }
+            }
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int u = u0 + lane + 32 * j, i = u >> shift, col = u & (cols - 1);
+                if (p[j] >= 0) {
+                    data[((base + i) << shift) + col] = x[j];
+                    if (scale && col == 0) scale[base + i] = s[j];
+                }
+            }
+            __syncwarp();
+        }
+        return;
+    }
+    uint4 x[kMaxPath * 16 / 32];
+    float s[kMaxPath * 16 / 32];
+#pragma unroll 1
+    for (int j = 0; 32 * j < n * cols; ++j) {
+        const int u = lane + 32 * j, p = source(u >> shift), col = u & (cols - 1);
+        if (p >= 0) {
+            x[j] = data[((base + p) << shift) + col];
+            if (scale && col == 0) s[j] = scale[base + p];
+        }
+    }
+    __syncwarp();
+#pragma unroll 1
+    for (int j = 0; 32 * j < n * cols; ++j) {
+        const int u = lane + 32 * j, i = u >> shift, col = u & (cols - 1);
+        if (source(i) >= 0) {
+            data[((base + i) << shift) + col] = x[j];
+            if (scale && col == 0) scale[base + i] = s[j];
+        }
+    }
+}
 __global__ void __launch_bounds__(256) keep_rows_kernel(const MoveArgs a) {
     pdl_trigger();
     pdl_wait();
-    const int m = blockIdx.y, side = blockIdx.x & 1, plane = blockIdx.x >> 1;
-    const int layer = plane / a.c.heads, g = plane - layer * a.c.heads;
+    const int m = blockIdx.y, unit = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (unit >= 2 * a.layers * a.c.heads) return;
     const int first = a.from[m], n = min(a.to[m], a.n);
     if (first < 0 || n <= 0) return;
-    const bool coded = a.c.coded();
-    const int cols = coded ? 8 : 16;
+    const int side = unit & 1, plane = unit >> 1, layer = plane / a.c.heads, g = plane - layer * a.c.heads;
     uint4* data = reinterpret_cast<uint4*>(side ? a.c.v : a.c.k);
     float* scale = side ? a.c.vs : a.c.ks;
     const size_t base = a.c.row(m, g, first) + layer * a.layer_stride;
-    constexpr int kPer = kMaxPath * 16 / 256;
-    uint4 x[kPer];
-    float s[kPer];
-    bool moves[kPer];
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-        const int u = threadIdx.x + 256 * j, i = u / cols, col = u - i * cols;
-        moves[j] = false;
-        if (i < n) {
-            const int p = a.index[(size_t)m * a.n + i];
-            moves[j] = p >= 0 && p < a.n && p != i && (long)first + max(p, i) < a.c.max_seq;
-            if (moves[j]) {
-                x[j] = data[(base + p) * cols + col];
-                if (coded && col == 0) s[j] = scale[base + p];
-            }
-        }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < kPer; ++j)
-        if (moves[j]) {
-            const int u = threadIdx.x + 256 * j, i = u / cols, col = u - i * cols;
-            data[(base + i) * cols + col] = x[j];
-            if (coded && col == 0) scale[base + i] = s[j];
-        }
+    const int* path = a.index + (size_t)m * a.n;
+    keep_plane(a, data, scale, base, path, first, n, lane);
 }
 
 }  // namespace kv
@@ -240,9 +287,12 @@ extern "C" int bw_qk_norm_rope_kv_rows(void* q_out, const bw_kv_cache* cache, co
     a.q_out = q_out; a.qkv = qkv; a.q_w = q_norm_w_or_null; a.k_w = k_norm_w_or_null;
     a.first = d_first_row; a.offset = d_offset_or_null; a.count = d_count_or_null;
     a.nq = num_q_heads; a.M = M; a.T = T; a.eps = eps;
-    a.ratio = pow((double)rope_base, -2.0 / kv::kHd);
+    kv::Turns turns;
+    const double ratio = pow((double)rope_base, -2.0 / kv::kHd);
+    double f = 0.15915494309189535;                    // 1 / 2 pi
+    for (int i = 0; i < kv::kHd / 2; ++i, f *= ratio) turns.f[i] = (unsigned long long)(long long)((f - floor(f)) * 0x1p63) << 1;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return bf16 ? kv::write_launch<__nv_bfloat16>(a, st) : kv::write_launch<float>(a, st);
+    return bf16 ? kv::write_launch<__nv_bfloat16>(a, turns, st) : kv::write_launch<float>(a, turns, st);
 }
 
 // What both moves check of their planes: layers of layer_stride elements from the cache's own layer on.
@@ -278,7 +328,7 @@ extern "C" int bw_kv_keep_rows(const bw_kv_cache* cache, const int* d_first_row,
     a.index = d_path; a.from = d_first_row; a.to = d_count; a.n = T;
     const long planes = 2L * layers * a.c.heads;
     if (planes > 0x7FFFFFFFL) return cudaErrorInvalidValue;
-    const cudaError_t e = launch_pdl(kv::keep_rows_kernel, dim3((unsigned)planes, (unsigned)M), dim3(256), 0, static_cast<cudaStream_t>(stream), a);
+    const cudaError_t e = launch_pdl(kv::keep_rows_kernel, dim3((unsigned)((planes + 7) / 8), (unsigned)M), dim3(256), 0, static_cast<cudaStream_t>(stream), a);
     count_launch(1);
     return e != cudaSuccess ? e : cudaPeekAtLastError();
 }
