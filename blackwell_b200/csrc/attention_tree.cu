@@ -82,7 +82,7 @@ static cudaError_t launch_tc(const Args& a, cudaStream_t st) {
     cudaError_t e = launch_pdl(kern, dim3(a.blocks), dim3(kTcThreads), smem, st, a);
     count_launch(1);
     if (e == cudaSuccess && a.flat) {
-        e = launch_pdl(attend_tc_merge_kernel<A>, dim3((a.rows + 31) / 32, a.c.heads, a.M), dim3(256), 0, st, a);
+        e = launch_pdl(attend_tc_merge_kernel<A>, dim3((a.rows + 31) / 32 * 2, a.c.heads, a.M), dim3(256), 0, st, a);
         count_launch(1);
     }
     return e != cudaSuccess ? e : cudaPeekAtLastError();

@@ -122,14 +122,15 @@ __global__ void __launch_bounds__(Shape<NT, kCoded>::kWarps * 32, 2) attend_kern
     __shared__ float2 s_ml[Sh::kRows];                  // this block's maximum and sum, for the cluster
     uint4* s_q = reinterpret_cast<uint4*>(dsm + kWarps * Sh::kPerWarp);
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31, g = lane >> 2, tq = lane & 3;
-    const int split = blockIdx.x, head = blockIdx.y / a.tiles, r0 = (blockIdx.y - head * a.tiles) * Sh::kRows, m = blockIdx.z;
+    const int split = blockIdx.x, head = blockIdx.y / (uint32_t)a.tiles, r0 = (blockIdx.y - head * a.tiles) * Sh::kRows, m = blockIdx.z;
     pdl_trigger();
     pdl_wait();
     const int first = a.first[m], nodes = node_count(a, m);
     if (first < 0 || r0 >= nodes * a.group) return;     // (all blocks of the cluster)
     const int ctx = min(first, a.c.max_seq), end = (int)min((long)first + nodes, (long)a.c.max_seq);
     const int ntile = (end + kTile - 1) / kTile;
-    const int tile0 = (int)((long)ntile * split / a.nsplit), tile1 = (int)((long)ntile * (split + 1) / a.nsplit);
+    const int each = ntile / (uint32_t)a.nsplit, over = ntile - each * a.nsplit;   // equal shares, the first ones a tile longer
+    const int tile0 = split * each + min(split, over), tile1 = tile0 + each + (split < over ? 1 : 0);
 
     const size_t row0 = a.c.row(m, head, 0);
     constexpr int kRowBytes = kCoded ? kHd : 2 * kHd, kChunks = kRowBytes / 16, kStep = 32 / kChunks;
@@ -141,7 +142,7 @@ __global__ void __launch_bounds__(Shape<NT, kCoded>::kWarps * 32, 2) attend_kern
     if (comes) {
         const unsigned long long mine = (lane < nodes ? mask_of(a, m, lane, nodes) : 0) | (lane + 32 < nodes ? mask_of(a, m, lane + 32, nodes) : 0);
         any = (unsigned long long)__reduce_or_sync(0xffffffffu, (uint32_t)(mine >> 32)) << 32 | __reduce_or_sync(0xffffffffu, (uint32_t)mine);
-        for (int r = t; r < Sh::kRows; r += kWarps * 32) s_mask[r] = r0 + r < nodes * a.group ? mask_of(a, m, (r0 + r) / a.group, nodes) : 0;
+        for (int r = t; r < Sh::kRows; r += kWarps * 32) s_mask[r] = r0 + r < nodes * a.group ? mask_of(a, m, (uint32_t)(r0 + r) / (uint32_t)a.group, nodes) : 0;
     }
     auto there = [&](int p) { return p < ctx || (p < end && (any >> (p - ctx) & 1)); };
     // 16 rows of K and V to a stage: piece c of rows rr, rr + kStep, ...; rows that nobody sees become zeros, whatever lies there
@@ -170,12 +171,17 @@ __global__ void __launch_bounds__(Shape<NT, kCoded>::kWarps * 32, 2) attend_kern
         }
     };
     // key and value scales of this thread's positions g, g + 8 of a tile
+    const float *ksp = kCoded ? a.c.ks + row0 + g : nullptr, *vsp = kCoded ? a.c.vs + row0 + g : nullptr;
     auto scales_of = [&](int tile, float (&s)[4]) {
-        const int p = tile * kTile + g;
-        const bool a0 = there(p), a1 = there(p + 8);
-        const size_t i0 = row0 + p;
-        s[0] = a0 ? a.c.ks[i0] : 0.f; s[1] = a1 ? a.c.ks[i0 + 8] : 0.f;
-        s[2] = a0 ? a.c.vs[i0] : 0.f; s[3] = a1 ? a.c.vs[i0 + 8] : 0.f;
+        const int p0 = tile * kTile;
+        if (p0 + kTile <= ctx) {
+            s[0] = ksp[p0]; s[1] = ksp[p0 + 8];
+            s[2] = vsp[p0]; s[3] = vsp[p0 + 8];
+        } else {
+            const bool a0 = there(p0 + g), a1 = there(p0 + g + 8);
+            s[0] = a0 ? ksp[p0] : 0.f; s[1] = a1 ? ksp[p0 + 8] : 0.f;
+            s[2] = a0 ? vsp[p0] : 0.f; s[3] = a1 ? vsp[p0 + 8] : 0.f;
+        }
     };
     int next = tile0 + warp;
 #pragma unroll
@@ -197,7 +203,7 @@ __global__ void __launch_bounds__(Shape<NT, kCoded>::kWarps * 32, 2) attend_kern
     for (int jj = 0; jj < kRegs; ++jj) {
         const int j = NT > 2 ? warp : jj;
         if (NT > 2 && warp >= NT) break;
-        const int r = r0 + 8 * j + g, node = r / a.group;
+        const int r = r0 + 8 * j + g, node = (uint32_t)r / (uint32_t)a.group;
         const bool in = node < nodes;
         const A* q = static_cast<const A*>(a.q) + (((size_t)m * a.T + (in ? node : 0)) * a.nq + head * a.group + (in ? r - node * a.group : 0)) * kHd;
         float2 x[8][2];
@@ -471,7 +477,7 @@ __global__ void __launch_bounds__(Shape<NT, kCoded>::kWarps * 32, 2) attend_kern
     // ---- and together: a warp per row, four dimensions a lane; over the first warp's where a cluster goes on with them
     const int groups = a.nsplit / a.cluster, grp = split / a.cluster;
     auto emit = [&](int r, const float4& acc, float top, float sum) {
-        const int row = r0 + r, node = row / a.group;
+        const int row = r0 + r, node = (uint32_t)row / (uint32_t)a.group;
         if (groups == 1) {
             const float inv = sum == 0.f ? 0.f : 1.f / sum;   // a row that sees nothing: 0
             A* out = static_cast<A*>(a.out) + (((size_t)m * a.T + node) * a.nq + head * a.group + row - node * a.group) * kHd + 4 * lane;

@@ -747,14 +747,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
     if (t == 0 && *abort_flag) atomicExch(a.status, kStatusMbarTimeout);
 }
 
-// Joins the records of contexts that several blocks have: a block per 32 rows of a head, a lane per row, 16 columns per warp; from
+// Joins the records of contexts that several blocks have: a block per 32 rows and 64 columns of a head, a lane per row, eight columns per warp; from
 // shared memory rows go out whole.
 template <typename A>
 __global__ void __launch_bounds__(256) attend_tc_merge_kernel(const Args a) {
-    __shared__ __align__(16) float s_out[32][kHd + 4];
+    __shared__ __align__(16) float s_out[32][64 + 4];
     pdl_trigger();
     pdl_wait();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r0 = blockIdx.x * 32, head = blockIdx.y, m = blockIdx.z;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r0 = (blockIdx.x >> 1) * 32, c0 = (blockIdx.x & 1) * 64, head = blockIdx.y, m = blockIdx.z;
     const Seq q = seq_of(a, m);
     const int rows = q.nodes * a.group;
     if (q.tiles == 0 || r0 >= rows) return;
@@ -773,46 +773,46 @@ __global__ void __launch_bounds__(256) attend_tc_merge_kernel(const Args a) {
     const size_t record = (size_t)a.rec_rows * kPart;
     const float* rec = a.part + row - g * a.group_rows;
     const size_t late = starts[b0] < x0 ? record : 0;              // (the first block may have other work before)
-    float top = -FLT_MAX, sum = 0.f, acc[16];
+    float top = -FLT_MAX, sum = 0.f, acc[8];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) acc[i] = 0.f;
-    for (int c0 = b0; c0 <= b1; c0 += 4) {                         // four records in flight
-        float v[4][16], mt[4], lt[4];
+    for (int i = 0; i < 8; ++i) acc[i] = 0.f;
+    for (int b = b0; b <= b1; b += 4) {                            // four records in flight
+        float v[4][8], mt[4], lt[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int c = min(c0 + j, b1);
-            const bool there = c0 + j <= b1 && starts[c] < starts[c + 1];
+            const int c = min(b + j, b1);
+            const bool there = b + j <= b1 && starts[c] < starts[c + 1];
             const float* at = rec + 2 * c * record + (c == b0 ? late : 0);
             mt[j] = there ? at[(size_t)kHd * a.rec_rows] : -FLT_MAX;
             lt[j] = there ? at[(size_t)(kHd + 1) * a.rec_rows] : 0.f;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[j][i] = there ? at[(size_t)(warp * 16 + i) * a.rec_rows] : 0.f;
+            for (int i = 0; i < 8; ++i) v[j][i] = there ? at[(size_t)(c0 + warp * 8 + i) * a.rec_rows] : 0.f;
         }
         const float to = fmaxf(top, fmaxf(fmaxf(mt[0], mt[1]), fmaxf(mt[2], mt[3]))), f = lm::exp2_fast(top - to);
         top = to;
         sum *= f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) acc[i] *= f;
+        for (int i = 0; i < 8; ++i) acc[i] *= f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const float e = lm::exp2_fast(mt[j] - to);
             sum = fmaf(lt[j], e, sum);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[i] = fmaf(v[j][i], e, acc[i]);
+            for (int i = 0; i < 8; ++i) acc[i] = fmaf(v[j][i], e, acc[i]);
         }
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-    for (int i = 0; i < 16; i += 4)
-        *reinterpret_cast<float4*>(&s_out[lane][warp * 16 + i]) = make_float4(acc[i] * inv, acc[i + 1] * inv, acc[i + 2] * inv, acc[i + 3] * inv);
+    for (int i = 0; i < 8; i += 4)
+        *reinterpret_cast<float4*>(&s_out[lane][warp * 8 + i]) = make_float4(acc[i] * inv, acc[i + 1] * inv, acc[i + 2] * inv, acc[i + 3] * inv);
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int r = r0 + warp + 8 * i;
+    for (int i = 0; i < 2; ++i) {
+        const int r = r0 + 2 * warp + (lane >> 4) + 16 * i;
         if (r >= rows) break;
         const uint32_t node = (uint32_t)r / (uint32_t)a.group;
-        store_o4(static_cast<A*>(a.out) + (((size_t)m * a.T + node) * a.nq + head * a.group + r - node * a.group) * kHd + 4 * lane,
-                 *reinterpret_cast<const float4*>(&s_out[r - r0][4 * lane]));
+        store_o4(static_cast<A*>(a.out) + (((size_t)m * a.T + node) * a.nq + head * a.group + r - node * a.group) * kHd + c0 + 4 * (lane & 15),
+                 *reinterpret_cast<const float4*>(&s_out[r - r0][4 * (lane & 15)]));
     }
 }
 

@@ -43,21 +43,25 @@ __device__ __forceinline__ float2 turn_of(long long position, unsigned long long
     return make_float2(c, s);
 }
 
+// A lane that warp_sum_many<N> leaves the sum of value j.
+template <int N>
+__device__ __forceinline__ constexpr int lane_of(int j) {
+    int lane = 0;
+    for (int w = N, off = 16; w > 1; w >>= 1, off >>= 1)
+        if (j & (w / 2)) lane |= off;
+    return lane;
+}
 // A warp takes HW heads of one row (token or node), four dimensions of each per lane.  x / sqrt(mean x^2 + eps) * w, then pairs
 // (2i, 2i + 1) turned; a cached row is stored in binary16, or divided by absmax / 448 and rounded to e4m3.
+constexpr int kWriteWarps = 12;         // warps of a block, at most
 template <typename A, int HW>
-__global__ void __launch_bounds__(256) write_rows_kernel(const WriteArgs a, const __grid_constant__ Turns turns) {
-    // (a lane's own entry of the parameters' constant bank costs a pass per lane: once per block)
-    __shared__ __align__(16) unsigned long long s_turns[kHd / 2];
+__global__ void __launch_bounds__(kWriteWarps * 32, 3) write_rows_kernel(const WriteArgs a, const __grid_constant__ Turns turns) {
+    __shared__ __align__(16) float2 s_turn[kHd / 2];                 // of the block's row, a pair of dimensions each
     pdl_trigger();
-    if (threadIdx.x < kHd / 2) s_turns[threadIdx.x] = turns.f[threadIdx.x];
-    __syncthreads();
     pdl_wait();
-    const int lane = threadIdx.x & 31, heads = a.nq + 2 * a.c.heads, per_row = (heads + HW - 1) / HW;
-    const long gw = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const long at = gw / per_row;                       // row of the call
-    if (at >= (long)a.M * a.T) return;
-    const int m = (int)(at / a.T), i = (int)(at - (long)m * a.T), h0 = (int)(gw - at * per_row) * HW;
+    const int lane = threadIdx.x & 31, heads = a.nq + 2 * a.c.heads;
+    const int m = blockIdx.x / (uint32_t)a.T, i = blockIdx.x - m * a.T, h0 = (blockIdx.y * (blockDim.x >> 5) + (threadIdx.x >> 5)) * HW;
+    const size_t at = blockIdx.x;                       // row of the call
     const int first = a.first[m];
     if (first < 0 || (a.count && i >= a.count[m])) return;
     const A* x = static_cast<const A*>(a.qkv) + (at * heads + h0) * kHd + 4 * lane;
@@ -65,13 +69,15 @@ __global__ void __launch_bounds__(256) write_rows_kernel(const WriteArgs a, cons
 #pragma unroll
     for (int j = 0; j < HW; ++j) v[j] = h0 + j < heads ? load_act4(x + j * kHd) : make_float4(0.f, 0.f, 0.f, 0.f);
     const int turned = a.nq + a.c.heads;                // heads that are normed and turned
+    for (int e = threadIdx.x; e < kHd / 2; e += blockDim.x)
+            s_turn[e] = turn_of((long long)first + (a.offset ? a.offset[at] : i), turns.f[e]);
+    __syncthreads();
     if (h0 < turned) {
         float4 qw = make_float4(1.f, 1.f, 1.f, 1.f), kw = qw;
         if (a.q_w && h0 < a.nq) qw = *reinterpret_cast<const float4*>(a.q_w + 4 * lane);
         if (a.k_w && h0 + HW > a.nq) kw = *reinterpret_cast<const float4*>(a.k_w + 4 * lane);
-        const long long p = (long long)first + (a.offset ? a.offset[at] : i);
-        const ulonglong2 per = *reinterpret_cast<const ulonglong2*>(&s_turns[2 * lane]);
-        const float2 r0 = turn_of(p, per.x), r1 = turn_of(p, per.y);
+        const float4 turn = *reinterpret_cast<const float4*>(&s_turn[2 * lane]);
+        const float2 r0 = make_float2(turn.x, turn.y), r1 = make_float2(turn.z, turn.w);
         float ss[HW];
 #pragma unroll
         for (int j = 0; j < HW; ++j) ss[j] = fmaf(v[j].w, v[j].w, fmaf(v[j].z, v[j].z, fmaf(v[j].y, v[j].y, v[j].x * v[j].x)));
@@ -84,7 +90,7 @@ __global__ void __launch_bounds__(256) write_rows_kernel(const WriteArgs a, cons
             const bool is_q = h < a.nq;
             float4 y = v[j];
             if (is_q ? a.q_w != nullptr : a.k_w != nullptr) {
-                const float is = __shfl_sync(0xffffffffu, root, HW == 1 ? 0 : (j >> 1) * 16 + (j & 1) * 8);   // warp_sum_many_index
+                const float is = __shfl_sync(0xffffffffu, root, lane_of<HW>(j));
                 const float4 g = is_q ? qw : kw;
                 y = make_float4(y.x * is * g.x, y.y * is * g.y, y.z * is * g.z, y.w * is * g.w);
             }
@@ -126,11 +132,14 @@ template <typename A>
 static cudaError_t write_launch(const WriteArgs& a, const Turns& turns, cudaStream_t st) {
     const int heads = a.nq + 2 * a.c.heads;
     const long rows = (long)a.M * a.T;
-    // Few rows: a warp per head, everything is latency.  Many: four heads a warp share the angles and keep four loads in flight.
+    // A block has a row, or part of its heads.  Few rows: a head per warp and two warps per block, everything is latency.  Many: four heads per
+    // warp.  Measured (8 x 512 rows, 32 / 8 heads, fp32 to 8 bits, 176 MB): 32.0 us, 5.5 TB/s; with the angles formed by every warp 34.3, in 64-bit
+    // floating point 37.6; eight heads per warp leave too few warps (44).
     const bool many = rows * heads > 32L * sm_count(current_device());
-    const long warps = rows * (many ? (heads + 3) / 4 : heads), blocks = (warps + 7) / 8;
-    if (blocks > 0x7FFFFFFFL) return cudaErrorInvalidValue;
-    const cudaError_t e = launch_pdl(many ? write_rows_kernel<A, 4> : write_rows_kernel<A, 1>, dim3((unsigned)blocks), dim3(256), 0, st, a, turns);
+    const int per_row = many ? (heads + 3) / 4 : heads, warps = many ? (per_row < kWriteWarps ? per_row : kWriteWarps) : 2;
+    const long parts = (per_row + warps - 1) / warps;
+    if (rows > 0x7FFFFFFFL || parts > 65535) return cudaErrorInvalidValue;
+    const cudaError_t e = launch_pdl(many ? write_rows_kernel<A, 4> : write_rows_kernel<A, 1>, dim3((unsigned)rows, (unsigned)parts), dim3(warps * 32), 0, st, a, turns);
     count_launch(1);
     return e != cudaSuccess ? e : cudaPeekAtLastError();
 }
