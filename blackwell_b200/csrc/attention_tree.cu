@@ -13,17 +13,23 @@ static int tiles_of_eight(int rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
 
 constexpr int kFewRows = 32;            // query rows of a head that the mma.sync kernel takes
 constexpr int kMaxCluster = 8;
-// Blocks that share a context of a (sequence, head, row tile).  Few of those: one wave of two blocks per SM, but two tiles of 16 positions
-// for each warp or more.  Many: a block has a context whole.  In any case about 512 positions for a warp at most, because its sums are
-// cut, not rounded, at 24 bits.  Measured (us, 32 / 8 heads, 8 bits, fp32): 1 x 2,048 positions 9.7 in 16 shares, 8.8 in 8; 32 x 4,096 to
-// 8,192 positions 123 in 8 shares, 95 in 4, 90 in 2.  Clusters of 16 need 16 free SMs next to each other: 1 x 2,048 positions with 64
-// rows 27 us, as two clusters of 8 and a merge 20.
-static int choose_splits(long pairs, int ctx, int slots, int warps) {
+constexpr int kCut = 512;               // positions of a warp: its sums are cut, not rounded, at 24 bits, which adds up
+// Blocks that share a context of a (sequence, head, row tile), a multiple of eight where more than a cluster.  Few contexts: one wave of two
+// blocks per SM, but two tiles of 16 positions for each warp or more.  Many: a block has a context whole.  In any case kCut positions for a
+// warp at most, as far as the records allow: rows of few heads have them for any length (scratch_bytes), many rows in two waves of blocks.
+// Measured (us, 32 / 8 heads, 8 bits, fp32): 1 x 2,048 positions 9.7 in 16 shares, 8.8 in 8; 32 x 4,096 to 8,192 positions 123 in 8 shares,
+// 95 in 4, 90 in 2.  Clusters of 16 need 16 free SMs next to each other: 1 x 2,048 positions with 64 rows 27 us, as two clusters of 8 and
+// a merge 20.
+static int choose_splits(long pairs, int ctx, int slots, int warps, bool few) {
     long n = slots / pairs;
-    if (n > ctx / (32 * warps)) n = ctx / (32 * warps);
-    if (n < ctx / (512 * warps)) n = ctx / (512 * warps);
-    const long most = 2L * slots / pairs;               // (more than a cluster leave records: not of many rows)
-    if (n > kMaxCluster && n > most) n = most > kMaxCluster ? most : kMaxCluster;
+    const long most = ctx / (32 * warps), least = (ctx + (long)kCut * warps - 1) / (kCut * warps);
+    if (n > most) n = most;
+    if (n > kMaxCluster) n = n / kMaxCluster * kMaxCluster;
+    if (n < least) {
+        n = least > kMaxCluster ? (least + kMaxCluster - 1) / kMaxCluster * kMaxCluster : least;
+        const long records = 2L * slots / pairs;
+        if (!few && n > kMaxCluster && n > records) n = records < kMaxCluster ? kMaxCluster : records / kMaxCluster * kMaxCluster;
+    }
     return n < 1 ? 1 : (int)n;
 }
 
@@ -37,10 +43,9 @@ static cudaError_t launch(Args a, int ctx, void* scratch, size_t scratch_bytes, 
         cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem);
         cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     });
-    a.nsplit = choose_splits((long)a.M * a.c.heads * a.tiles, ctx, 2 * sm_count(dev), Sh::kWarps);
+    a.nsplit = choose_splits((long)a.M * a.c.heads * a.tiles, ctx, 2 * sm_count(dev), Sh::kWarps, a.rows <= kFewRows);
     a.cluster = a.nsplit <= kMaxCluster ? a.nsplit : kMaxCluster;
     const int groups = a.nsplit / a.cluster;
-    a.nsplit = groups * a.cluster;
     if (groups > 1) {
         if (!scratch || scratch_bytes < (size_t)a.M * a.c.heads * a.rows * groups * kPart * sizeof(float)) return cudaErrorInvalidValue;
         a.part = static_cast<float*>(scratch);
@@ -119,12 +124,15 @@ static size_t kept_bytes(long blocks) { return (size_t)blocks * 2 * kHd * 128 * 
 }  // namespace tree
 }  // namespace bw
 
-// Bounds for any smaller call too: the blocks are at most as many as SMs (mma.sync kernel: records of 32 rows of two waves at most).
+// A bound for any smaller call too.  The blocks are at most as many as SMs; mma.sync kernel: records of 32 rows of two waves, or of long
+// contexts' shares of four warps for rows of few heads.
 extern "C" size_t bw_attention_tree_scratch_bytes(int M, int T, int num_q_heads, int num_kv_heads, int max_context) {
     if (M < 1 || T < 1 || T > tree::kMaxNodes || num_kv_heads < 1 || num_q_heads < 1 || num_q_heads % num_kv_heads || max_context < 1) return 0;
-    const int sms = sm_count(current_device()), rows = T * (num_q_heads / num_kv_heads);
-    if (rows <= tree::kFewRows) return tree::record_bytes(sms, 32);
-    return tree::kLineBytes + tree::record_bytes(sms, rows < 256 ? rows : 256) + tree::kept_bytes(sms);
+    const int sms = sm_count(current_device()), rows = T * (num_q_heads / num_kv_heads), few = rows < tree::kFewRows ? rows : tree::kFewRows;
+    size_t need = rows <= tree::kFewRows ? tree::record_bytes(sms, 32) : tree::kLineBytes + tree::record_bytes(sms, rows < 256 ? rows : 256) + tree::kept_bytes(sms);
+    const long positions = 4L * tree::kCut * tree::kMaxCluster, groups = ((long)max_context + positions - 1) / positions;
+    const size_t shares = (size_t)M * num_kv_heads * few * groups * tree::kPart * sizeof(float);
+    return groups > 1 && shares > need ? shares : need;
 }
 
 extern "C" int bw_attention_tree(void* out, const void* q, const bw_kv_cache* cache, const int* d_first_row,

@@ -287,6 +287,45 @@ def test_attention_value_scales_of_all_sizes(cuda):
         check_attention(1, 2, 4, 2, [390], 400, True, torch.float32, store=st)
 
 
+@BOTH
+@CACHES
+@pytest.mark.parametrize("M, T, nq, nkv, top", [(40, 9, 32, 8, 1500), (20, 64, 32, 8, 1200), (23, 13, 28, 4, 2050), (80, 3, 24, 8, 700), (460, 2, 20, 1, 300), (90, 40, 32, 8, 130)])
+def test_attention_many_tiles_of_a_block(cuda, M, T, nq, nkv, top, coded, act):
+    """Blocks that have whole contexts, several of them, many tiles of each, with and without a line of work."""
+    g = torch.Generator().manual_seed(M)
+    first = torch.randint(top // 2, top, (M,), generator=g).tolist()
+    first[M // 2], first[M // 3] = -1, 0
+    check_attention(M, T, nq, nkv, first, top + T, coded, act, masks=tree_masks(g, M, T), count=[T - m % 2 * (T // 3) if m % 7 else 0 for m in range(M)])
+
+
+@BOTH
+@CACHES
+@pytest.mark.parametrize("T", [5, 64])
+def test_attention_scores_and_values_that_grow(cuda, T, coded, act):
+    """The maximum and the values' scale move at many places of a long context, up or down."""
+    g = torch.Generator("cuda").manual_seed(T)
+    M, nq, nkv, top = 22, 32, 8, 1100
+    for falling in (False, True):
+        st = Store(g, M, 1, nkv, top + T, coded)
+        at = torch.linspace(0, 1, top + T, device="cuda")
+        at = at.flip(0) if falling else at
+        if coded:
+            st.ks *= 0.05 + 3 * at
+            st.vs *= 2 ** (at * 20 - 10)
+        else:
+            st.k *= (0.05 + 3 * at)[:, None].half()
+            st.v *= 2 ** (at * 10 - 5)[:, None].half()
+        check_attention(M, T, nq, nkv, [top - 31 * m for m in range(M)], top + T, coded, act, store=st, clean=False)
+
+
+@CACHES
+def test_attention_shares_of_long_contexts(cuda, coded):
+    """More shares than a cluster has blocks where there are heads enough for every SM."""
+    check_attention(10, 2, 16, 16, [20000 - 7 * m if m % 3 else 3000 for m in range(10)], 20100, coded, torch.float32)
+    if coded:
+        check_attention(19, 1, 8, 8, [33000 + m for m in range(19)], 34000, coded, torch.float32)
+
+
 def test_attention_far_offsets(cuda):
     """Sequences whose rows lie beyond 2^32 bytes and elements."""
     g = torch.Generator("cuda").manual_seed(4)
@@ -317,11 +356,12 @@ def test_attention_far_offsets(cuda):
 
 
 @CACHES
-def test_attention_same_bits_again_and_in_graphs(cuda, coded):
+@pytest.mark.parametrize("T, nq", [(4, 16), (60, 32)])
+def test_attention_same_bits_again_and_in_graphs(cuda, coded, T, nq):
     """Repeated calls, a captured one that is replayed with other positions, and calls on two streams at once."""
     g = torch.Generator("cuda").manual_seed(5)
     k = kernels()
-    M, T, nq, nkv = 2, 4, 16, 4
+    M, nkv = 2, 4
     st = Store(g, M, 1, nkv, 2100, coded)
     q = torch.randn((M, T, nq, HD), generator=g, device="cuda")
     first, out = ints([2000, 700]), torch.zeros((M, T, nq, HD), device="cuda")
