@@ -33,10 +33,10 @@ static int choose_splits(long pairs, int ctx, int slots, int warps, bool few) {
     return n < 1 ? 1 : (int)n;
 }
 
-template <int NT, bool kCoded, typename A>
+template <int NT, bool kCoded, typename A, bool kPair = false>
 static cudaError_t launch(Args a, int ctx, void* scratch, size_t scratch_bytes, cudaStream_t st) {
     using Sh = Shape<NT, kCoded>;
-    auto kern = attend_kernel<NT, kCoded, A>;
+    auto kern = attend_kernel<NT, kCoded, A, kPair>;
     static std::once_flag once[kMaxDevices];
     const int dev = current_device();
     std::call_once(once[dev], [&] {
@@ -74,6 +74,7 @@ static cudaError_t launch(Args a, int ctx, void* scratch, size_t scratch_bytes, 
 }
 template <bool kCoded, typename A>
 static cudaError_t launch_rows(const Args& a, int nt, int ctx, void* scratch, size_t bytes, cudaStream_t st) {
+    if (sizeof(A) == 4 && a.rows <= 4) return launch<1, kCoded, float, true>(a, ctx, scratch, bytes, st);
     return nt == 1 ? launch<1, kCoded, A>(a, ctx, scratch, bytes, st) : nt == 2 ? launch<2, kCoded, A>(a, ctx, scratch, bytes, st)
                                                                                 : launch<4, kCoded, A>(a, ctx, scratch, bytes, st);
 }

@@ -10,8 +10,9 @@
 // P goes from the accumulator layout to the operand layout by movmatrix.  e4m3 codes become f16 exactly (no rounding); the key scale
 // multiplies the score, the value scale the probability, there relative to the largest one met so far (a power of two), which keeps
 // the f16 operand in range whatever the values' size.
-// fp32 activations: Q and P are split in an f16 high part and an f16 remainder (22 significant bits) and multiplied twice; bfloat16
-// activations: once, which rounds P to 11 bits where the result keeps 8.  Each query row is brought to a maximum of 1 to 2 by a power
+// fp32 activations: Q and P are split in an f16 high part and an f16 remainder (22 significant bits) and multiplied twice, or, with four
+// rows or fewer (kPair), once with the remainders in the other four columns; bfloat16 activations: once, which rounds P to 11 bits where
+// the result keeps 8.  Each query row is brought to a maximum of 1 to 2 by a power
 // of two first.
 // The running maximum moves only when a score exceeds the reference by more than 2^14 / 2^6: otherwise no lane needs another's score.
 #pragma once
@@ -53,11 +54,11 @@ struct Shape {
     static constexpr int kStages = NT > 2 && !kCoded ? 2 : 3;              // (two blocks fit an SM)
     static constexpr int kWarps = NT == 1 && kCoded ? 8 : 4;               // two blocks per SM, as many warps as the registers allow
     static constexpr int kSide = kTile * kHd * (kCoded ? 1 : 2);           // bytes of 16 K or V rows
-    static constexpr int kStage = 2 * kSide;
+    static constexpr int kStage = 2 * kSide + (kCoded ? 2 * kTile * 4 : 0);  // ... and their scales
     static constexpr int kRing = kStages * kStage;
     static constexpr int kO = kRows * kHd * 4;                             // a warp's O, over its stages once they have drained
     static constexpr int kPerWarp = kRing > kO ? kRing : kO;
-    static constexpr int kQ = NT > 2 ? 8 * NT * 32 * 16 : 0;               // the query operand where it does not fit in registers
+    static constexpr int kQ = 8 * NT * 32 * 16;                            // the query operand, [k-step][tile][lane] high parts and remainders
     static constexpr int kSmem = kWarps * kPerWarp + kQ;
 };
 
@@ -76,17 +77,32 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// The same with a sum that starts at zero.
+__device__ __forceinline__ void mma_f16_new(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+// 4 bytes to shared memory on their way, zeros without `in`.
+__device__ __forceinline__ void cp_async4z(uint32_t to, const void* from, bool in) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(in ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ float lds_f32(uint32_t at) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at));
+    return v;
+}
+// (x, y) += (a, b), as one instruction.
+__device__ __forceinline__ void add2(float& x, float& y, float a, float b) {
+    asm("{\n\t.reg .b64 v, f;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 f, {%2, %3};\n\tadd.rn.f32x2 v, v, f;\n\tmov.b64 {%0, %1}, v;\n\t}" : "+f"(x), "+f"(y) : "f"(a), "f"(b));
+}
 __device__ __forceinline__ float4 ld_dsmem4(uint32_t addr, uint32_t rank) {
     uint32_t ra;
     float4 v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"(addr), "r"(rank));
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(ra) : "memory");
     return v;
-}
-__device__ __forceinline__ float2 load_q2(const float* p) { return *reinterpret_cast<const float2*>(p); }
-__device__ __forceinline__ float2 load_q2(const __nv_bfloat16* p) {
-    const uint32_t u = *reinterpret_cast<const uint32_t*>(p);
-    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
 }
 __device__ __forceinline__ float4 load_q4(const float* p) { return *reinterpret_cast<const float4*>(p); }
 __device__ __forceinline__ float4 load_q4(const __nv_bfloat16* p) {
@@ -111,11 +127,13 @@ __device__ __forceinline__ unsigned long long mask_of(const Args& a, int m, int 
     return (a.mask ? a.mask[(size_t)m * a.T + node] : low_bits(node + 1)) & low_bits(nodes);
 }
 
-template <int NT, bool kCoded, typename A>
+template <int NT, bool kCoded, typename A, bool kPair>
 __global__ void __launch_bounds__(Shape<NT, kCoded>::kWarps * 32, 2) attend_kernel(const Args a) {
     using Sh = Shape<NT, kCoded>;
     constexpr int kWarps = Sh::kWarps;
-    constexpr bool kSplit = sizeof(A) == 4;             // fp32 activations: two products
+    constexpr bool kSplit = sizeof(A) == 4 && !kPair;   // fp32 activations: two products
+    constexpr int kRowOf = kPair ? 3 : 7;               // row of a column, in bits
+    static_assert(!kPair || (NT == 1 && sizeof(A) == 4), "four rows");
     extern __shared__ __align__(128) unsigned char dsm[];
     __shared__ unsigned long long s_mask[Sh::kRows];
     __shared__ float s_m[kWarps][Sh::kRows], s_l[kWarps][Sh::kRows], s_unit[Sh::kRows];
@@ -148,6 +166,7 @@ __global__ void __launch_bounds__(Shape<NT, kCoded>::kWarps * 32, 2) attend_kern
     // 16 rows of K and V to a stage: piece c of rows rr, rr + kStep, ...; rows that nobody sees become zeros, whatever lies there
     const int c = lane % kChunks, rr = lane / kChunks;
     const uint32_t off = rr * kRowBytes + ((c ^ (rr & 7)) << 4);
+    const float* scale = kCoded ? (lane < kTile ? a.c.ks : a.c.vs) + row0 + (lane & (kTile - 1)) : nullptr;
     auto issue = [&](int tile, int stage) {
         const int p0 = tile * kTile;
         const uint32_t to = stage0 + stage * Sh::kStage;
@@ -160,6 +179,7 @@ __global__ void __launch_bounds__(Shape<NT, kCoded>::kWarps * 32, 2) attend_kern
                 amma::cp_async16(at, k + i * kStep * kRowBytes);
                 amma::cp_async16(at + Sh::kSide, v + i * kStep * kRowBytes);
             }
+            if (kCoded) cp_async4z(to + 2 * Sh::kSide + lane * 4, scale + p0, true);
         } else {
 #pragma unroll 1
             for (int i = 0; i < kTile / kStep; ++i) {
@@ -168,19 +188,10 @@ __global__ void __launch_bounds__(Shape<NT, kCoded>::kWarps * 32, 2) attend_kern
                 lm::cp_async16z(at, in ? k + i * kStep * kRowBytes : Kb, in);
                 lm::cp_async16z(at + Sh::kSide, in ? v + i * kStep * kRowBytes : Vb, in);
             }
-        }
-    };
-    // key and value scales of this thread's positions g, g + 8 of a tile
-    const float *ksp = kCoded ? a.c.ks + row0 + g : nullptr, *vsp = kCoded ? a.c.vs + row0 + g : nullptr;
-    auto scales_of = [&](int tile, float (&s)[4]) {
-        const int p0 = tile * kTile;
-        if (p0 + kTile <= ctx) {
-            s[0] = ksp[p0]; s[1] = ksp[p0 + 8];
-            s[2] = vsp[p0]; s[3] = vsp[p0 + 8];
-        } else {
-            const bool a0 = there(p0 + g), a1 = there(p0 + g + 8);
-            s[0] = a0 ? ksp[p0] : 0.f; s[1] = a1 ? ksp[p0 + 8] : 0.f;
-            s[2] = a0 ? vsp[p0] : 0.f; s[3] = a1 ? vsp[p0 + 8] : 0.f;
+            if (kCoded) {
+                const bool in = there(p0 + (lane & (kTile - 1)));
+                cp_async4z(to + 2 * Sh::kSide + lane * 4, scale + (in ? p0 : 0), in);
+            }
         }
     };
     int next = tile0 + warp;
@@ -190,69 +201,60 @@ __global__ void __launch_bounds__(Shape<NT, kCoded>::kWarps * 32, 2) attend_kern
         lm::cp_async_commit();
         next += kWarps;
     }
-    float sc[4] = {1.f, 1.f, 1.f, 1.f};
-    if (kCoded && tile0 + warp < tile1) scales_of(tile0 + warp, sc);
 
     // The query operand: column n of tile j is row r0 + 8 j + n.  Coded keys: a thread's four dimensions of k-step s are 32 tq + 4 s ...,
-    // as it finds them in 16 bytes of a key row; otherwise 16 s + 2 tq, + 1, + 8, + 9.  NT > 2: warp j prepares tile j for all.
-    constexpr int kRegs = NT > 2 ? 1 : NT;
-    uint32_t qh[kRegs][8][2], ql[kSplit ? kRegs : 1][8][2];
-    float qf[NT][2];                                    // factor of the scores of columns 2 tq, 2 tq + 1, base 2
+    // as it finds them in 16 bytes of a key row; otherwise 16 s + 2 tq, + 1, + 8, + 9.  Warp j brings tile j to its place, four lanes a row (each
+    // warp fetching its operand by itself takes 256 lines of the cache a warp: 2,000 cycles with eight).
     constexpr float kScore = 0.08838834764831845f * 1.4426950408889634f;
-#pragma unroll
-    for (int jj = 0; jj < kRegs; ++jj) {
-        const int j = NT > 2 ? warp : jj;
-        if (NT > 2 && warp >= NT) break;
-        const int r = r0 + 8 * j + g, node = (uint32_t)r / (uint32_t)a.group;
+    if (warp < NT) {
+        const int r = 8 * warp + g, row = r0 + r, node = (uint32_t)row / (uint32_t)a.group;
         const bool in = node < nodes;
-        const A* q = static_cast<const A*>(a.q) + (((size_t)m * a.T + (in ? node : 0)) * a.nq + head * a.group + (in ? r - node * a.group : 0)) * kHd;
-        float2 x[8][2];
+        const A* q = static_cast<const A*>(a.q) + (((size_t)m * a.T + (in ? node : 0)) * a.nq + head * a.group + (in ? row - node * a.group : 0)) * kHd + 4 * tq;
+        float4 x[8];
         float top = 0.f;
 #pragma unroll
-        for (int s = 0; s < 8; ++s)
+        for (int i = 0; i < 8; ++i) x[i] = in ? load_q4(q + 16 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int e = 0; e < 2; ++e) x[s][e] = in ? load_q2(q + (kCoded ? 32 * tq + 4 * s + 2 * e : 16 * s + 2 * tq + 8 * e)) : make_float2(0.f, 0.f);
-#pragma unroll
-        for (int s = 0; s < 8; ++s)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) top = fmaxf(top, fmaxf(fabsf(x[s][e].x), fabsf(x[s][e].y)));
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const float2 unit = binade(top);
 #pragma unroll
-        for (int s = 0; s < 8; ++s) {
-            uint32_t h[2], l[2] = {0, 0};
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                if (kSplit) {
-                    amma::split_hi_lo(x[s][e].x * unit.y, x[s][e].y * unit.y, h[e], l[e]);
-                } else {
-                    const __half2 v = __floats2half2_rn(x[s][e].x * unit.y, x[s][e].y * unit.y);
-                    h[e] = *reinterpret_cast<const uint32_t*>(&v);
-                }
-            }
-            if (NT > 2) {
-                s_q[(s * NT + j) * 32 + lane] = make_uint4(h[0], h[1], l[0], l[1]);
+        for (int i = 0; i < 8; ++i) {
+            uint4 f;
+            amma::split_hi_lo(x[i].x * unit.y, x[i].y * unit.y, f.x, f.z);
+            amma::split_hi_lo(x[i].z * unit.y, x[i].w * unit.y, f.y, f.w);
+            if (kCoded) {                               // lane l's operand of k-step s lies at l ^ s: banks
+                const int st = 4 * (i & 1) + tq;
+                s_q[(st * NT + warp) * 32 + ((4 * g + (i >> 1)) ^ st)] = f;
             } else {
-                qh[NT > 2 ? 0 : jj][s][0] = h[0]; qh[NT > 2 ? 0 : jj][s][1] = h[1];
-                if (kSplit) { ql[NT > 2 ? 0 : jj][s][0] = l[0]; ql[NT > 2 ? 0 : jj][s][1] = l[1]; }
+                uint32_t *p0 = reinterpret_cast<uint32_t*>(s_q + (i * NT + warp) * 32 + ((4 * g + 2 * (tq & 1)) ^ i)) + (tq >> 1),
+                         *p1 = reinterpret_cast<uint32_t*>(s_q + (i * NT + warp) * 32 + ((4 * g + 2 * (tq & 1) + 1) ^ i)) + (tq >> 1);
+                p0[0] = f.x; p0[2] = f.z;
+                p1[0] = f.y; p1[2] = f.w;
             }
         }
-        if (NT > 2) {
-            if (tq == 0) s_unit[8 * j + g] = unit.x;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 2; ++e)                 // (column 2 tq + e is lane group 2 tq + e's row)
-                qf[jj][e] = __shfl_sync(0xffffffffu, unit.x, (2 * tq + e) * 4) * kScore;
-        }
+        if (tq == 0) s_unit[r] = unit.x * kScore;
     }
     __syncthreads();                                    // masks, queries
-    if (NT > 2) {
+    constexpr int kRegs = NT > 2 ? 1 : NT;
+    uint32_t qh[kRegs][8][2], ql[kSplit ? kRegs : 1][8][2];
+    if (NT <= 2) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
+        for (int j = 0; j < kRegs; ++j)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) qf[j][e] = s_unit[8 * j + 2 * tq + e] * kScore;
+            for (int st = 0; st < 8; ++st) {
+                const uint4 f = s_q[(st * NT + j) * 32 + ((kPair ? lane & 15 : lane) ^ st)];
+                const bool low = kPair && lane > 15;
+                qh[j][st][0] = low ? f.z : f.x; qh[j][st][1] = low ? f.w : f.y;
+                if (kSplit) { ql[kSplit ? j : 0][st][0] = f.z; ql[kSplit ? j : 0][st][1] = f.w; }
+            }
     }
+    float qf[NT][2];                                    // factor of the scores of columns 2 tq, 2 tq + 1, base 2
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) qf[j][e] = s_unit[8 * j + ((2 * tq + e) & kRowOf)];
 
     float o[NT][8][4], mx[NT][2], l[NT][2], vref = __uint_as_float(2u << 23);
 #pragma unroll
@@ -268,11 +270,14 @@ __global__ void __launch_bounds__(Shape<NT, kCoded>::kWarps * 32, 2) attend_kern
         if (next < tile1) issue(next, stage == 0 ? Sh::kStages - 1 : stage - 1);
         lm::cp_async_commit();
         next += kWarps;
-        float sc_next[4] = {1.f, 1.f, 1.f, 1.f};
-        if (kCoded && tile + kWarps < tile1) scales_of(tile + kWarps, sc_next);
         lm::cp_async_wait<Sh::kStages - 1>();
         __syncwarp();
         const uint32_t ks = stage0 + stage * Sh::kStage, vs = ks + Sh::kSide;
+        float sc[4];                                    // scales of the keys g, g + 8 and of these values
+        if (kCoded) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[e] = lds_f32(ks + 2 * Sh::kSide + ((e >> 1) * kTile + g + 8 * (e & 1)) * 4);
+        }
 
         // ---- S^T: rows g, g + 8 of the tile's positions, columns 2 tq, 2 tq + 1 of each query tile
         float s[NT][4], s2[kSplit ? NT : 1][4];
@@ -285,7 +290,7 @@ __global__ void __launch_bounds__(Shape<NT, kCoded>::kWarps * 32, 2) attend_kern
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
                 if (NT > 2) {
-                    const uint4 b = s_q[(st * NT + j) * 32 + lane];
+                    const uint4 b = s_q[(st * NT + j) * 32 + (lane ^ st)];
                     mma_f16(s[j], k, b.x, b.y);
                     if (kSplit) mma_f16(s2[kSplit ? j : 0], k, b.z, b.w);
                 } else {
@@ -327,6 +332,7 @@ __global__ void __launch_bounds__(Shape<NT, kCoded>::kWarps * 32, 2) attend_kern
             for (int e = 0; e < 4; ++e) {
                 float x = s[j][e];
                 if (kSplit) x += s2[kSplit ? j : 0][e];
+                if (kPair) x += __shfl_xor_sync(0xffffffffu, x, 2);
                 x *= qf[j][e & 1];
                 if (kCoded) x *= sc[e >> 1];
                 s[j][e] = x;
@@ -337,7 +343,7 @@ __global__ void __launch_bounds__(Shape<NT, kCoded>::kWarps * 32, 2) attend_kern
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int p = p0 + g + 8 * (e >> 1);
-                    const bool yes = p < ctx || (p < end && (s_mask[8 * j + 2 * tq + (e & 1)] >> (p - ctx) & 1));
+                    const bool yes = p < ctx || (p < end && (s_mask[8 * j + ((2 * tq + (e & 1)) & kRowOf)] >> (p - ctx) & 1));
                     s[j][e] = yes ? s[j][e] : -INFINITY;
                 }
         }
@@ -399,6 +405,10 @@ __global__ void __launch_bounds__(Shape<NT, kCoded>::kWarps * 32, 2) attend_kern
                     amma::split_hi_lo(p[2 * e], p[2 * e + 1], h, lo);
                     ph[j][e] = transpose8x8(h);
                     pl[kSplit ? j : 0][e] = transpose8x8(lo);
+                } else if (kPair) {
+                    uint32_t h, lo;
+                    amma::split_hi_lo(p[2 * e], p[2 * e + 1], h, lo);
+                    ph[j][e] = transpose8x8(tq < 2 ? h : lo);
                 } else {
                     const __half2 h = __floats2half2_rn(p[2 * e], p[2 * e + 1]);
                     ph[j][e] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h));
@@ -409,8 +419,20 @@ __global__ void __launch_bounds__(Shape<NT, kCoded>::kWarps * 32, 2) attend_kern
         auto value_step = [&](int d, const uint32_t (&v)[4]) {
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-                mma_f16(o[j][d], v, ph[j][0], ph[j][1]);
-                if (kSplit) mma_f16(o[j][d], v, pl[kSplit ? j : 0][0], pl[kSplit ? j : 0][1]);
+                if (kSplit) {
+                    float c[4];
+                    mma_f16_new(c, v, pl[kSplit ? j : 0][0], pl[kSplit ? j : 0][1]);
+                    mma_f16(c, v, ph[j][0], ph[j][1]);
+                    add2(o[j][d][0], o[j][d][1], c[0], c[1]);
+                    add2(o[j][d][2], o[j][d][3], c[2], c[3]);
+                } else if (kPair) {
+                    float c[4];
+                    mma_f16_new(c, v, ph[j][0], ph[j][1]);
+                    add2(o[j][d][0], o[j][d][1], c[0], c[1]);
+                    add2(o[j][d][2], o[j][d][3], c[2], c[3]);
+                } else {
+                    mma_f16(o[j][d], v, ph[j][0], ph[j][1]);
+                }
             }
         };
         if (kCoded) {
@@ -444,8 +466,6 @@ __global__ void __launch_bounds__(Shape<NT, kCoded>::kWarps * 32, 2) attend_kern
         }
         __syncwarp();                                   // the stage is filled again in the next turn
         stage = stage == Sh::kStages - 1 ? 0 : stage + 1;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sc[i] = sc_next[i];
     }
     lm::cp_async_wait<0>();
     __syncwarp();
@@ -453,6 +473,17 @@ __global__ void __launch_bounds__(Shape<NT, kCoded>::kWarps * 32, 2) attend_kern
     // ---- the warps' results to shared memory: [row][128]
     float* so = reinterpret_cast<float*>(dsm + warp * Sh::kPerWarp);
     const float vmul = kCoded ? vref : 1.f;
+    if (kPair) {                                        // high parts and remainders: lanes of columns 0-3 get dimension tiles 0-3, the others 4-7
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float mine = tq < 2 ? o[0][d][e] : o[0][d + 4][e], other = tq < 2 ? o[0][d + 4][e] : o[0][d][e];
+                o[0][d][e] = mine + __shfl_xor_sync(0xffffffffu, other, 2);
+            }
+    }
+    constexpr int kTiles = kPair ? 4 : 8;
+    const int d0 = kPair && tq > 1 ? 4 : 0;
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -461,15 +492,15 @@ __global__ void __launch_bounds__(Shape<NT, kCoded>::kWarps * 32, 2) attend_kern
             sum += __shfl_xor_sync(0xffffffffu, sum, 4);
             sum += __shfl_xor_sync(0xffffffffu, sum, 8);
             sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-            const int r = 8 * j + 2 * tq + e;
+            const int r = 8 * j + ((2 * tq + e) & kRowOf);
             if (g == 0) { s_m[warp][r] = mx[j][e]; s_l[warp][r] = sum; }
 #pragma unroll
-            for (int d = 0; d < 8; ++d) {
+            for (int d = 0; d < kTiles; ++d) {
                 if (kCoded) {
-                    *reinterpret_cast<float2*>(so + r * kHd + 16 * g + 2 * d) = make_float2(o[j][d][e] * vmul, o[j][d][e + 2] * vmul);
+                    *reinterpret_cast<float2*>(so + r * kHd + 16 * g + 2 * (d0 + d)) = make_float2(o[j][d][e] * vmul, o[j][d][e + 2] * vmul);
                 } else {
-                    so[r * kHd + 16 * d + g] = o[j][d][e];
-                    so[r * kHd + 16 * d + g + 8] = o[j][d][e + 2];
+                    so[r * kHd + 16 * (d0 + d) + g] = o[j][d][e];
+                    so[r * kHd + 16 * (d0 + d) + g + 8] = o[j][d][e + 2];
                 }
             }
         }

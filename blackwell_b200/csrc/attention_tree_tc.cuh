@@ -65,13 +65,10 @@ struct Part {
 __device__ __forceinline__ void mul2(float& x, float& y, float fx, float fy) {
     asm("{\n\t.reg .b64 v, f;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 f, {%2, %3};\n\tmul.rn.f32x2 v, v, f;\n\tmov.b64 {%0, %1}, v;\n\t}" : "+f"(x), "+f"(y) : "f"(fx), "f"(fy));
 }
-// (x, y) = (x, y) * f + c and (x, y) += (a, b), as one instruction each.
+// (x, y) = (x, y) * f + c, as one instruction.
 __device__ __forceinline__ void fma2(float& x, float& y, float f, float c) {
     asm("{\n\t.reg .b64 v, f, c;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 f, {%2, %2};\n\tmov.b64 c, {%3, %3};\n\tfma.rn.f32x2 v, v, f, c;\n\tmov.b64 {%0, %1}, v;\n\t}"
         : "+f"(x), "+f"(y) : "f"(f), "f"(c));
-}
-__device__ __forceinline__ void add2(float& x, float& y, float a, float b) {
-    asm("{\n\t.reg .b64 v, f;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 f, {%2, %3};\n\tadd.rn.f32x2 v, v, f;\n\tmov.b64 {%0, %1}, v;\n\t}" : "+f"(x), "+f"(y) : "f"(a), "f"(b));
 }
 // f16 high parts and remainders of a pair.
 __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
