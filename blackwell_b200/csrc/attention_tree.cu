@@ -13,22 +13,27 @@ static int tiles_of_eight(int rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
 
 constexpr int kFewRows = 32;            // query rows of a head that the mma.sync kernel takes
 constexpr int kMaxCluster = 8;
-constexpr int kCut = 512;               // positions of a warp: its sums are cut, not rounded, at 24 bits, which adds up
+constexpr int kCut = 512;               // positions of a warp, where contexts are long: their lengths differ, and the last block is waited for
 // Blocks that share a context of a (sequence, head, row tile), a multiple of eight where more than a cluster.  Few contexts: one wave of two
-// blocks per SM, but two tiles of 16 positions for each warp or more.  Many: a block has a context whole.  In any case kCut positions for a
-// warp at most, as far as the records allow: rows of few heads have them for any length (scratch_bytes), many rows in two waves of blocks.
-// Measured (us, 32 / 8 heads, 8 bits, fp32): 1 x 2,048 positions 9.7 in 16 shares, 8.8 in 8; 32 x 4,096 to 8,192 positions 123 in 8 shares,
-// 95 in 4, 90 in 2.  Clusters of 16 need 16 free SMs next to each other: 1 x 2,048 positions with 64 rows 27 us, as two clusters of 8 and
-// a merge 20.
+// blocks per SM, but two tiles of 16 positions for each warp or more.  Many: kCut positions for a warp at most, as far as the records allow
+// (rows of few heads: any number, scratch_bytes; many rows: two waves of blocks), and one or two more where that fills the last wave.
+// Measured (us, 32 / 8 heads, 8 bits, fp32): 32 x 4,096 to 8,192 positions in 1 to 8 shares 75 74 75 76 79 85 95, 20 x 3,000 to 6,000 48 47 41 44
+// 43 48 54, 8 x 2,000 to 4,000 24 20 17 15 22 22 21.  Clusters of 16 need 16 free SMs next to each other: 1 x 2,048 positions with 64 rows 27 us,
+// as two clusters of 8 and a merge 20.
 static int choose_splits(long pairs, int ctx, int slots, int warps, bool few) {
     long n = slots / pairs;
     const long most = ctx / (32 * warps), least = (ctx + (long)kCut * warps - 1) / (kCut * warps);
     if (n > most) n = most;
     if (n > kMaxCluster) n = n / kMaxCluster * kMaxCluster;
-    if (n < least) {
-        n = least > kMaxCluster ? (least + kMaxCluster - 1) / kMaxCluster * kMaxCluster : least;
+    if (n < least && least > kMaxCluster) {
+        n = (least + kMaxCluster - 1) / kMaxCluster * kMaxCluster;
         const long records = 2L * slots / pairs;
-        if (!few && n > kMaxCluster && n > records) n = records < kMaxCluster ? kMaxCluster : records / kMaxCluster * kMaxCluster;
+        if (!few && n > records) n = records < kMaxCluster ? kMaxCluster : records / kMaxCluster * kMaxCluster;
+    } else if (n < least) {
+        auto waves = [&](long k) { return (pairs * k + slots - 1) / slots; };
+        n = least;
+        for (long k = least + 1; k <= least + 2 && k <= kMaxCluster && k * (kCut / 4) * warps <= ctx; ++k)
+            if (20 * waves(k) * n < 19 * waves(n) * k) n = k;
     }
     return n < 1 ? 1 : (int)n;
 }
@@ -99,14 +104,14 @@ static cudaError_t launch_tc_rows(const Args& a, cudaStream_t st) {
 }
 
 // Which kernel.  The tcgen05 kernel takes some 20 us before it pays (queries into shared memory, the pipeline's start, records and their merge); a
-// tile of the mma.sync kernel (32 rows, 16 positions) takes a block 0.5 us.  So: by the tiles that an SM gets, and not for one or two row
-// tiles, which leave the 128 lanes of an accumulator half empty, unless there is much of it.  Measured (us, mma.sync / tcgen05; 32 / 8 heads, fp32): 64 nodes,
-// 8 x 2,048 positions 108 / 66, 4 x 1,000 39 / 36, 4 x 300 21 / 31; 24 nodes, 8 x 2,048 62 / 44, 4 x 1,000 22 / 27, 32 x 100 38 / 24; 16 nodes,
-// 32 x 1,000 62 / 71, 32 x 8,192 383 / 346.
+// tile of the mma.sync kernel (32 rows, 16 positions) takes a block 0.4 us.  So: by the tiles that an SM gets, and not for one or two row
+// tiles, which leave the 128 lanes of an accumulator half empty, unless there is much of it.  Measured (us, mma.sync / tcgen05; 32 / 8 heads, fp32,
+// 8 bits): 64 nodes, 8 x 2,048 positions 152 / 65, 4 x 1,000 40 / 34, 4 x 300 21 / 30; 24 nodes, 8 x 2,048 55 / 42, 4 x 1,000 22 / 28; 16 nodes,
+// 32 x 1,000 67 / 77, 8 x 5,310 83 / 74; 8 nodes, 32 x 4,000 117 / 189.
 static bool many_rows(long heads, int rows, int ctx, int sms) {
     if (rows <= kFewRows) return false;
     const double tiles = (double)heads * ((rows + 31) / 32) * ((ctx + 15) / 16) / sms;
-    return tiles >= (rows <= 64 ? 600 : ctx <= 128 ? 40 : 80);
+    return tiles >= (rows <= 64 ? 280 : ctx <= 128 ? 40 : 80);
 }
 static int g_route = 0;   // experiments: 1 mma.sync, 2 tcgen05
 void set_route(int v) { g_route = v; }

@@ -7,8 +7,9 @@
 // (ln keep + 1), so that after the first turns hardly a warp has one.  The maxima only grow, so that warps share them without waiting for
 // each other: a stale one lowers the bar.  A list that has grown is cut to its best.  The second launch, a block per request, forms the rows' log-sums and ranks the
 // stretches' candidates across the beams, scores in 64 bits: two beams' candidates may lie closer to each other than 32 bits tell apart.
-// The exponentials are 32-bit, taken of differences that are exact where they matter; their roundings average out in the sum.  64-bit exp
-// and log are avoided: a chain of some 300 64-bit instructions took the merge 5 us.
+// The exponentials and their sums are 32-bit, taken of differences that are exact where they matter; a log-sum is right to some 1e-7.
+// Measured (16 x 8 beams of 151,643 tokens, 78 MB): 25.5 us, 3.0 TB/s, of which the merge and its launch are 5; the first launch alone is bound
+// by the instructions that a value takes, not by memory (the exponentials some 5 us of it).  1 x 4 beams of 32,768: 8 us, two launches' latency.
 #include <float.h>
 
 #include "common.cuh"
@@ -393,7 +394,7 @@ static size_t bytes_of(long records, int keep) {
 }
 static bool sizes_ok(int vocab, int beams, int keep, int M) {
     return vocab >= 1 && beams >= 1 && beams <= kMaxBeams && keep >= 1 && keep <= kMaxKeep && M >= 1 && (long)M * beams <= 65535 &&
-           (long)beams * vocab < 0x7FFFFFFFL;
+           (long)beams * vocab <= 0x7FFF0000L;   // (vectors of a turn past the end are counted in 32 bits)
 }
 
 }  // namespace beam
@@ -412,6 +413,7 @@ extern "C" int bw_beam_select(int* parent_out, int* token_out, float* score_out,
                               int M, void* scratch, size_t scratch_bytes, void* stream) {
     if (!beam::sizes_ok(vocab, beams, keep, M) || !parent_out || !token_out || !score_out || !logits || !score || !scratch) return cudaErrorInvalidValue;
     if (row_stride < vocab || (ended_or_null && (eos_id < 0 || eos_id >= vocab)) || !kv::aligned(scratch, 16)) return cudaErrorInvalidValue;
+    if (keep != beams && (score_out == score || (ended_or_null && ended_out_or_null == ended_or_null))) return cudaErrorInvalidValue;   // (other requests' are still read)
     const long rows = (long)M * beams;
     beam::Args a{};
     beam::stretches(vocab, beams, rows, sm_count(current_device()), &a);

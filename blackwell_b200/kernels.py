@@ -316,6 +316,8 @@ class KVCache:
             raise ValueError("contiguous tensors of one device")
         if k.numel() != v.numel() or (coded and any(s.dtype != torch.float32 or s.numel() * 128 != k.numel() for s in (k_scale, v_scale))):
             raise ValueError("k, v and their scales (fp32, one per row of 128) have the same rows")
+        if min(kv_heads, max_seq) < 1 or min(batch_elems, layer_elems) < 0:
+            raise ValueError("kv_heads and max_seq are positive, batch_elems and layer_elems not negative")
         self.tensors, self.index, self.rows = tuple(sides), k.get_device(), k.numel() // 128
         self.kv_heads, self.max_seq, self.batch_elems, self.layer_elems = kv_heads, max_seq, batch_elems, layer_elems
         self._args = _KVCacheArgs(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if coded else None, v_scale.data_ptr() if coded else None,
@@ -325,7 +327,7 @@ class KVCache:
     def _check(self, name, sequences, layers=1, layer_stride=0):
         """The rows that a call addresses lie inside the tensors, on the current device."""
         last = (sequences - 1) * self.batch_elems + self.layer_elems + (layers - 1) * layer_stride
-        if sequences < 1 or layers < 1 or last // 128 + self.kv_heads * self.max_seq > self.rows:
+        if sequences < 1 or layers < 1 or layer_stride < 0 or last // 128 + self.kv_heads * self.max_seq > self.rows:
             raise ValueError(f"{name}: the cache has {self.rows} rows; {sequences} sequences and {layers} layers reach past them")
         if self.index != torch.cuda.current_device():
             raise ValueError(f"{name}: the cache is on device {self.index}, not on the current one")

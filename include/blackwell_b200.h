@@ -335,13 +335,14 @@ size_t bw_attention_tree_scratch_bytes(int M, int T, int num_q_heads, int num_kv
  * tokens, of which the `keep` best (largest first; equal ones by lower beam, then token) go to parent_out, token_out, score_out [M][keep].  logits fp32 [M * beams][row_stride].
  * A beam that has ended (ended[m][b] != 0) offers itself alone, as (eos_id, score unchanged); ended_out = ended[parent] or token == eos_id.
  * Candidates of score -inf are none: where fewer than `keep` are left, parent and token are -1 and the score -inf.  A NaN logit counts as -inf; a
- * row with a logit of +inf offers nothing.  Log-sums and comparisons are in 64 bits.  beams <= 64, keep <= 64.  score_out may be score and
- * ended_out ended, with keep == beams. */
+ * row with a logit of +inf offers nothing.  Scores are formed and compared in 64 bits; a log-sum is right to some 1e-7.  beams <= 64, keep <= 64.
+ * score_out may be score and ended_out ended, with keep == beams. */
 int bw_beam_select(int* parent_out, int* token_out, float* score_out, unsigned char* ended_out_or_null, const float* logits, long row_stride,
                    int vocab, const float* score, const unsigned char* ended_or_null, int eos_id, int beams, int keep, int M, void* scratch,
                    size_t scratch_bytes, void* stream);
 size_t bw_beam_select_scratch_bytes(int vocab, int beams, int keep, int M);
-/* Moves rows inside a cache, in `layers` layers from layer_elems on, layer_stride_elems apart (a multiple of 128).
+/* Moves rows inside a cache, in `layers` layers from layer_elems on, layer_stride_elems apart (a multiple of 128): all layers of a sequence
+ * together, or all sequences of a layer.
  * bw_kv_reorder: sequence m * beams + b takes the rows [from[m], to[m]) (from NULL: 0; cut off at max_seq) of sequence m * beams + parent[m][b], all beams at
  * once: a beam may be overwritten and the parent of others.  A parent outside of 0 .. beams - 1 leaves its beam as it is.  beams <= 32.
  * bw_kv_keep_rows: row first[m] + i takes row first[m] + path[m][i] for i < count[m], all at once (path [M][T], T <= 64): the accepted

@@ -45,7 +45,7 @@ def attend(lib, c=None, **kw):
 
 
 def select(lib, **kw):
-    a = {**dict(parent=P, token=P, out=P, logits=P, stride=100, vocab=100, score=P, ended=P, eos=2, beams=4, keep=4, M=2, scratch=P, n=1 << 30), **kw}
+    a = {**dict(parent=P, token=P, out=2 * P, logits=P, stride=100, vocab=100, score=P, ended=P, eos=2, beams=4, keep=4, M=2, scratch=P, n=1 << 30), **kw}
     return lib.bw_beam_select(C.c_void_p(a["parent"]), C.c_void_p(a["token"]), C.c_void_p(a["out"]), None, C.c_void_p(a["logits"]), C.c_long(a["stride"]),
                               a["vocab"], C.c_void_p(a["score"]), C.c_void_p(a["ended"]), a["eos"], a["beams"], a["keep"], a["M"], C.c_void_p(a["scratch"]),
                               C.c_size_t(a["n"]), None)
@@ -78,7 +78,8 @@ def test_bad_caches(lib, call, bad):
     (select, dict(parent=None)), (select, dict(token=None)), (select, dict(out=None)), (select, dict(logits=None)), (select, dict(score=None)),
     (select, dict(vocab=0)), (select, dict(stride=99)), (select, dict(eos=100)), (select, dict(eos=-1)), (select, dict(beams=0)), (select, dict(beams=65)),
     (select, dict(keep=0)), (select, dict(keep=65)), (select, dict(M=0)), (select, dict(scratch=None)), (select, dict(scratch=P + 4)), (select, dict(n=8)),
-    (select, dict(beams=64, vocab=1 << 30, stride=1 << 30)),
+    (select, dict(beams=64, vocab=1 << 30, stride=1 << 30)), (select, dict(beams=1, keep=1, vocab=(1 << 31) - 2, stride=1 << 31)),
+    (select, dict(out=P, score=P, keep=3)),
     (reorder, dict(parent=None)), (reorder, dict(to=None)), (reorder, dict(beams=0)), (reorder, dict(beams=33)), (reorder, dict(M=0)), (reorder, dict(layers=0)),
     (reorder, dict(stride=8 * 64 * 128 - 128)), (reorder, dict(stride=8 * 64 * 128 + 64)), (reorder, dict(M=70000)),
     (keep, dict(first=None)), (keep, dict(path=None)), (keep, dict(count=None)), (keep, dict(M=0)), (keep, dict(T=0)), (keep, dict(T=65)), (keep, dict(layers=0)),
@@ -92,6 +93,14 @@ def test_refusals(lib, call, bad):
 def test_sequences_that_are_written_do_not_overlap(lib, call):
     assert call(lib, cache(batch_elems=8 * 64 * 128 - 128)) == INVALID
     assert call(lib, cache(batch_elems=0)) == INVALID
+
+
+@pytest.mark.parametrize("call", [reorder, keep])
+def test_layers_and_sequences_that_share_rows(lib, call):
+    plane = 8 * 64 * 128
+    for batch, stride in ((plane, plane), (2 * plane, 3 * plane), (3 * plane - 128, 2 * plane)):
+        assert call(lib, cache(batch_elems=batch), layers=2, stride=stride, M=4) == INVALID
+    assert call(lib, layers=1 << 28) == INVALID
 
 
 def test_no_cache_at_all(lib):

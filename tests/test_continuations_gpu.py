@@ -525,8 +525,53 @@ def test_reorder_of_nothing(cuda, coded):
     st = Store(torch.Generator("cuda").manual_seed(1), 4, 1, 2, 30, coded)
     before = st.bits()
     kernels().kv_reorder(st.args(), ints([[1, 0], [1, 0]]), ints([9, -4]), ints([9, -1]), 2, 2, 1, st.plane)
+    kernels().kv_reorder(st.args(), ints([[1, 0], [1, 0]]), ints([2 ** 31 - 1, 1]), ints([-2 ** 31, 1 - 2 ** 31]), 2, 2, 1, st.plane)
     kernels().kv_reorder(st.args(), ints([[0, 1], [0, 1]]), None, ints([30, 30]), 2, 2, 1, st.plane)
     assert all(torch.equal(a, b) for a, b in zip(before, st.bits()))
+
+
+@CACHES
+def test_layers_around_sequences(cuda, coded):
+    """A cache [layer][sequence]: rows moved between beams and along paths, and one layer's attention."""
+    g = torch.Generator("cuda").manual_seed(12)
+    k, L, M, B, nkv, top = kernels(), 3, 2, 3, 2, 40
+    st = Store(g, L, M * B, nkv, top, coded)
+    sides = [t.view(torch.uint8) for t in (st.k, st.v) + ((st.ks, st.vs) if coded else ())]
+    rows = lambda t: t.view(L, M, B, nkv, top, -1)  # noqa: E731
+    before = [rows(t).clone() for t in sides]
+    cache = lambda layer: k.KVCache(st.k, st.v, st.ks, st.vs, nkv, top, st.plane, layer * M * B * st.plane)  # noqa: E731
+    k.kv_reorder(cache(0), ints([[1, 2, 0], [2, 1, 2]]), ints([4, 0]), ints([17, 33]), B, M, L, M * B * st.plane)
+    for m, (parents, lo, hi) in enumerate((((1, 2, 0), 4, 17), ((2, 1, 2), 0, 33))):
+        for t, old in zip(sides, before):
+            want = old[:, m].clone()
+            want[:, :, :, lo:hi] = old[:, m][:, list(parents), :, lo:hi]
+            assert torch.equal(rows(t)[:, m], want)
+    now = [rows(t).clone() for t in sides]
+    k.kv_keep_rows(cache(1), ints([5] * 6), ints([[0, 2, 3]] * 6), ints([3] * 6), M * B, 3, L - 1, M * B * st.plane)
+    for t, old in zip(sides, now):
+        want = old.clone()
+        want[1:, :, :, :, 5:8] = old[1:, :, :, :, [5, 7, 7]]   # (path 3 is not inside 0 .. T - 1)
+        assert torch.equal(rows(t), want)
+    q = torch.randn((M * B, 2, 4, HD), generator=g, device="cuda")
+    outs = [torch.zeros_like(q) for _ in range(2)]
+    k.attention_tree(outs[0], q, cache(2), ints([30] * 6), None, None, 0, 4, M * B, 2, None)
+    k.attention_tree(outs[1], q, k.KVCache(st.k[2], st.v[2], st.ks[2] if coded else None, st.vs[2] if coded else None, nkv, top, st.plane), ints([30] * 6),
+                     None, None, 0, 4, M * B, 2, None)
+    assert torch.equal(*outs) and bool(outs[0].any())
+
+
+@CACHES
+def test_sequences_that_share_a_cache(cuda, coded):
+    """batch_elems 0: every sequence reads the same rows."""
+    g = torch.Generator("cuda").manual_seed(13)
+    k, M, nkv, top = kernels(), 5, 2, 300
+    st = Store(g, 1, 1, nkv, top, coded)
+    q = torch.randn((M, 3, 4, HD), generator=g, device="cuda")
+    out, one = torch.zeros_like(q), torch.zeros_like(q)
+    for n, o in ((M, out), (1, one)):
+        for m in range(0, M, n):
+            k.attention_tree(o[m:m + n], q[m:m + n], k.KVCache(st.k, st.v, st.ks, st.vs, nkv, top, 0), ints([290] * n), None, None, 0, 4, n, 3, None)
+    assert torch.equal(out, one) and bool(out.any())
 
 
 @CACHES
@@ -645,6 +690,11 @@ def test_refused_tensors(cuda):
         k.KVCache(st.k, st.v, None, None, 2, 16, st.plane)
     with pytest.raises(ValueError):
         k.KVCache(st.k, st.v, st.ks[:1], st.vs, 2, 16, st.plane)
+    for bad in ((2, 16, -HD), (2, 16, st.plane, -HD), (0, 16, st.plane), (2, 0, st.plane)):
+        with pytest.raises(ValueError):
+            k.KVCache(st.k, st.v, st.ks, st.vs, *bad)
+    with pytest.raises(ValueError):
+        k.kv_reorder(st.args(), ints([0, 0]), None, ints([4]), 2, 1, 1, -HD)
     ok = (q, q, st.args(), ints([0, 0]), None, None, 0, 4, 2, 1, None)
     k.attention_tree(*ok)
     for i, bad in ((0, q[:1]), (0, q.half()), (1, q.transpose(0, 2)), (3, torch.zeros(2, device="cuda")), (3, torch.zeros(2, dtype=torch.int32)), (4, ints([0, 0])),
