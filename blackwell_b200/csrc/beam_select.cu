@@ -1,6 +1,6 @@
 // Beam search's selection: of the candidates  score[b] + log_softmax(logits[b])[v]  of a request's beams the best few.
 //
-// Two launches.  The first reads the logits once, a stretch of a row per block, 4,096 values at a time with the next ones in flight.  A
+// Two launches, or one of clusters that joins them.  The first reads the logits once, a stretch of a row per block, 4,096 values at a time with the next ones in flight.  A
 // warp works by itself: running maxima and sums of exponentials per lane, and a list of the values that may be among the `keep` largest of
 // the stretch (within a row the order of the candidates is that of the logits).  What enters the list is at or above a bar: the
 // smallest of the running maxima of `keep` or more groups of the block's threads.  At least `keep` values lie there, of the first n some keep *
@@ -9,8 +9,10 @@
 // stretches' candidates across the beams, scores in 64 bits: two beams' candidates may lie closer to each other than 32 bits tell apart.
 // The exponentials and their sums are 32-bit, taken of differences that are exact where they matter; a log-sum is right to some 1e-7.
 // Measured (16 x 8 beams of 151,643 tokens, 78 MB): 25.5 us, 3.0 TB/s, of which the merge and its launch are 5; the first launch alone is bound
-// by the instructions that a value takes, not by memory (the exponentials some 5 us of it).  1 x 4 beams of 32,768: 8 us, two launches' latency.
+// by the instructions that a value takes, not by memory (the exponentials some 5 us of it).
 #include <float.h>
+
+#include <mutex>
 
 #include "common.cuh"
 #include "host_util.h"
@@ -124,6 +126,116 @@ __device__ __forceinline__ float exponentials(const float4 (&v)[kVec], float to)
     return (p[0] + p[1]) + (p[2] + p[3]);
 }
 
+// The best of up to 64 sorted lists, two per lane, one after the other: head(l, i) is entry i of list l (score 0: none), emit(r, cand)
+// takes the r-th best, by the lane that holds it.  A round is three warp-wide integer reductions; only the winner's list moves on.
+template <typename Head, typename Emit>
+__device__ __forceinline__ void tournament(int lists, int keep, int lane, const Head& head, const Emit& emit) {
+    Cand x[2];
+    int i[2] = {0, 0};
+#pragma unroll
+    for (int e = 0; e < 2; ++e) x[e] = lane + 32 * e < lists ? head(lane + 32 * e, 0) : Cand{0, 0};
+    for (int r = 0; r < keep; ++r) {
+        const int e = before(x[1], x[0]);
+        const Cand y = e ? x[1] : x[0];
+        const uint32_t hi = (uint32_t)(y.score >> 32), lo = (uint32_t)y.score;
+        const uint32_t mhi = __reduce_max_sync(0xffffffffu, hi);
+        const uint32_t mlo = __reduce_max_sync(0xffffffffu, hi == mhi ? lo : 0u);
+        const bool tied = hi == mhi && lo == mlo;
+        const uint32_t at = __reduce_min_sync(0xffffffffu, tied ? y.at : 0xFFFFFFFFu);
+        if (mhi == 0 && mlo == 0) {
+            if (lane == 0)
+                for (; r < keep; ++r) emit(r, Cand{0, 0});
+            break;
+        }
+        if (tied && y.at == at) {
+            emit(r, y);
+            if (e) x[1] = ++i[1] < keep ? head(lane + 32, i[1]) : Cand{0, 0};
+            else x[0] = ++i[0] < keep ? head(lane, i[0]) : Cand{0, 0};
+        }
+    }
+    __syncwarp();
+}
+
+// The rest of request m: log-sums, then the best of the stretches' candidates.  s_key: room for `room` keys.  kFew: 64 lists at most.
+template <bool kFew>
+__device__ __forceinline__ void merge(const Args& a, int m, unsigned long long* s_key, int room) {
+    __shared__ double s_lse[kMaxBeams];
+    __shared__ float s_score[kMaxBeams];
+    __shared__ unsigned char s_ended[kMaxBeams];
+    __shared__ Cand s_best[kFew ? 1 : kWarps][kMaxKeep];
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const int lists = a.beams * a.chunks, total = lists * a.keep;
+    const unsigned long long* best = a.best + (size_t)m * total;
+    const bool staged = total <= room;
+    if (staged)
+        for (int i = t; i < total; i += kThreads) s_key[i] = best[i];
+    for (int b = warp; b < a.beams; b += kWarps) {
+        const float2* rec = a.sums + ((size_t)m * a.beams + b) * a.chunks;
+        const float2 one = lane < a.chunks ? rec[lane] : make_float2(-INFINITY, 0.f);
+        float mx = one.x;
+        for (int c = lane + 32; c < a.chunks; c += 32) mx = fmaxf(mx, rec[c].x);
+        mx = warp_max(mx);
+        float sum = one.x > -INFINITY ? one.y * exp2f((one.x - mx) * kLog2e) : 0.f;
+        for (int c = lane + 32; c < a.chunks; c += 32) {
+            const float2 r = rec[c];
+            if (r.x > -INFINITY) sum += r.y * exp2f((r.x - mx) * kLog2e);
+        }
+        sum = warp_sum(sum);
+        if (lane == 0) {
+            // log sum = k ln 2 + log of what is left, which lies in [1, 2): its 32-bit rounding is under 2^-24
+            int k = 0;
+            float left = sum;
+            if (sum >= 1.f && sum < INFINITY) {
+                k = (int)(__float_as_uint(sum) >> 23) - 127;
+                left = __uint_as_float((__float_as_uint(sum) & 0x7FFFFFu) | 0x3F800000u);
+            }
+            s_lse[b] = (double)mx + fma((double)k, 0.6931471805599453, (double)logf(left));
+            s_score[b] = a.score[m * a.beams + b];
+            s_ended[b] = a.ended ? a.ended[m * a.beams + b] : 0;
+        }
+    }
+    __syncthreads();
+    // Entry i of list l (a beam's stretch); an ended beam has one, its first stretch's.
+    auto head = [&](int l, int i) {
+        const int b = l / a.chunks;
+        Cand x{0, 0};
+        if (s_ended[b]) {
+            if (l == b * a.chunks && i == 0 && s_score[b] > -INFINITY) x = Cand{order64((double)s_score[b]), (uint32_t)b * a.vocab + a.eos};
+            return x;
+        }
+        const unsigned long long k = staged ? s_key[l * a.keep + i] : best[(size_t)l * a.keep + i];
+        if (k == 0) return x;
+        const double s = (double)s_score[b] + ((double)order32_value((uint32_t)(k >> 32)) - s_lse[b]);
+        if (s > -INFINITY) x = Cand{order64(s), (uint32_t)b * a.vocab + (0xFFFFFFFFu - (uint32_t)k)};
+        return x;
+    };
+    auto out = [&](int r, const Cand& x) {
+        const size_t o = (size_t)m * a.keep + r;
+        const bool some = x.score != 0;
+        const int b = some ? (int)(x.at / (uint32_t)a.vocab) : -1, v = some ? (int)(x.at - (uint32_t)b * a.vocab) : -1;
+        a.parent[o] = b;
+        a.token[o] = v;
+        a.score_out[o] = some ? (float)order64_value(x.score) : -INFINITY;
+        if (a.ended_out) a.ended_out[o] = some && (s_ended[b] || v == a.eos);
+    };
+    if (kFew || lists <= 64) {
+        if (warp == 0) tournament(lists, a.keep, lane, head, out);
+        return;
+    }
+    const int per = (lists + kWarps - 1) / kWarps, l0 = min(warp * per, lists);
+    tournament(min(per, lists - l0), a.keep, lane, [&](int l, int i) { return head(l0 + l, i); }, [&](int r, const Cand& x) { s_best[warp][r] = x; });
+    __syncthreads();
+    if (warp == 0) tournament(kWarps, a.keep, lane, [&](int l, int i) { return s_best[l][i]; }, out);
+}
+__global__ void __launch_bounds__(kThreads) merge_kernel(const Args a) {
+    __shared__ unsigned long long s_key[kStaged];
+    pdl_trigger();
+    pdl_wait();
+    merge<false>(a, blockIdx.x, s_key, kStaged);
+}
+
+// kFused: a request's blocks are a cluster, whose first goes on with the merge.
+template <bool kFused>
 __global__ void __launch_bounds__(kThreads, 4) chunk_kernel(const Args a) {
     __shared__ unsigned long long s_list[kWarps][kList], s_all[kWarps * kMaxKeep];
     __shared__ float s_f[kWarps], s_g[kWarps];
@@ -274,119 +386,26 @@ __global__ void __launch_bounds__(kThreads, 4) chunk_kernel(const Args a) {
         for (int w = 0; w < kWarps; ++w) whole += s_f[w];
         a.sums[rec] = make_float2(top, whole);
     }
+    if (kFused) {
+        cluster_sync_all();
+        const int m = row / (uint32_t)a.beams;
+        if (c == 0 && row == m * a.beams) merge<true>(a, m, s_list[0], kWarps * kList);
+    }
 }
 
-// The best of up to 64 sorted lists, two per lane, one after the other: head(l, i) is entry i of list l (score 0: none), emit(r, cand)
-// takes the r-th best, by the lane that holds it.  A round is three warp-wide integer reductions; only the winner's list moves on.
-template <typename Head, typename Emit>
-__device__ __forceinline__ void tournament(int lists, int keep, int lane, const Head& head, const Emit& emit) {
-    Cand x[2];
-    int i[2] = {0, 0};
-#pragma unroll
-    for (int e = 0; e < 2; ++e) x[e] = lane + 32 * e < lists ? head(lane + 32 * e, 0) : Cand{0, 0};
-    for (int r = 0; r < keep; ++r) {
-        const int e = before(x[1], x[0]);
-        const Cand y = e ? x[1] : x[0];
-        const uint32_t hi = (uint32_t)(y.score >> 32), lo = (uint32_t)y.score;
-        const uint32_t mhi = __reduce_max_sync(0xffffffffu, hi);
-        const uint32_t mlo = __reduce_max_sync(0xffffffffu, hi == mhi ? lo : 0u);
-        const bool tied = hi == mhi && lo == mlo;
-        const uint32_t at = __reduce_min_sync(0xffffffffu, tied ? y.at : 0xFFFFFFFFu);
-        if (mhi == 0 && mlo == 0) {
-            if (lane == 0)
-                for (; r < keep; ++r) emit(r, Cand{0, 0});
-            break;
-        }
-        if (tied && y.at == at) {
-            emit(r, y);
-            if (e) x[1] = ++i[1] < keep ? head(lane + 32, i[1]) : Cand{0, 0};
-            else x[0] = ++i[0] < keep ? head(lane, i[0]) : Cand{0, 0};
-        }
-    }
-    __syncwarp();
-}
-
-__global__ void __launch_bounds__(kThreads) merge_kernel(const Args a) {
-    __shared__ double s_lse[kMaxBeams];
-    __shared__ float s_score[kMaxBeams];
-    __shared__ unsigned char s_ended[kMaxBeams];
-    __shared__ unsigned long long s_key[kStaged];
-    __shared__ Cand s_best[kWarps][kMaxKeep];
-    const int m = blockIdx.x, t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    const int lists = a.beams * a.chunks, total = lists * a.keep;
-    const unsigned long long* best = a.best + (size_t)m * total;
-    pdl_trigger();
-    pdl_wait();
-    const bool staged = total <= kStaged;
-    if (staged)
-        for (int i = t; i < total; i += kThreads) s_key[i] = best[i];
-    for (int b = warp; b < a.beams; b += kWarps) {
-        const float2* rec = a.sums + ((size_t)m * a.beams + b) * a.chunks;
-        const float2 one = lane < a.chunks ? rec[lane] : make_float2(-INFINITY, 0.f);
-        float mx = one.x;
-        for (int c = lane + 32; c < a.chunks; c += 32) mx = fmaxf(mx, rec[c].x);
-        mx = warp_max(mx);
-        float sum = one.x > -INFINITY ? one.y * exp2f((one.x - mx) * kLog2e) : 0.f;
-        for (int c = lane + 32; c < a.chunks; c += 32) {
-            const float2 r = rec[c];
-            if (r.x > -INFINITY) sum += r.y * exp2f((r.x - mx) * kLog2e);
-        }
-        sum = warp_sum(sum);
-        if (lane == 0) {
-            // log sum = k ln 2 + log of what is left, which lies in [1, 2): its 32-bit rounding is under 2^-24
-            int k = 0;
-            float left = sum;
-            if (sum >= 1.f && sum < INFINITY) {
-                k = (int)(__float_as_uint(sum) >> 23) - 127;
-                left = __uint_as_float((__float_as_uint(sum) & 0x7FFFFFu) | 0x3F800000u);
-            }
-            s_lse[b] = (double)mx + fma((double)k, 0.6931471805599453, (double)logf(left));
-            s_score[b] = a.score[m * a.beams + b];
-            s_ended[b] = a.ended ? a.ended[m * a.beams + b] : 0;
-        }
-    }
-    __syncthreads();
-    // Entry i of list l (a beam's stretch); an ended beam has one, its first stretch's.
-    auto head = [&](int l, int i) {
-        const int b = l / a.chunks;
-        Cand x{0, 0};
-        if (s_ended[b]) {
-            if (l == b * a.chunks && i == 0 && s_score[b] > -INFINITY) x = Cand{order64((double)s_score[b]), (uint32_t)b * a.vocab + a.eos};
-            return x;
-        }
-        const unsigned long long k = staged ? s_key[l * a.keep + i] : best[(size_t)l * a.keep + i];
-        if (k == 0) return x;
-        const double s = (double)s_score[b] + ((double)order32_value((uint32_t)(k >> 32)) - s_lse[b]);
-        if (s > -INFINITY) x = Cand{order64(s), (uint32_t)b * a.vocab + (0xFFFFFFFFu - (uint32_t)k)};
-        return x;
-    };
-    auto out = [&](int r, const Cand& x) {
-        const size_t o = (size_t)m * a.keep + r;
-        const bool some = x.score != 0;
-        const int b = some ? (int)(x.at / (uint32_t)a.vocab) : -1, v = some ? (int)(x.at - (uint32_t)b * a.vocab) : -1;
-        a.parent[o] = b;
-        a.token[o] = v;
-        a.score_out[o] = some ? (float)order64_value(x.score) : -INFINITY;
-        if (a.ended_out) a.ended_out[o] = some && (s_ended[b] || v == a.eos);
-    };
-    if (lists <= 64) {
-        if (warp == 0) tournament(lists, a.keep, lane, head, out);
-        return;
-    }
-    const int per = (lists + kWarps - 1) / kWarps, l0 = min(warp * per, lists);
-    tournament(min(per, lists - l0), a.keep, lane, [&](int l, int i) { return head(l0 + l, i); }, [&](int r, const Cand& x) { s_best[warp][r] = x; });
-    __syncthreads();
-    if (warp == 0) tournament(kWarps, a.keep, lane, [&](int l, int i) { return s_best[l][i]; }, out);
-}
-
-// Stretches of a row: whole turns, four blocks per SM where that many are to be had.
-static void stretches(int vocab, int beams, long rows, int sms, Args* a) {
-    const int turns = (vocab + 3 + 3) / 4 / kTurn + 1;
-    long n = 4L * sms / rows;
+// Stretches of a row: whole turns, four blocks per SM where that many are to be had.  A few requests that a cluster each reads in two turns or fewer:
+// one launch.  On the device both take the same (1 x 4 beams of 32,768 tokens 8.0 us, in two launches 7.3), but a launch costs the caller 2 us: calls
+// in a row take 9 instead of 11.  skew: elements that rows may start behind a 16-byte boundary.
+constexpr int kFusedBlocks = 16, kFusedTurns = 2;
+static bool stretches(int vocab, int skew, int beams, long rows, int sms, Args* a) {
+    const int vectors = (vocab + skew + 3) / 4, turns = (vectors + kTurn - 1) / kTurn;
+    const bool fused = beams <= kFusedBlocks && kFusedBlocks * rows <= (long)sms * beams && (turns + kFusedBlocks / beams - 1) / (kFusedBlocks / beams) <= kFusedTurns;
+    long n = fused ? kFusedBlocks / beams : 4L * sms / rows;
     n = n > kMaxLists / beams ? kMaxLists / beams : n;
     n = n < 1 ? 1 : n > turns ? turns : n;
     a->chunk = (int)((turns + n - 1) / n) * kTurn;
-    a->chunks = ((vocab + 6) / 4 + a->chunk - 1) / a->chunk;
+    a->chunks = (vectors + a->chunk - 1) / a->chunk;
+    return fused;
 }
 static size_t round16(size_t n) { return (n + 15) & ~(size_t)15; }
 static size_t bytes_of(long records, int keep) {
@@ -416,7 +435,8 @@ extern "C" int bw_beam_select(int* parent_out, int* token_out, float* score_out,
     if (keep != beams && (score_out == score || (ended_or_null && ended_out_or_null == ended_or_null))) return cudaErrorInvalidValue;   // (other requests' are still read)
     const long rows = (long)M * beams;
     beam::Args a{};
-    beam::stretches(vocab, beams, rows, sm_count(current_device()), &a);
+    const int skew = (reinterpret_cast<uintptr_t>(logits) & 15) == 0 && row_stride % 4 == 0 ? 0 : 3;
+    const bool fused = beam::stretches(vocab, skew, beams, rows, sm_count(current_device()), &a);
     if (scratch_bytes < beam::bytes_of(rows * a.chunks, keep)) return cudaErrorInvalidValue;
     a.parent = parent_out; a.token = token_out; a.score_out = score_out; a.ended_out = ended_out_or_null;
     a.logits = logits; a.row_stride = row_stride; a.vocab = vocab; a.score = score; a.ended = ended_or_null;
@@ -425,7 +445,27 @@ extern "C" int bw_beam_select(int* parent_out, int* token_out, float* score_out,
     a.best = reinterpret_cast<unsigned long long*>(static_cast<unsigned char*>(scratch) + beam::round16((size_t)rows * a.chunks * sizeof(float2)));
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const dim3 grid((unsigned)a.chunks, (unsigned)rows);
-    cudaError_t e = launch_pdl(beam::chunk_kernel, grid, dim3(beam::kThreads), 0, st, a);
+    if (fused) {
+        static std::once_flag once[kMaxDevices];
+        std::call_once(once[current_device()], [] { cudaFuncSetAttribute(beam::chunk_kernel<true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1); });
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = grid;
+        cfg.blockDim = dim3(beam::kThreads);
+        cfg.stream = st;
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = grid.x;
+        attr[1].val.clusterDim.y = beams;
+        attr[1].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 2;
+        const cudaError_t e = cudaLaunchKernelEx(&cfg, beam::chunk_kernel<true>, a);
+        count_launch(1);
+        return e != cudaSuccess ? e : cudaPeekAtLastError();
+    }
+    cudaError_t e = launch_pdl(beam::chunk_kernel<false>, grid, dim3(beam::kThreads), 0, st, a);
     if (e == cudaSuccess) e = launch_pdl(beam::merge_kernel, dim3((unsigned)M), dim3(beam::kThreads), 0, st, a);
     count_launch(2);
     return e != cudaSuccess ? e : cudaPeekAtLastError();
