@@ -410,21 +410,26 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
                 const int odd = pc >> 2;
                 const uint32_t base = to + odd * kTcPanel + r0 * 128;
                 const uint32_t c0 = base + (((2 * (pc & 3) + odd) ^ (r0 & 7)) << 4), c1 = base + (((2 * (pc & 3) + 1 - odd) ^ (r0 & 7)) << 4);
+                uint4 raw[2][kRows];                               // (all on their way before the first is stored)
 #pragma unroll
                 for (int side = 0; side < 2; ++side)
 #pragma unroll
-                    for (int i = 0; i < kRows; ++i) {              // rows r0 + 16 i: the same low bits
-                        uint4 w, lo, hi;
-                        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+                    for (int i = 0; i < kRows; ++i)                // rows r0 + 16 i: the same low bits
+                        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(raw[side][i].x), "=r"(raw[side][i].y), "=r"(raw[side][i].z), "=r"(raw[side][i].w)
                                      : "r"(from + place + side * kSideOff + i * kRowOff));
-                        codes_f16(w.x, lo.x, lo.y);
-                        codes_f16(w.y, lo.z, lo.w);
-                        codes_f16(w.z, hi.x, hi.y);
-                        codes_f16(w.w, hi.z, hi.w);
-                        const uint4 first = odd ? hi : lo, second = odd ? lo : hi;
+#pragma unroll
+                for (int side = 0; side < 2; ++side)
+#pragma unroll
+                    for (int i = 0; i < kRows; ++i) {
+                        const uint4 w = raw[side][i];
+                        uint4 lo, hi;
+                        codes_f16(odd ? w.z : w.x, lo.x, lo.y);
+                        codes_f16(odd ? w.w : w.y, lo.z, lo.w);
+                        codes_f16(odd ? w.x : w.z, hi.x, hi.y);
+                        codes_f16(odd ? w.y : w.w, hi.z, hi.w);
                         const uint32_t at = side * 2 * kTcPanel + i * kRowOff;
-                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(c0 + at), "r"(first.x), "r"(first.y), "r"(first.z), "r"(first.w) : "memory");
-                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(c1 + at), "r"(second.x), "r"(second.y), "r"(second.z), "r"(second.w) : "memory");
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(c0 + at), "r"(lo.x), "r"(lo.y), "r"(lo.z), "r"(lo.w) : "memory");
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(c1 + at), "r"(hi.x), "r"(hi.y), "r"(hi.z), "r"(hi.w) : "memory");
                     }
                 raw_out = raw_out == Sh::kRaws - 1 ? 0 : raw_out + 1;
             }
