@@ -307,37 +307,40 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
         // that leaves may be asked for ahead of it.
         constexpr int kAhead = kCoded ? Sh::kRaws : kTall ? NS - 1 : NS - 2;
         static_assert(NS >= (kTall ? 2 : 3) && kAhead >= 1, "stages");
-        int xi = x_first, xo = x_first, it_in = 0, it_out = 0, st_in = 0, st_out = 0, raw_in = 0, raw_out = 0;
+        int x = x_first, it_in = 0, it_out = 0, st_in = 0, st_out = 0, raw_in = 0, raw_out = 0;
         uint32_t lap_in = 1, lap_out = 1;                          // parity of the stages' next release
-        Part in{}, out{};
-        bool in_more = next_part(xi, in), out_more = next_part(xo, out);
-        int in_tile = in.t0, out_tile = out.t0, ctx = 0, end = 0;
+        uint32_t opens = 0;                                        // of the tiles in flight, by number modulo 32: first of a part
+        bool more, opening = false;
+        int tile = 0, tile_end = 0, ctx = 0, end = 0;
         unsigned long long any = 0;
-        const unsigned char *kp = nullptr, *vp = nullptr;          // this thread's piece of the part's first row
         size_t row0 = 0;
-        auto open_part = [&]() {                                   // what the sequence's rows see
-            const int nodes = in.nodes;
-            ctx = min(in.first, a.c.max_seq);
-            end = (int)min((long)in.first + nodes, (long)a.c.max_seq);
+        auto open_part = [&]() {                                   // the next part and what its sequence's rows see
+            Part p{};
+            more = next_part(x, p);
+            if (!more) return;
+            opening = true;
+            tile = p.t0;
+            tile_end = p.t1;
+            ctx = min(p.first, a.c.max_seq);
+            end = (int)min((long)p.first + p.nodes, (long)a.c.max_seq);
             any = 0;
-            if (in.t1 * kTcKeys > ctx) {
-                const unsigned long long mine = (lane < nodes ? mask_of(a, in.m, lane, nodes) : 0) | (lane + 32 < nodes ? mask_of(a, in.m, lane + 32, nodes) : 0);
+            if (tile_end * kTcKeys > ctx) {
+                const unsigned long long mine = (lane < p.nodes ? mask_of(a, p.m, lane, p.nodes) : 0) | (lane + 32 < p.nodes ? mask_of(a, p.m, lane + 32, p.nodes) : 0);
                 any = (unsigned long long)__reduce_or_sync(0xffffffffu, (uint32_t)(mine >> 32)) << 32 | __reduce_or_sync(0xffffffffu, (uint32_t)mine);
             }
-            row0 = a.c.row(in.m, in.head, 0);
-            kp = a.c.k + (row0 + r0) * kRowBytes + pc * 16;
-            vp = a.c.v + (row0 + r0) * kRowBytes + pc * 16;
+            row0 = a.c.row(p.m, p.head, 0);
         };
+        open_part();
         // where this thread's piece of row r0 goes; the others are kStep rows on (binary16: swizzled, kStep = 8 keeps a row's low bits)
         const uint32_t place = kCoded ? r0 * kHd + pc * 16 : (pc >> 3) * kTcPanel + r0 * 128 + (((pc & 7) ^ (r0 & 7)) << 4);
         constexpr uint32_t kSideOff = kCoded ? kTcKeys * kHd : 2 * kTcPanel, kRowOff = kStep * 128;
         auto issue = [&]() {                                       // the next tile on its way
-            if (in_more) {
-                if (in_tile == in.t0) open_part();
-                const int p0 = in_tile * kTcKeys;
+            if (more) {
+                const int p0 = tile * kTcKeys;
                 if (!kCoded) wait(Sh::kEmptyKV + st_in, lap_in);
                 const uint32_t to = kCoded ? sraw + raw_in * kTcRaw : skv + st_in * kTcStage;
-                const unsigned char *k = kp + (size_t)p0 * kRowBytes, *v = vp + (size_t)p0 * kRowBytes;
+                const size_t first_row = (row0 + p0 + r0) * kRowBytes + pc * 16;
+                const unsigned char *k = a.c.k + first_row, *v = a.c.v + first_row;
                 if (p0 + kTcKeys <= ctx) {
 #pragma unroll
                     for (int i = 0; i < kRows; ++i) {
@@ -354,8 +357,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
 #pragma unroll 1
                     for (int i = 0; i < kRows; ++i) {
                         const bool in_seq = there(p0 + r0 + kStep * i);
-                        lm::cp_async16z(to + place + i * kRowOff, in_seq ? k + i * kStep * kRowBytes : kp, in_seq);
-                        lm::cp_async16z(to + place + kSideOff + i * kRowOff, in_seq ? v + i * kStep * kRowBytes : vp, in_seq);
+                        lm::cp_async16z(to + place + i * kRowOff, in_seq ? k + i * kStep * kRowBytes : a.c.k, in_seq);
+                        lm::cp_async16z(to + place + kSideOff + i * kRowOff, in_seq ? v + i * kStep * kRowBytes : a.c.v, in_seq);
                     }
                     if (kCoded && (warp & 1) == 0) {
 #pragma unroll 1
@@ -367,6 +370,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
                         }
                     }
                 }
+                opens = (opens & ~(1u << (it_in & 31))) | (opening ? 1u : 0u) << (it_in & 31);
+                opening = false;
                 ++it_in;
                 if (kCoded) {
                     raw_in = raw_in == Sh::kRaws - 1 ? 0 : raw_in + 1;
@@ -374,17 +379,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
                     st_in = 0;
                     lap_in ^= 1;
                 }
-                if (++in_tile == in.t1) {
-                    in_more = next_part(xi, in);
-                    in_tile = in.t0;
-                }
+                if (++tile == tile_end) open_part();
             }
             lm::cp_async_commit();
         };
         float vref = 0.f;                                          // warp 10: the largest value scale of the part so far, a power of two
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) issue();
-        while (out_more && !*abort_flag) {
+        while ((more || it_out < it_in) && !*abort_flag) {
             const int st = st_out;
             lm::cp_async_wait<kAhead - 1>();
             if (kCoded) {
@@ -395,7 +397,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
                     const float* fs = reinterpret_cast<const float*>(smem + (from - bar0) + 2 * kTcKeys * kHd) + (warp - 8) * 32 + lane;
                     float s0 = fs[0], s1 = fs[32];
                     if (warp == 10) {
-                        if (out_tile == out.t0) vref = __uint_as_float(2u << 23);
+                        if (opens >> (it_out & 31) & 1) vref = __uint_as_float(2u << 23);
                         const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fabsf(s0), fabsf(s1)))));
                         if (top > vref) vref = __uint_as_float(min((__float_as_uint(top) + 0x7FFFFFu) & 0x7F800000u, 252u << 23));
                         const float inv = __uint_as_float((254u << 23) - __float_as_uint(vref));
@@ -439,10 +441,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
             if (++st_out == NS) {
                 st_out = 0;
                 lap_out ^= 1;
-            }
-            if (++out_tile == out.t1) {
-                out_more = next_part(xo, out);
-                out_tile = out.t0;
             }
             issue();
         }
