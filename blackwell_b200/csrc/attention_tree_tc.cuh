@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
     using Sh = TcShape<kTall, kCoded, kSplit>;
     constexpr int NS = Sh::kStages;
     extern __shared__ unsigned char smem_raw[];
-    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    unsigned char* smem = smem_raw + (-smem_u32(smem_raw) & 1023);   // (not rounded as an address: loads stay loads of shared memory)
     unsigned char* q_area = smem + Sh::kHead + Sh::kScales;       // (a multiple of 1,024 from the base)
     static_assert((Sh::kHead + Sh::kScales) % 1024 == 0, "swizzled tiles start at 1,024 bytes");
     const uint32_t sq = smem_u32(q_area), skv = sq + Sh::kQ, sraw = skv + NS * kTcStage, bar0 = smem_u32(smem), flag = bar0 + 516;
