@@ -560,28 +560,29 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
                 if (kCoded) wait(Sh::kFullKV + st, lap);                         // (long full: the scales)
                 tc::tc_fence_after();
                 if (active) {
-                    uint32_t r[64];
-                    tc::tmem_ld32(at, r);
-                    tc::tmem_ld32(at + 32, r + 32);
                     if (kSplit && k > 0 && k % kFlush == 0) {                    // O so far to the sum; the next product starts afresh
                         wait(Sh::kDoneO + 2 * w + (b ^ 1), ((kk - 1) >> 1) & 1);
                         tc::tc_fence_after();
                         const float f = has_kept ? lm::exp2_fast(m_kept - m) * (v_kept * __uint_as_float((254u << 23) - __float_as_uint(vref))) : 0.f;
 #pragma unroll 1
-                        for (int d = 0; d < kHd; d += 16) {
-                            uint32_t o[16];
-                            float old[16];
-                            tc::tmem_ld16(lanes + 128 + d, o);
+                        for (int d = 0; d < kHd; d += 64) {                      // (half of it on its way at once: the latency of L2)
+                            uint32_t o[64];
+                            float old[64];
+                            tc::tmem_ld32(lanes + 128 + d, o);
+                            tc::tmem_ld32(lanes + 160 + d, o + 32);
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) old[i] = has_kept ? kept[(d + i) * 128] : 0.f;
+                            for (int i = 0; i < 64; ++i) old[i] = has_kept ? kept[(d + i) * 128] : 0.f;
                             tc::tmem_wait_ld();
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) kept[(d + i) * 128] = fmaf(old[i], f, __uint_as_float(o[i]));
+                            for (int i = 0; i < 64; ++i) kept[(d + i) * 128] = fmaf(old[i], f, __uint_as_float(o[i]));
                         }
                         has_kept = true;
                         m_kept = m;
                         v_kept = vref;
                     }
+                    uint32_t r[64];
+                    tc::tmem_ld32(at, r);
+                    tc::tmem_ld32(at + 32, r + 32);
                     tc::tmem_wait_ld();
                     const float* ks = s_scale + st * 2 * kTcKeys;
                     const float* vs = ks + kTcKeys;
@@ -697,34 +698,41 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
                 float* rec = whole ? nullptr : a.part + (size_t)p.slot * a.rec_rows * kPart + (kTall ? w * 128 : 0) + rt;
                 A* out = static_cast<A*>(a.out) + at_row;
                 const float* kept1 = kSplit ? a.kept + ((size_t)c * 2 + (w ^ 1)) * kHd * 128 + rt : nullptr;
+                constexpr int kCols = kTall && kSplit ? 64 : 16;              // columns on their way at once
 #pragma unroll 1
-                for (int d = kTall ? 0 : w * 64; d < (kTall ? kHd : w * 64 + 64); d += 16) {
-                    uint32_t o[16], q[16];
-                    tc::tmem_ld16(lanes + 128 + d, o);
-                    if (!kTall) tc::tmem_ld16((lanes ^ 256) + 128 + d, q);
-                    float old[16], old1[16];
+                for (int d = kTall ? 0 : w * 64; d < (kTall ? kHd : w * 64 + 64); d += kCols) {
+                    uint32_t o[kCols], q[kTall ? 16 : kCols];
+                    float old[kSplit ? kCols : 1], old1[kSplit && !kTall ? kCols : 1];
+#pragma unroll
+                    for (int i = 0; i < kCols; i += 16) {
+                        tc::tmem_ld16(lanes + 128 + d + i, reinterpret_cast<uint32_t(&)[16]>(o[i]));
+                        if (!kTall) tc::tmem_ld16((lanes ^ 256) + 128 + d + i, reinterpret_cast<uint32_t(&)[16]>(q[kTall ? 0 : i]));
+                    }
                     if (kSplit) {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            old[i] = f0 != 0.f ? kept[(d + i) * 128] : 0.f;
-                            old1[i] = !kTall && f1 != 0.f ? kept1[(d + i) * 128] : 0.f;
+                        for (int i = 0; i < kCols; ++i) {
+                            old[kSplit ? i : 0] = f0 != 0.f ? kept[(d + i) * 128] : 0.f;
+                            if (!kTall) old1[kSplit && !kTall ? i : 0] = f1 != 0.f ? kept1[(d + i) * 128] : 0.f;
                         }
                     }
                     tc::tmem_wait_ld();
-                    float v[16];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        v[i] = jobs > 0 ? __uint_as_float(o[i]) * c0 : 0.f;
-                        if (!kTall && other) v[i] = fmaf(__uint_as_float(q[i]), c1, v[i]);
-                        if (kSplit) v[i] = fmaf(old[i], f0, v[i]);
-                        if (kSplit && !kTall) v[i] = fmaf(old1[i], f1, v[i]);
-                    }
-                    if (mine) {
-                        if (whole) {
-                            store_o16(out + d, v);
-                        } else {
+                    for (int i0 = 0; i0 < kCols; i0 += 16) {
+                        float v[16];
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) rec[(size_t)(d + i) * a.rec_rows] = v[i];
+                        for (int i = 0; i < 16; ++i) {
+                            v[i] = jobs > 0 ? __uint_as_float(o[i0 + i]) * c0 : 0.f;
+                            if (!kTall && other) v[i] = fmaf(__uint_as_float(q[kTall ? 0 : i0 + i]), c1, v[i]);
+                            if (kSplit) v[i] = fmaf(old[kSplit ? i0 + i : 0], f0, v[i]);
+                            if (kSplit && !kTall) v[i] = fmaf(old1[kSplit && !kTall ? i0 + i : 0], f1, v[i]);
+                        }
+                        if (mine) {
+                            if (whole) {
+                                store_o16(out + d + i0, v);
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) rec[(size_t)(d + i0 + i) * a.rec_rows] = v[i];
+                            }
                         }
                     }
                 }
