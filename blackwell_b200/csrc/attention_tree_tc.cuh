@@ -9,11 +9,17 @@
 //   S = Q K^T    two S buffers of 64 columns per stream, the next scores are on their way while the softmax has these
 //   O += P V     P over the scores' columns as the f16 A operand, V from shared memory as it lies there ([position][column])
 // fp32 activations: Q and P as f16 high parts and remainders, multiplied one after the other.  The accumulator's sums are cut, not rounded, at
-// 24 bits, which adds up over a long context: there O is added to a sum in the scratch memory (L2) every eight tiles and starts afresh.
+// 24 bits, which adds up: so the remainders of a score come first, and O is added to a sum in the scratch memory (L2) every four tiles and
+// starts afresh (64 nodes over 5,279 positions: error 1.1e-6 of the result, as that of 32-bit sums; every eight tiles 2.3e-6 and a tenth faster).
 // Scales and the moving maximum as in attention_tree.cuh; a warp brings its rows of O to a new maximum by itself.
 // Work is shared out in tiles of 64 positions: all sequences' tiles, heads and row groups in one line, an equal stretch of it per block; what
 // a block has of a head's context that it does not have whole goes to a record that the merge kernel joins.
 // All waits are bounded; a wait that gives up raises an abort flag.
+// Measured (8 trees of 64 nodes over 2,000 to 4,096 positions, 32 / 8 heads, 8 bits): bf16 59 us, 0.42 PFLOP/s, fp32 93.  Of a block's 88,000 cycles a
+// tile takes 2,600, the softmax of a stream that long from one tile to the next (scores out of tensor memory 250, scales and maximum 600, exponentials 1,200;
+// the units' own rates would allow 1,100, the rest is latency of one warp per scheduler and stream); the start 4,000, and each of two parts 12,000 for the
+// queries' place, the first scores and the record, whose 128 KB an SM stores in 5,000.  The merge takes 5 us.  Tried and not kept: maximum and exponentials in
+// one pass over the scores (slower), streams held half a tile apart (1 to 3 %).
 #pragma once
 #include "attention_tree.cuh"
 #include "gemm_w4a8_tc.cuh"
@@ -24,7 +30,7 @@ namespace tree {
 constexpr int kTcKeys = 64, kTcPanel = kTcKeys * 128, kTcThreads = 512;   // positions of a tile, bytes of 64 x 64 f16
 constexpr int kTcStage = 4 * kTcPanel;                                    // K and V of a tile
 constexpr int kTcRaw = 2 * kTcKeys * kHd + 2 * kTcKeys * 4;               // codes and scales of a tile
-constexpr int kFlush = 8;
+constexpr int kFlush = 4;
 constexpr int kPlanned = 448;                                              // sequences whose work is laid out in a line
 
 template <bool kTall, bool kCoded, bool kSplit>
@@ -248,13 +254,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
                     if (elected) {
                         const uint32_t d = acc + b * 64, kt = skv + st_s * kTcStage;
 #pragma unroll
-                        for (int part = 0; part < (kSplit ? 2 : 1); ++part)
+                        for (int part = kSplit ? 1 : 0; part >= 0; --part)   // remainders first, while the sum is small
 #pragma unroll
                             for (int pan = 0; pan < 2; ++pan)
 #pragma unroll
                                 for (int e = 0; e < 4; ++e)   // 16 dimensions = 32 bytes further inside the swizzle atom
                                     tc::tc_mma_bf16(d, tc::flash_desc(q + part * Sh::kQTile + pan * 2 * kTcPanel, 16, 1024) + 2 * e,
-                                                    tc::flash_desc(kt + pan * kTcPanel, 16, 1024) + 2 * e, id_s, part + pan + e > 0 ? 1u : 0u);
+                                                    tc::flash_desc(kt + pan * kTcPanel, 16, 1024) + 2 * e, id_s, part < (kSplit ? 1 : 0) || pan + e > 0 ? 1u : 0u);
                         tc::tc_commit(bar(Sh::kFullS + 2 * w + b));
                     }
                     __syncwarp();
