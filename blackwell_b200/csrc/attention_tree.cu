@@ -14,17 +14,26 @@ static int tiles_of_eight(int rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
 constexpr int kFewRows = 32;            // query rows of a head that the mma.sync kernel takes
 constexpr int kMaxCluster = 8;
 constexpr int kCut = 512;               // positions of a warp, where contexts are long: their lengths differ, and the last block is waited for
-// Blocks that share a context of a (sequence, head, row tile), a multiple of eight where more than a cluster.  Few contexts: one wave of two
-// blocks per SM, but two tiles of 16 positions for each warp or more.  Many: kCut positions for a warp at most, as far as the records allow
+// Blocks that share a context of a (sequence, head, row tile), a multiple of eight where more than a cluster.
+// Few contexts: one wave of two blocks per SM, by the tiles of 16 positions that a warp is left with (0.45 us for eight columns), against 0.9 us for a
+// cluster's merge; clusters of other than 2, 4 or 8 blocks leave places of the chip empty and take longer to be placed.  Still more shares of a
+// long context, joined by a second launch, where a wave has room for them.  Many contexts: kCut positions for a warp at most, as far as the records allow
 // (rows of few heads: any number, scratch_bytes; many rows: two waves of blocks), and one or two more where that fills the last wave.
-// Measured (us, 32 / 8 heads, 8 bits, fp32): 32 x 4,096 to 8,192 positions in 1 to 8 shares 75 74 75 76 79 85 95, 20 x 3,000 to 6,000 48 47 41 44
-// 43 48 54, 8 x 2,000 to 4,000 24 20 17 15 22 22 21.  Clusters of 16 need 16 free SMs next to each other: 1 x 2,048 positions with 64 rows 27 us,
-// as two clusters of 8 and a merge 20.
-static int choose_splits(long pairs, int ctx, int slots, int warps, bool few) {
-    long n = slots / pairs;
-    const long most = ctx / (32 * warps), least = (ctx + (long)kCut * warps - 1) / (kCut * warps);
-    if (n > most) n = most;
-    if (n > kMaxCluster) n = n / kMaxCluster * kMaxCluster;
+// Measured (us, 32 / 8 heads, fp32; in 1 2 3 4 5 6 8 shares): 1 x 100 positions of 8 bits 3.9 5.1 5.3 5.7 5.9 6.0 6.1, 1 x 500 6.1 5.9 6.0 5.5 5.6 5.7 5.7, 1 x 2,048
+// 13.7 10.0 8.8 7.7 7.6 7.3 6.7, 8 x 4,000 24 20 17 15 22 22 21, 20 x 6,000 48 47 41 44 43 48 54, 32 x 8,192 75 74 75 76 79 85 95; 4 trees of 8 nodes,
+// 1,000 positions of 16 bits, 28 / 4 heads, 25.6 20.4 18.4 16.6 15.7 15.9 13.9.  Clusters of 16 need 16 free SMs next to each other: 1 x 2,048 positions
+// with 64 rows 27 us, as two clusters of 8 and a merge 20.
+static int choose_splits(long pairs, int ctx, int slots, int warps, int nt, bool few) {
+    const long tiles = (ctx + kTile - 1) / kTile, least = (ctx + (long)kCut * warps - 1) / (kCut * warps);
+    auto whole = [](long k) { return (k & (k - 1)) == 0; };
+    auto cost = [&](long k) { return (tiles + k * warps - 1) / (k * warps) * nt + (k == 1 ? 0 : whole(k) ? 2 : 3); };
+    long n = 1;
+    for (long k = 2; k <= kMaxCluster; ++k)
+        if (pairs * k <= (whole(k) ? slots : slots * 17 / 20) && cost(k) < cost(n)) n = k;
+    if (n == kMaxCluster) {
+        const long room = slots / pairs, most = ctx / (32 * warps), more = (room < most ? room : most) / kMaxCluster * kMaxCluster;
+        if (more > n) n = more;
+    }
     if (n < least && least > kMaxCluster) {
         n = (least + kMaxCluster - 1) / kMaxCluster * kMaxCluster;
         const long records = 2L * slots / pairs;
@@ -35,7 +44,7 @@ static int choose_splits(long pairs, int ctx, int slots, int warps, bool few) {
         for (long k = least + 1; k <= least + 2 && k <= kMaxCluster && k * (kCut / 4) * warps <= ctx; ++k)
             if (20 * waves(k) * n < 19 * waves(n) * k) n = k;
     }
-    return n < 1 ? 1 : (int)n;
+    return (int)n;
 }
 
 template <int NT, bool kCoded, typename A, bool kPair = false>
@@ -48,7 +57,7 @@ static cudaError_t launch(Args a, int ctx, void* scratch, size_t scratch_bytes, 
         cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem);
         cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     });
-    a.nsplit = choose_splits((long)a.M * a.c.heads * a.tiles, ctx, 2 * sm_count(dev), Sh::kWarps, a.rows <= kFewRows);
+    a.nsplit = choose_splits((long)a.M * a.c.heads * a.tiles, ctx, 2 * sm_count(dev), Sh::kWarps, NT, a.rows <= kFewRows);
     a.cluster = a.nsplit <= kMaxCluster ? a.nsplit : kMaxCluster;
     const int groups = a.nsplit / a.cluster;
     if (groups > 1) {

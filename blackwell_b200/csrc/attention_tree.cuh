@@ -20,7 +20,7 @@
 // of it the chain of a launch, the position, the first tile from memory and the merge inside the cluster.  What it took: the scales with the tiles by
 // cp.async (loaded to registers a tile ahead: 92 us), queries brought to their place once per block (by every warp: + 2,000 cycles), and the remainders in
 // the idle columns (8 us at 32 sequences).  Trees of up to 32 rows a head are bound by mma.sync, whose rate is a sixth of
-// tcgen05's: 4 of 8 nodes over 1,000 positions, 28 / 4 heads, binary16, 15.6 us.  Tried and not kept: an equal stretch of all contexts per block with records
+// tcgen05's: 4 of 8 nodes over 1,000 positions, 28 / 4 heads, binary16, 13.9 us.  Tried and not kept: an equal stretch of all contexts per block with records
 // and a merge (10 us more below 16,000 positions, as much beyond).
 #pragma once
 #include <float.h>
