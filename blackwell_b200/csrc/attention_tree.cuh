@@ -47,11 +47,11 @@ struct Args {
     const unsigned long long* mask;     // [M * T] or NULL: node j <= i
     int nq, M, T, group, rows, tiles;   // rows = T * group query rows per kv head, in `tiles` blocks of 8 * NT
     int nsplit, cluster;                // blocks that share a context; those that join as a cluster
-    float* part;                        // [M][heads][rows][nsplit / cluster][kPart] where there are several; tcgen05 kernel: [2 * blocks][rec_rows][kPart]
+    float* part;                        // [M][heads][rows][nsplit / cluster][kPart] where there are several; tcgen05 kernel: [2 * blocks][kPart / 4][rec_rows][4]
     // tcgen05 kernel
     int flat, blocks, pairs, groups, group_rows, rec_rows;   // work in a line; heads and row groups of 128 or 256 rows in all
     int* cum;                           // tiles before each sequence; from kPlanned on, [blocks + 1], where each block's stretch starts
-    float* kept;                        // fp32: [blocks][2][128][128]
+    float* kept;                        // fp32: [blocks][2][32][128][4]
     int* status;
 };
 

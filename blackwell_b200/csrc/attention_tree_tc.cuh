@@ -456,8 +456,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
         // ---- softmax, a thread per row of the stream's accumulator
         const int w = warp >> 2, rt = t & 127;
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16) + w * 256;
-        // fp32: O of the tiles before, [column][row], relative to the maximum and scale that it had then
-        float* kept = kSplit ? a.kept + ((size_t)c * 2 + w) * kHd * 128 + rt : nullptr;
+        // fp32: O of the tiles before, [four columns][row], relative to the maximum and scale that it had then
+        float4* kept = kSplit ? reinterpret_cast<float4*>(a.kept) + ((size_t)c * 2 + w) * (kHd / 4) * 128 + rt : nullptr;
         int x = x_first, st = 0, kb = 0, nth = 0;
         uint32_t lap = 0;
         Part p;
@@ -573,14 +573,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
 #pragma unroll 1
                         for (int d = 0; d < kHd; d += 64) {                      // (half of it on its way at once: the latency of L2)
                             uint32_t o[64];
-                            float old[64];
+                            float4 old[16];
                             tc::tmem_ld32(lanes + 128 + d, o);
                             tc::tmem_ld32(lanes + 160 + d, o + 32);
 #pragma unroll
-                            for (int i = 0; i < 64; ++i) old[i] = has_kept ? kept[(d + i) * 128] : 0.f;
+                            for (int i = 0; i < 16; ++i) old[i] = has_kept ? kept[(d / 4 + i) * 128] : make_float4(0.f, 0.f, 0.f, 0.f);
                             tc::tmem_wait_ld();
 #pragma unroll
-                            for (int i = 0; i < 64; ++i) kept[(d + i) * 128] = fmaf(old[i], f, __uint_as_float(o[i]));
+                            for (int i = 0; i < 16; ++i)
+                                kept[(d / 4 + i) * 128] =
+                                    make_float4(fmaf(old[i].x, f, __uint_as_float(o[4 * i])), fmaf(old[i].y, f, __uint_as_float(o[4 * i + 1])),
+                                                fmaf(old[i].z, f, __uint_as_float(o[4 * i + 2])), fmaf(old[i].w, f, __uint_as_float(o[4 * i + 3])));
                         }
                         has_kept = true;
                         m_kept = m;
@@ -700,15 +703,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
                 const bool whole = p.slot < 0;
                 const float inv = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;   // (a row that sees nothing: 0)
                 c0 *= inv; c1 *= inv; f0 *= inv; f1 *= inv;
-                // A record is [column][row], then the rows' maxima and sums: a warp stores 32 rows of a column.
-                float* rec = whole ? nullptr : a.part + (size_t)p.slot * a.rec_rows * kPart + (kTall ? w * 128 : 0) + rt;
+                // A record is [four columns][row], then the rows' maxima and sums: a warp stores 512 bytes at once.
+                float4* rec = whole ? nullptr : reinterpret_cast<float4*>(a.part + (size_t)p.slot * a.rec_rows * kPart) + (kTall ? w * 128 : 0) + rt;
                 A* out = static_cast<A*>(a.out) + at_row;
-                const float* kept1 = kSplit ? a.kept + ((size_t)c * 2 + (w ^ 1)) * kHd * 128 + rt : nullptr;
+                const float4* kept1 = kSplit ? reinterpret_cast<const float4*>(a.kept) + ((size_t)c * 2 + (w ^ 1)) * (kHd / 4) * 128 + rt : nullptr;
                 constexpr int kCols = kTall && kSplit ? 64 : 16;              // columns on their way at once
 #pragma unroll 1
                 for (int d = kTall ? 0 : w * 64; d < (kTall ? kHd : w * 64 + 64); d += kCols) {
                     uint32_t o[kCols], q[kTall ? 16 : kCols];
-                    float old[kSplit ? kCols : 1], old1[kSplit && !kTall ? kCols : 1];
+                    float4 old[kSplit ? kCols / 4 : 1], old1[kSplit && !kTall ? kCols / 4 : 1];
 #pragma unroll
                     for (int i = 0; i < kCols; i += 16) {
                         tc::tmem_ld16(lanes + 128 + d + i, reinterpret_cast<uint32_t(&)[16]>(o[i]));
@@ -716,9 +719,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
                     }
                     if (kSplit) {
 #pragma unroll
-                        for (int i = 0; i < kCols; ++i) {
-                            old[kSplit ? i : 0] = f0 != 0.f ? kept[(d + i) * 128] : 0.f;
-                            if (!kTall) old1[kSplit && !kTall ? i : 0] = f1 != 0.f ? kept1[(d + i) * 128] : 0.f;
+                        for (int i = 0; i < kCols / 4; ++i) {
+                            old[kSplit ? i : 0] = f0 != 0.f ? kept[(d / 4 + i) * 128] : make_float4(0.f, 0.f, 0.f, 0.f);
+                            if (!kTall) old1[kSplit && !kTall ? i : 0] = f1 != 0.f ? kept1[(d / 4 + i) * 128] : make_float4(0.f, 0.f, 0.f, 0.f);
                         }
                     }
                     tc::tmem_wait_ld();
@@ -729,22 +732,30 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
                         for (int i = 0; i < 16; ++i) {
                             v[i] = jobs > 0 ? __uint_as_float(o[i0 + i]) * c0 : 0.f;
                             if (!kTall && other) v[i] = fmaf(__uint_as_float(q[kTall ? 0 : i0 + i]), c1, v[i]);
-                            if (kSplit) v[i] = fmaf(old[kSplit ? i0 + i : 0], f0, v[i]);
-                            if (kSplit && !kTall) v[i] = fmaf(old1[kSplit && !kTall ? i0 + i : 0], f1, v[i]);
+                        }
+                        if (kSplit) {
+#pragma unroll
+                            for (int i = 0; i < 16; i += 4) {
+                                const float4 x = old[kSplit ? (i0 + i) / 4 : 0], y = old1[kSplit && !kTall ? (i0 + i) / 4 : 0];
+                                v[i] = fmaf(x.x, f0, v[i]); v[i + 1] = fmaf(x.y, f0, v[i + 1]); v[i + 2] = fmaf(x.z, f0, v[i + 2]); v[i + 3] = fmaf(x.w, f0, v[i + 3]);
+                                if (!kTall) {
+                                    v[i] = fmaf(y.x, f1, v[i]); v[i + 1] = fmaf(y.y, f1, v[i + 1]); v[i + 2] = fmaf(y.z, f1, v[i + 2]); v[i + 3] = fmaf(y.w, f1, v[i + 3]);
+                                }
+                            }
                         }
                         if (mine) {
                             if (whole) {
                                 store_o16(out + d + i0, v);
                             } else {
 #pragma unroll
-                                for (int i = 0; i < 16; ++i) rec[(size_t)(d + i0 + i) * a.rec_rows] = v[i];
+                                for (int i = 0; i < 16; i += 4)
+                                    rec[(size_t)((d + i0 + i) / 4) * a.rec_rows] = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
                             }
                         }
                     }
                 }
                 if (!whole && mine && (kTall || w == 0)) {
-                    rec[(size_t)kHd * a.rec_rows] = top;
-                    rec[(size_t)(kHd + 1) * a.rec_rows] = l;
+                    *reinterpret_cast<float2*>(rec + (size_t)(kHd / 4) * a.rec_rows) = make_float2(top, l);
                 }
             }
             if (!kTall) mbar_arrive(bar(Sh::kTaken));
@@ -784,8 +795,8 @@ __global__ void __launch_bounds__(256) attend_tc_merge_kernel(const Args a) {
     };
     const int b0 = block_of(x0), b1 = block_of(x1 - 1);
     if (b0 == b1) return;                                          // one block had it whole
-    const size_t record = (size_t)a.rec_rows * kPart;
-    const float* rec = a.part + row - g * a.group_rows;
+    const size_t record = (size_t)a.rec_rows * (kPart / 4);
+    const float4* rec = reinterpret_cast<const float4*>(a.part) + row - g * a.group_rows;
     const size_t late = starts[b0] < x0 ? record : 0;              // (the first block may have other work before)
     float top = -FLT_MAX, sum = 0.f, acc[8];
 #pragma unroll
@@ -796,11 +807,15 @@ __global__ void __launch_bounds__(256) attend_tc_merge_kernel(const Args a) {
         for (int j = 0; j < 4; ++j) {
             const int c = min(b + j, b1);
             const bool there = b + j <= b1 && starts[c] < starts[c + 1];
-            const float* at = rec + 2 * c * record + (c == b0 ? late : 0);
-            mt[j] = there ? at[(size_t)kHd * a.rec_rows] : -FLT_MAX;
-            lt[j] = there ? at[(size_t)(kHd + 1) * a.rec_rows] : 0.f;
+            const float4* at = rec + 2 * c * record + (c == b0 ? late : 0);
+            const float2 ml = there ? *reinterpret_cast<const float2*>(at + (size_t)(kHd / 4) * a.rec_rows) : make_float2(-FLT_MAX, 0.f);
+            mt[j] = ml.x;
+            lt[j] = ml.y;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[j][i] = there ? at[(size_t)(c0 + warp * 8 + i) * a.rec_rows] : 0.f;
+            for (int i = 0; i < 8; i += 4) {
+                const float4 x = there ? at[(size_t)((c0 + warp * 8 + i) / 4) * a.rec_rows] : make_float4(0.f, 0.f, 0.f, 0.f);
+                v[j][i] = x.x; v[j][i + 1] = x.y; v[j][i + 2] = x.z; v[j][i + 3] = x.w;
+            }
         }
         const float to = fmaxf(top, fmaxf(fmaxf(mt[0], mt[1]), fmaxf(mt[2], mt[3]))), f = lm::exp2_fast(top - to);
         top = to;
