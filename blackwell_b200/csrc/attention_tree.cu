@@ -29,7 +29,7 @@ static int choose_splits(long pairs, int ctx, int slots, int warps, int nt, bool
     auto cost = [&](long k) { return (tiles + k * warps - 1) / (k * warps) * nt + (k == 1 ? 0 : whole(k) ? 2 : 3); };
     long n = 1;
     for (long k = 2; k <= kMaxCluster; ++k)
-        if (pairs * k <= (whole(k) ? slots : slots * 17 / 20) && cost(k) < cost(n)) n = k;
+        if (pairs * k <= (whole(k) || nt > 1 ? slots : slots * 17 / 20) && cost(k) < cost(n)) n = k;
     if (n == kMaxCluster) {
         const long room = slots / pairs, most = ctx / (32 * warps), more = (room < most ? room : most) / kMaxCluster * kMaxCluster;
         if (more > n) n = more;
@@ -113,14 +113,14 @@ static cudaError_t launch_tc_rows(const Args& a, cudaStream_t st) {
 }
 
 // Which kernel.  The tcgen05 kernel takes some 20 us before it pays (queries into shared memory, the pipeline's start, records and their merge); a
-// tile of the mma.sync kernel (32 rows, 16 positions) takes a block 0.4 us.  So: by the tiles that an SM gets, and not for one or two row
-// tiles, which leave the 128 lanes of an accumulator half empty, unless there is much of it.  Measured (us, mma.sync / tcgen05; 32 / 8 heads, fp32,
-// 8 bits): 64 nodes, 8 x 2,048 positions 152 / 65, 4 x 1,000 40 / 34, 4 x 300 21 / 30; 24 nodes, 8 x 2,048 55 / 42, 4 x 1,000 22 / 28; 16 nodes,
-// 32 x 1,000 67 / 77, 8 x 5,310 83 / 74; 8 nodes, 32 x 4,000 117 / 189.
+// tile of the mma.sync kernel (32 rows, 16 positions) takes a block 0.4 us.  So: by the tiles that an SM gets.  One or two row tiles leave the 128
+// lanes of an accumulator half empty, the more so the more heads there are to begin with.  Measured (us, mma.sync / tcgen05; 32 / 8 heads, fp32, 8 bits): 64
+// nodes, 8 x 2,048 positions 152 / 60, 4 x 1,000 40 / 32, 4 x 300 20 / 28; 24 nodes, 8 x 2,048 55 / 39, 4 x 1,000 22 / 26; 16 nodes, 32 x 1,000 67 / 70,
+// 8 x 5,310 83 / 63; 10 nodes, 8 x 1,300 29 / 30, 8 x 3,000 53 / 43, 32 x 400 35 / 46; 8 nodes, 32 x 4,000 117 / 148.
 static bool many_rows(long heads, int rows, int ctx, int sms) {
     if (rows <= kFewRows) return false;
     const double tiles = (double)heads * ((rows + 31) / 32) * ((ctx + 15) / 16) / sms;
-    return tiles >= (rows <= 64 ? 280 : ctx <= 128 ? 40 : 80);
+    return tiles >= (rows <= 64 ? 60 + 0.8 * heads : ctx <= 128 ? 40 : 80);
 }
 static int g_route = 0;   // experiments: 1 mma.sync, 2 tcgen05
 void set_route(int v) { g_route = v; }

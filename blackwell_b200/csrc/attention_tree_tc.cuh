@@ -15,10 +15,10 @@
 // Work is shared out in tiles of 64 positions: all sequences' tiles, heads and row groups in one line, an equal stretch of it per block; what
 // a block has of a head's context that it does not have whole goes to a record that the merge kernel joins.
 // All waits are bounded; a wait that gives up raises an abort flag.
-// Measured (8 trees of 64 nodes over 2,000 to 4,096 positions, 32 / 8 heads, 8 bits): bf16 59 us, 0.42 PFLOP/s, fp32 93.  Of a block's 88,000 cycles a
+// Measured (8 trees of 64 nodes over 2,000 to 4,096 positions, 32 / 8 heads, 8 bits): bf16 58 us, 0.43 PFLOP/s, fp32 90.  Of a block's 85,000 cycles a
 // tile takes 2,600, the softmax of a stream that long from one tile to the next (scores out of tensor memory 250, scales and maximum 600, exponentials 1,200;
-// the units' own rates would allow 1,100, the rest is latency of one warp per scheduler and stream); the start 4,000, and each of two parts 12,000 for the
-// queries' place, the first scores and the record, whose 128 KB an SM stores in 5,000.  The merge takes 5 us.  Tried and not kept: maximum and exponentials in
+// the units' own rates would allow 1,100, the rest is latency of one warp per scheduler and stream); the start 4,000, and each of two parts 10,000 to
+// 12,000 for the queries' place, the first scores and the record of 128 KB (stored a column at a time it took 5,000).  The merge takes 5 us.  Tried and not kept: maximum and exponentials in
 // one pass over the scores (slower), streams held half a tile apart (1 to 3 %).
 #pragma once
 #include "attention_tree.cuh"
