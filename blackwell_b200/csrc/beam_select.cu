@@ -8,7 +8,7 @@
 // each other: a stale one lowers the bar.  A list that has grown is cut to its best.  The second launch, a block per request, forms the rows' log-sums and ranks the
 // stretches' candidates across the beams, scores in 64 bits: two beams' candidates may lie closer to each other than 32 bits tell apart.
 // The exponentials and their sums are 32-bit, taken of differences that are exact where they matter; a log-sum is right to some 1e-7.
-// Measured (16 x 8 beams of 151,643 tokens, 78 MB): 25.5 us, 3.0 TB/s, of which the merge and its launch are 5; the first launch alone is bound
+// Measured (16 x 8 beams of 151,643 tokens, 78 MB): 23.9 us, 3.2 TB/s, of which the merge and its launch are 4; the first launch alone is bound
 // by the instructions that a value takes, not by memory (the exponentials some 5 us of it).
 #include <float.h>
 
@@ -31,7 +31,7 @@ constexpr int kVec = 4;                       // 16-byte vectors of a thread in 
 constexpr int kTurn = kThreads * kVec;        // vectors a block takes at once
 constexpr int kGrown = 128;                   // entries from which a warp's list is cut to the best
 constexpr int kList = kGrown + 32 * 4 * kVec; // ... and one turn that enters whole
-constexpr int kStaged = 4096;                 // candidates of a request that the merge holds in shared memory
+constexpr int kStaged = 2048;                 // candidates of a request that the merge holds in shared memory
 constexpr int kMaxLists = 64 * kWarps;        // stretches of a request's beams, at most: two per lane of the merge's warps
 
 struct Args {
@@ -156,17 +156,18 @@ __device__ __forceinline__ void tournament(int lists, int keep, int lane, const 
     __syncwarp();
 }
 
-// The rest of request m: log-sums, then the best of the stretches' candidates.  s_key: room for `room` keys.  kFew: 64 lists at most.
+// The rest of request m: log-sums, then the best of the stretches' candidates, whose scores are formed before, all at once: a round that forms the
+// winner's next one takes 1,000 cycles, one that finds it 300.  s_key, s_at: kStaged each.  kFew: 64 lists at most.
 template <bool kFew>
-__device__ __forceinline__ void merge(const Args& a, int m, unsigned long long* s_key, int room) {
+__device__ __forceinline__ void merge(const Args& a, int m, unsigned long long* s_key, uint32_t* s_at) {
     __shared__ double s_lse[kMaxBeams];
     __shared__ float s_score[kMaxBeams];
     __shared__ unsigned char s_ended[kMaxBeams];
-    __shared__ Cand s_best[kFew ? 1 : kWarps][kMaxKeep];
+    __shared__ Cand s_best[kFew ? 1 : kWarps][kMaxKeep], s_out[kMaxKeep];
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int lists = a.beams * a.chunks, total = lists * a.keep;
     const unsigned long long* best = a.best + (size_t)m * total;
-    const bool staged = total <= room;
+    const bool staged = total <= kStaged;
     if (staged)
         for (int i = t; i < total; i += kThreads) s_key[i] = best[i];
     for (int b = warp; b < a.beams; b += kWarps) {
@@ -196,20 +197,44 @@ __device__ __forceinline__ void merge(const Args& a, int m, unsigned long long* 
     }
     __syncthreads();
     // Entry i of list l (a beam's stretch); an ended beam has one, its first stretch's.
-    auto head = [&](int l, int i) {
-        const int b = l / a.chunks;
+    auto formed = [&](int l, int i, unsigned long long k) {
+        const int b = l / (uint32_t)a.chunks;
         Cand x{0, 0};
         if (s_ended[b]) {
             if (l == b * a.chunks && i == 0 && s_score[b] > -INFINITY) x = Cand{order64((double)s_score[b]), (uint32_t)b * a.vocab + a.eos};
             return x;
         }
-        const unsigned long long k = staged ? s_key[l * a.keep + i] : best[(size_t)l * a.keep + i];
         if (k == 0) return x;
         const double s = (double)s_score[b] + ((double)order32_value((uint32_t)(k >> 32)) - s_lse[b]);
         if (s > -INFINITY) x = Cand{order64(s), (uint32_t)b * a.vocab + (0xFFFFFFFFu - (uint32_t)k)};
         return x;
     };
-    auto out = [&](int r, const Cand& x) {
+    if (staged) {
+        for (int j = t; j < total; j += kThreads) {
+            const int l = j / (uint32_t)a.keep;
+            const Cand x = formed(l, j - l * a.keep, s_key[j]);
+            s_key[j] = x.score;
+            s_at[j] = x.at;
+        }
+        __syncthreads();
+    }
+    auto head = [&](int l, int i) {
+        const int j = l * a.keep + i;
+        return staged ? Cand{s_key[j], s_at[j]} : formed(l, i, best[(size_t)j]);
+    };
+    auto out = [&](int r, const Cand& x) { s_out[r] = x; };
+    if (kFew || lists <= 64) {
+        if (warp != 0) return;
+        tournament(lists, a.keep, lane, head, out);
+    } else {
+        const int per = (lists + kWarps - 1) / kWarps, l0 = min(warp * per, lists);
+        tournament(min(per, lists - l0), a.keep, lane, [&](int l, int i) { return head(l0 + l, i); }, [&](int r, const Cand& x) { s_best[kFew ? 0 : warp][r] = x; });
+        __syncthreads();
+        if (warp != 0) return;
+        tournament(kWarps, a.keep, lane, [&](int l, int i) { return s_best[kFew ? 0 : l][i]; }, out);
+    }
+    for (int r = lane; r < a.keep; r += 32) {            // (the tournament ends with its warp's writes in place)
+        const Cand x = s_out[r];
         const size_t o = (size_t)m * a.keep + r;
         const bool some = x.score != 0;
         const int b = some ? (int)(x.at / (uint32_t)a.vocab) : -1, v = some ? (int)(x.at - (uint32_t)b * a.vocab) : -1;
@@ -217,21 +242,15 @@ __device__ __forceinline__ void merge(const Args& a, int m, unsigned long long* 
         a.token[o] = v;
         a.score_out[o] = some ? (float)order64_value(x.score) : -INFINITY;
         if (a.ended_out) a.ended_out[o] = some && (s_ended[b] || v == a.eos);
-    };
-    if (kFew || lists <= 64) {
-        if (warp == 0) tournament(lists, a.keep, lane, head, out);
-        return;
     }
-    const int per = (lists + kWarps - 1) / kWarps, l0 = min(warp * per, lists);
-    tournament(min(per, lists - l0), a.keep, lane, [&](int l, int i) { return head(l0 + l, i); }, [&](int r, const Cand& x) { s_best[warp][r] = x; });
-    __syncthreads();
-    if (warp == 0) tournament(kWarps, a.keep, lane, [&](int l, int i) { return s_best[l][i]; }, out);
 }
+
 __global__ void __launch_bounds__(kThreads) merge_kernel(const Args a) {
     __shared__ unsigned long long s_key[kStaged];
+    __shared__ uint32_t s_at[kStaged];
     pdl_trigger();
     pdl_wait();
-    merge<false>(a, blockIdx.x, s_key, kStaged);
+    merge<false>(a, blockIdx.x, s_key, s_at);
 }
 
 // kFused: a request's blocks are a cluster, whose first goes on with the merge.
@@ -389,18 +408,21 @@ __global__ void __launch_bounds__(kThreads, 4) chunk_kernel(const Args a) {
     if (kFused) {
         cluster_sync_all();
         const int m = row / (uint32_t)a.beams;
-        if (c == 0 && row == m * a.beams) merge<true>(a, m, s_list[0], kWarps * kList);
+        static_assert(kWarps * kList * 8 >= kStaged * 12, "the merge's candidates lie over the lists");
+        if (c == 0 && row == m * a.beams) merge<true>(a, m, s_list[0], reinterpret_cast<uint32_t*>(s_list[0] + kStaged));
     }
 }
 
-// Stretches of a row: whole turns, four blocks per SM where that many are to be had.  A few requests that a cluster each reads in two turns or fewer:
-// one launch.  On the device both take the same (1 x 4 beams of 32,768 tokens 8.0 us, in two launches 7.3), but a launch costs the caller 2 us: calls
-// in a row take 9 instead of 11.  skew: elements that rows may start behind a 16-byte boundary.
-constexpr int kFusedBlocks = 16, kFusedTurns = 2;
+// Stretches of a row: whole turns, four blocks per SM where that many are to be had.  A few requests that a cluster each reads in three turns or fewer:
+// one launch.  On the device both take much the same (1 x 4 beams of 32,768 tokens 7.1 us, in two launches 6.4), but a launch costs the caller 2 us:
+// calls in a row take 9 instead of 11.  skew: elements that rows may start behind a 16-byte boundary.
+constexpr int kFusedBlocks = 16, kFusedTurns = 3;
 static bool stretches(int vocab, int skew, int beams, long rows, int sms, Args* a) {
     const int vectors = (vocab + skew + 3) / 4, turns = (vectors + kTurn - 1) / kTurn;
-    const bool fused = beams <= kFusedBlocks && kFusedBlocks * rows <= (long)sms * beams && (turns + kFusedBlocks / beams - 1) / (kFusedBlocks / beams) <= kFusedTurns;
-    long n = fused ? kFusedBlocks / beams : 4L * sms / rows;
+    int most = kFusedBlocks / beams;
+    most = most > turns ? turns : most;
+    const bool fused = most > 0 && rows * most <= 2L * sms && (turns + most - 1) / most <= kFusedTurns;
+    long n = fused ? most : 4L * sms / rows;
     n = n > kMaxLists / beams ? kMaxLists / beams : n;
     n = n < 1 ? 1 : n > turns ? turns : n;
     a->chunk = (int)((turns + n - 1) / n) * kTurn;

@@ -429,7 +429,7 @@ def check_select(logits, score, ended, eos, keep, M, B, stride=None, inplace=Fal
     assert torch.equal(e_out.bool(), gone)
 
 
-@pytest.mark.parametrize("M, B, V, keep", [(1, 1, 1, 1), (1, 1, 7, 10), (2, 4, 1000, 4), (1, 4, 32768, 8), (3, 7, 2049, 14), (2, 8, 151643, 8), (1, 64, 5000, 64),
+@pytest.mark.parametrize("M, B, V, keep", [(1, 1, 1, 1), (1, 1, 7, 10), (2, 4, 1000, 4), (1, 4, 32768, 8), (3, 7, 2049, 14), (2, 8, 151643, 8), (1, 64, 5000, 64), (9, 16, 4099, 16), (1, 16, 11000, 32), (4, 2, 90001, 3),
                                            (20, 16, 8193, 32), (1, 2, 300000, 1)])
 def test_select(cuda, M, B, V, keep):
     g = torch.Generator("cuda").manual_seed(V + keep)
