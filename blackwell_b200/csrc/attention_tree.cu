@@ -15,34 +15,34 @@ constexpr int kFewRows = 32;            // query rows of a head that the mma.syn
 constexpr int kMaxCluster = 8;
 constexpr int kCut = 512;               // positions of a warp, where contexts are long: their lengths differ, and the last block is waited for
 // Blocks that share a context of a (sequence, head, row tile), a multiple of eight where more than a cluster.
-// Few contexts: one wave of two blocks per SM, by the tiles of 16 positions that a warp is left with (0.45 us for eight columns), against 0.9 us for a
-// cluster's merge; clusters of other than 2, 4 or 8 blocks leave places of the chip empty and take longer to be placed.  Still more shares of a
-// long context, joined by a second launch, where a wave has room for them.  Many contexts: kCut positions for a warp at most, as far as the records allow
-// (rows of few heads: any number, scratch_bytes; many rows: two waves of blocks), and one or two more where that fills the last wave.
+// The fewest waves of two blocks per SM times what a block takes: the tiles of 16 positions that a warp is left with (0.45 us for eight columns) and 0.9 us
+// for a cluster's merge; clusters of other than 2, 4 or 8 blocks take longer to be placed, and in a wave that is nearly full not all find a place.  Four tiles of
+// columns, bound by mma.sync: one wave (32 x 10 nodes, 1,500 positions: 83 us, in three shares 109).
+// At least as many as leave a warp kCut positions, as far as the records allow (rows of few heads: any number, scratch_bytes; many rows: two waves of
+// blocks).  Still more shares of a long context, joined by a second launch, where a wave has room for them.
 // Measured (us, 32 / 8 heads, fp32; in 1 2 3 4 5 6 8 shares): 1 x 100 positions of 8 bits 3.9 5.1 5.3 5.7 5.9 6.0 6.1, 1 x 500 6.1 5.9 6.0 5.5 5.6 5.7 5.7, 1 x 2,048
 // 13.7 10.0 8.8 7.7 7.6 7.3 6.7, 8 x 4,000 24 20 17 15 22 22 21, 20 x 6,000 48 47 41 44 43 48 54, 32 x 8,192 75 74 75 76 79 85 95; 4 trees of 8 nodes,
 // 1,000 positions of 16 bits, 28 / 4 heads, 25.6 20.4 18.4 16.6 15.7 15.9 13.9.  Clusters of 16 need 16 free SMs next to each other: 1 x 2,048 positions
 // with 64 rows 27 us, as two clusters of 8 and a merge 20.
 static int choose_splits(long pairs, int ctx, int slots, int warps, int nt, bool few) {
     const long tiles = (ctx + kTile - 1) / kTile, least = (ctx + (long)kCut * warps - 1) / (kCut * warps);
-    auto whole = [](long k) { return (k & (k - 1)) == 0; };
-    auto cost = [&](long k) { return (tiles + k * warps - 1) / (k * warps) * nt + (k == 1 ? 0 : whole(k) ? 2 : 3); };
-    long n = 1;
-    for (long k = 2; k <= kMaxCluster; ++k)
-        if (pairs * k <= (whole(k) || nt > 1 ? slots : slots * 17 / 20) && cost(k) < cost(n)) n = k;
+    auto cost = [&](long k) {
+        const bool whole = (k & (k - 1)) == 0;
+        long waves = (pairs * k + slots - 1) / slots;
+        if (!whole && nt == 1 && pairs * k * 20 > (20 * waves - 3) * slots) ++waves;
+        return waves * ((tiles + k * warps - 1) / (k * warps) * nt + (k == 1 ? 0 : whole ? 2 : 3));
+    };
+    long n = least < 1 ? 1 : least > kMaxCluster ? kMaxCluster : least;
+    for (long k = n + 1; k <= kMaxCluster && k * warps < tiles + warps && (nt < 4 || pairs * k <= slots); ++k)
+        if (cost(k) < cost(n)) n = k;
     if (n == kMaxCluster) {
         const long room = slots / pairs, most = ctx / (32 * warps), more = (room < most ? room : most) / kMaxCluster * kMaxCluster;
         if (more > n) n = more;
-    }
-    if (n < least && least > kMaxCluster) {
-        n = (least + kMaxCluster - 1) / kMaxCluster * kMaxCluster;
-        const long records = 2L * slots / pairs;
-        if (!few && n > records) n = records < kMaxCluster ? kMaxCluster : records / kMaxCluster * kMaxCluster;
-    } else if (n < least) {
-        auto waves = [&](long k) { return (pairs * k + slots - 1) / slots; };
-        n = least;
-        for (long k = least + 1; k <= least + 2 && k <= kMaxCluster && k * (kCut / 4) * warps <= ctx; ++k)
-            if (20 * waves(k) * n < 19 * waves(n) * k) n = k;
+        if (n < least) {
+            n = (least + kMaxCluster - 1) / kMaxCluster * kMaxCluster;
+            const long records = 2L * slots / pairs;
+            if (!few && n > records) n = records < kMaxCluster ? kMaxCluster : records / kMaxCluster * kMaxCluster;
+        }
     }
     return (int)n;
 }
@@ -120,7 +120,7 @@ static cudaError_t launch_tc_rows(const Args& a, cudaStream_t st) {
 static bool many_rows(long heads, int rows, int ctx, int sms) {
     if (rows <= kFewRows) return false;
     const double tiles = (double)heads * ((rows + 31) / 32) * ((ctx + 15) / 16) / sms;
-    return tiles >= (rows <= 64 ? 60 + 0.8 * heads : ctx <= 128 ? 40 : 80);
+    return tiles >= (rows <= 64 ? 60 + 0.8 * heads : ctx <= 2 * kTcKeys ? 16 : 80);
 }
 static int g_route = 0;   // experiments: 1 mma.sync, 2 tcgen05
 void set_route(int v) { g_route = v; }
