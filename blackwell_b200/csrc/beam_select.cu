@@ -53,8 +53,8 @@ __device__ __forceinline__ uint32_t order32(float f) {
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float order32_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k); }
-// Larger value first, then the lower index.
-__device__ __forceinline__ unsigned long long key_of(float v, uint32_t index) { return (unsigned long long)order32(v) << 32 | (0xFFFFFFFFu - index); }
+// Larger value first, then the lower index; the zeros are one value.
+__device__ __forceinline__ unsigned long long key_of(float v, uint32_t index) { return (unsigned long long)order32(v + 0.f) << 32 | (0xFFFFFFFFu - index); }
 
 // A candidate of the merge: its score as an integer that orders as the score does (64-bit comparisons of floats have a long latency; ranking
 // is a chain of them), 0: none.
@@ -63,7 +63,7 @@ struct Cand {
     uint32_t at;                        // beam * vocab + token
 };
 __device__ __forceinline__ unsigned long long order64(double d) {
-    const unsigned long long b = (unsigned long long)__double_as_longlong(d);
+    const unsigned long long b = (unsigned long long)__double_as_longlong(d + 0.0);   // (-0 becomes +0)
     return b >> 63 ? ~b : b | 1ull << 63;
 }
 __device__ __forceinline__ double order64_value(unsigned long long k) { return __longlong_as_double((long long)(k >> 63 ? k & ~(1ull << 63) : ~k)); }

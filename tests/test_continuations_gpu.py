@@ -477,6 +477,26 @@ def test_select_dead_beams_and_odd_values(cuda):
     check_select(logits, score, None, 7, 4, 2, B)
 
 
+@pytest.mark.parametrize("keep", [1, 4, 20])
+@pytest.mark.parametrize("V", [50, 9001])
+def test_select_zeros_of_both_signs(cuda, V, keep):
+    """-0 and +0 are equal: the lower token first, inside a stretch of a row and across them."""
+    g = torch.Generator("cuda").manual_seed(V)
+    B = 2
+    logits = -torch.empty((2 * B, V), device="cuda").normal_(generator=g).abs().round()
+    logits = torch.where((logits == 0) & (torch.rand((2 * B, V), generator=g, device="cuda") < 0.5), 0.0, logits)
+    logits[:, 0], logits[:, 1] = -1.0, -0.0
+    assert bool((logits.view(torch.int32) == -2 ** 31).any()) and bool((logits.view(torch.int32) == 0).any())
+    check_select(logits, torch.tensor([[-1.0, -1.5], [-3.0, -0.25]], device="cuda"), None, -1, keep, 2, B)
+
+
+def test_select_scores_of_both_zeros(cuda):
+    """Beams that have ended with -0 and +0: the lower beam first."""
+    logits, score = torch.zeros((3, 40), device="cuda"), torch.tensor([[-0.0, 0.0, -0.0]], device="cuda")
+    check_select(logits, score, torch.ones((1, 3), dtype=torch.uint8, device="cuda"), 7, 3, 1, 3)
+    check_select(logits, score, torch.ones((1, 3), dtype=torch.uint8, device="cuda"), 7, 1, 1, 3)
+
+
 def test_select_in_a_graph(cuda):
     g = torch.Generator("cuda").manual_seed(10)
     k, B, V = kernels(), 4, 9000
