@@ -67,7 +67,6 @@ __device__ __forceinline__ unsigned long long order64(double d) {
     return b >> 63 ? ~b : b | 1ull << 63;
 }
 __device__ __forceinline__ double order64_value(unsigned long long k) { return __longlong_as_double((long long)(k >> 63 ? k & ~(1ull << 63) : ~k)); }
-__device__ __forceinline__ bool before(const Cand& a, const Cand& b) { return a.score > b.score || (a.score == b.score && a.at < b.at); }
 
 __device__ __forceinline__ unsigned long long pair_of(float lo, float hi) {
     unsigned long long r;
@@ -126,29 +125,50 @@ __device__ __forceinline__ float exponentials(const float4 (&v)[kVec], float to)
     return (p[0] + p[1]) + (p[2] + p[3]);
 }
 
+// Which of several candidates of the same score comes first: the lower beam, within a beam the larger logit, as inside a list (two logits may differ by
+// less than their 64-bit scores show), then the lower token.  x: the lane's two, of which `in` (by bits) are among them; bit 2: the winner is this
+// lane's, of number bit 0.  rows: the request's logits.  (A call: hardly ever needed, and the rounds are short.)
+__device__ __noinline__ int first_of_equal(uint32_t at0, uint32_t at1, int in, const float* rows, long row_stride, uint32_t vocab) {
+    auto logit = [&](uint32_t at) {
+        const uint32_t b = at / vocab;
+        return order32(rows[(size_t)b * row_stride + (at - b * vocab)] + 0.f);
+    };
+    const uint32_t beam0 = in & 1 ? at0 / vocab : 0xFFFFFFFFu, beam1 = in & 2 ? at1 / vocab : 0xFFFFFFFFu;
+    const uint32_t beam = __reduce_min_sync(0xffffffffu, min(beam0, beam1));
+    const uint32_t v0 = beam0 == beam ? logit(at0) : 0, v1 = beam1 == beam ? logit(at1) : 0;     // (order32 of a finite number is not 0)
+    const uint32_t v = __reduce_max_sync(0xffffffffu, max(v0, v1));
+    const uint32_t c0 = v0 == v ? at0 : 0xFFFFFFFFu, c1 = v1 == v ? at1 : 0xFFFFFFFFu;
+    const uint32_t at = __reduce_min_sync(0xffffffffu, min(c0, c1));
+    return c0 == at ? 4 : c1 == at ? 5 : 0;
+}
 // The best of up to 64 sorted lists, two per lane, one after the other: head(l, i) is entry i of list l (score 0: none), emit(r, cand)
 // takes the r-th best, by the lane that holds it.  A round is three warp-wide integer reductions; only the winner's list moves on.
 template <typename Head, typename Emit>
-__device__ __forceinline__ void tournament(int lists, int keep, int lane, const Head& head, const Emit& emit) {
+__device__ __forceinline__ void tournament(int lists, int keep, int lane, const float* rows, long row_stride, uint32_t vocab, const Head& head, const Emit& emit) {
     Cand x[2];
     int i[2] = {0, 0};
 #pragma unroll
     for (int e = 0; e < 2; ++e) x[e] = lane + 32 * e < lists ? head(lane + 32 * e, 0) : Cand{0, 0};
     for (int r = 0; r < keep; ++r) {
-        const int e = before(x[1], x[0]);
-        const Cand y = e ? x[1] : x[0];
-        const uint32_t hi = (uint32_t)(y.score >> 32), lo = (uint32_t)y.score;
+        int e = x[1].score > x[0].score;
+        const unsigned long long y = e ? x[1].score : x[0].score;
+        const uint32_t hi = (uint32_t)(y >> 32), lo = (uint32_t)y;
         const uint32_t mhi = __reduce_max_sync(0xffffffffu, hi);
         const uint32_t mlo = __reduce_max_sync(0xffffffffu, hi == mhi ? lo : 0u);
-        const bool tied = hi == mhi && lo == mlo;
-        const uint32_t at = __reduce_min_sync(0xffffffffu, tied ? y.at : 0xFFFFFFFFu);
+        bool best = hi == mhi && lo == mlo;
+        const bool both = x[0].score == x[1].score;
         if (mhi == 0 && mlo == 0) {
             if (lane == 0)
                 for (; r < keep; ++r) emit(r, Cand{0, 0});
             break;
         }
-        if (tied && y.at == at) {
-            emit(r, y);
+        if (__reduce_add_sync(0xffffffffu, best ? both ? 2u : 1u : 0u) > 1) {
+            const int w = first_of_equal(x[0].at, x[1].at, !best ? 0 : both ? 3 : 1 << e, rows, row_stride, vocab);
+            best = w != 0;
+            e = w & 1;
+        }
+        if (best) {
+            emit(r, e ? x[1] : x[0]);
             if (e) x[1] = ++i[1] < keep ? head(lane + 32, i[1]) : Cand{0, 0};
             else x[0] = ++i[0] < keep ? head(lane, i[0]) : Cand{0, 0};
         }
@@ -223,21 +243,23 @@ __device__ __forceinline__ void merge(const Args& a, int m, unsigned long long* 
         return staged ? Cand{s_key[j], s_at[j]} : formed(l, i, best[(size_t)j]);
     };
     auto out = [&](int r, const Cand& x) { s_out[r] = x; };
+    const uint32_t vocab = a.vocab;
+    const float* rows = a.logits + (size_t)m * a.beams * a.row_stride;
     if (kFew || lists <= 64) {
         if (warp != 0) return;
-        tournament(lists, a.keep, lane, head, out);
+        tournament(lists, a.keep, lane, rows, a.row_stride, vocab, head, out);
     } else {
         const int per = (lists + kWarps - 1) / kWarps, l0 = min(warp * per, lists);
-        tournament(min(per, lists - l0), a.keep, lane, [&](int l, int i) { return head(l0 + l, i); }, [&](int r, const Cand& x) { s_best[kFew ? 0 : warp][r] = x; });
+        tournament(min(per, lists - l0), a.keep, lane, rows, a.row_stride, vocab, [&](int l, int i) { return head(l0 + l, i); }, [&](int r, const Cand& x) { s_best[kFew ? 0 : warp][r] = x; });
         __syncthreads();
         if (warp != 0) return;
-        tournament(kWarps, a.keep, lane, [&](int l, int i) { return s_best[kFew ? 0 : l][i]; }, out);
+        tournament(kWarps, a.keep, lane, rows, a.row_stride, vocab, [&](int l, int i) { return s_best[kFew ? 0 : l][i]; }, out);
     }
     for (int r = lane; r < a.keep; r += 32) {            // (the tournament ends with its warp's writes in place)
         const Cand x = s_out[r];
         const size_t o = (size_t)m * a.keep + r;
         const bool some = x.score != 0;
-        const int b = some ? (int)(x.at / (uint32_t)a.vocab) : -1, v = some ? (int)(x.at - (uint32_t)b * a.vocab) : -1;
+        const int b = some ? (int)(x.at / vocab) : -1, v = some ? (int)(x.at - (uint32_t)b * vocab) : -1;
         a.parent[o] = b;
         a.token[o] = v;
         a.score_out[o] = some ? (float)order64_value(x.score) : -INFINITY;

@@ -332,7 +332,8 @@ int bw_attention_tree(void* out, const void* q, const bw_kv_cache* cache, const 
                       void* stream);
 size_t bw_attention_tree_scratch_bytes(int M, int T, int num_q_heads, int num_kv_heads, int max_context);
 /* Beam search's selection for M requests of `beams` beams each: candidates score[m][b] + log_softmax(logits[m * beams + b])[v] over all beams and
- * tokens, of which the `keep` best (largest first; equal ones by lower beam, then token) go to parent_out, token_out, score_out [M][keep].  logits fp32 [M * beams][row_stride].
+ * tokens, of which the `keep` best (largest first; equal scores by lower beam, within a beam by larger logit, then lower token) go to parent_out,
+ * token_out, score_out [M][keep].  logits fp32 [M * beams][row_stride].
  * A beam that has ended (ended[m][b] != 0) offers itself alone, as (eos_id, score unchanged); ended_out = ended[parent] or token == eos_id.
  * Candidates of score -inf are none: where fewer than `keep` are left, parent and token are -1 and the score -inf.  A NaN logit counts as -inf; a
  * row with a logit of +inf offers nothing.  Scores are formed and compared in 64 bits; a log-sum is right to some 1e-7.  beams <= 64, keep <= 64.

@@ -497,6 +497,22 @@ def test_select_scores_of_both_zeros(cuda):
     check_select(logits, score, torch.ones((1, 3), dtype=torch.uint8, device="cuda"), 7, 1, 1, 3)
 
 
+@pytest.mark.parametrize("B, V, keep", [(1, 300, 5), (2, 30000, 6), (1, 200000, 40), (8, 151643, 8), (16, 40000, 20)])
+def test_select_logits_closer_than_their_scores(cuda, B, V, keep):
+    """Scores that fall together in 64 bits: within a beam the larger logit first, wherever in the row; equal logits by token."""
+    g = torch.Generator("cuda").manual_seed(V)
+    k = kernels()
+    logits = torch.empty((B, V), device="cuda").normal_(generator=g) * 1e-20
+    logits[:, V // 3], logits[:, V - 2], logits[:, 5] = 9e-20, 9e-20, 8e-20
+    score = -torch.arange(B, device="cuda").float()[None]
+    assert len(set((score[0, :1].double() + (logits[0].double() - math.log(V))).tolist())) == 1
+    parent, token = torch.zeros((1, keep), dtype=torch.int32, device="cuda"), torch.zeros((1, keep), dtype=torch.int32, device="cuda")
+    out = torch.zeros((1, keep), device="cuda")
+    scratch = torch.empty(k.beam_select_scratch_bytes(V, B, keep, 1), dtype=torch.uint8, device="cuda")
+    k.beam_select(parent, token, out, None, logits, V, V, score, None, -1, B, keep, 1, scratch)
+    assert (parent == 0).all() and torch.equal(token[0].long(), logits[0].sort(descending=True, stable=True).indices[:keep])
+
+
 def test_select_in_a_graph(cuda):
     g = torch.Generator("cuda").manual_seed(10)
     k, B, V = kernels(), 4, 9000
