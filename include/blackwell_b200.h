@@ -315,7 +315,7 @@ typedef struct bw_kv_cache {
  * key heads get the RMS norm per head (weights fp32 [128]; NULL: none) and the rotation of interleaved pairs by position * rope_base^(-2i/128), the angle
  * formed in 64 bits; queries go to q_out [M][T][nq * 128], keys and values to the rows first[m] + i of the cache.  The position of row i is
  * first[m] + offset[m][i] (a node's depth), or first[m] + i where offset is NULL.  e4m3: scale = absmax / 448 (1 where absmax < 1e-10),
- * code = the nearest to x * (448 / absmax).  Rows i >= count[m] (NULL: T) and those of a sequence with first[m] < 0 are skipped: nothing of
+ * code = the nearest to x * (448 / absmax), that factor to 2^-22.  Rows i >= count[m] (NULL: T) and those of a sequence with first[m] < 0 are skipped: nothing of
  * them is read or written.  A row at or beyond max_seq is not stored; its query is. */
 int bw_qk_norm_rope_kv_rows(void* q_out, const bw_kv_cache* cache, const void* qkv, const float* q_norm_w_or_null,
                             const float* k_norm_w_or_null, const int* d_first_row, const int* d_offset_or_null, const int* d_count_or_null,

@@ -139,6 +139,26 @@ def test_write_rows_of_zeros_and_tiny_rows(cuda):
     assert (k[0, 0, 1:3] == 0).all() and (v[0, 0, 1:3] == 0).all() and (st.ks[0, 0, 0, 1:3] == 1).all() and st.ks[0, 0, 0, 3].isnan()
 
 
+@BOTH
+def test_write_codes_and_scales_of_values_of_any_size(cuda, act):
+    """Value rows are neither normed nor turned: up to the largest numbers scales are absmax / 448 to two roundings, and codes nearest to x * (448 /
+    absmax), the factor off by two steps of 2^-23 and the product by a rounding."""
+    g = torch.Generator("cuda").manual_seed(2)
+    st = Store(g, 1, 1, 2, 40, True)
+    size = torch.logspace(-9, 38, 40, dtype=torch.float64, device="cuda").float()
+    qkv = torch.empty((1, 40, 5, HD), device="cuda").uniform_(-1, 1, generator=g)
+    qkv[0, :, :3] = 1.0
+    qkv = (qkv * size[:, None, None]).to(act)
+    assert bool(qkv.isfinite().all()) and float(qkv.abs().max()) > 2.0 ** 126
+    kernels().qk_norm_rope_kv_rows(torch.empty((1, 40, 1, HD), dtype=act, device="cuda"), st.args(), qkv, None, None, ints([0]), None, None, 1, 1, 40, 1e-6, 1e4)
+    x = qkv[0, :, 3:].float().transpose(0, 1)
+    top = x.abs().amax(-1, keepdim=True)
+    unit = top[..., 0].double() / 448
+    assert ((st.vs[0, 0].double() - unit).abs() <= unit * 2.0 ** -23).all()
+    want = x.double() * 448 / top.double()
+    assert ((st.v[0, 0].double() - want).abs() <= torch.maximum(want.abs() * 2.0 ** -4, torch.full_like(want, 2.0 ** -10)) + want.abs() * 2.0 ** -21).all()
+
+
 # ------------------------------------------------------------------------------------------------------------------ attention
 def tree_masks(g, M, T):
     """Ancestor masks of random trees, as Python integers [M][T]."""
