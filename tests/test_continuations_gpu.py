@@ -113,6 +113,24 @@ def test_write(cuda, M, T, nq, nkv, coded, act):
     check_write(M, T, nq, nkv, [(11 * m) % 40 for m in range(M)], 300, coded, act)
 
 
+@BOTH
+@CACHES
+@pytest.mark.parametrize("M, nq, nkv", [(8, 28, 4), (3, 13, 13), (2, 5, 1), (5, 64, 8), (1, 6, 3), (4, 1, 1), (7, 32, 8)])
+def test_write_many_rows(cuda, M, nq, nkv, coded, act):
+    """Rows enough that a warp takes four heads (more than 32 rows * heads per SM): warps with heads of every kind, blocks of part of a row,
+    skipped rows and sequences, nodes, rows behind the cache's end."""
+    T = 32 * torch.cuda.get_device_properties(0).multi_processor_count // (M * (nq + 2 * nkv)) + 3
+    g = torch.Generator().manual_seed(T)
+    first, count = [(37 * m) % 50 for m in range(M)], [T - (m % 3) * (T // 4) for m in range(M)]
+    check_write(M, T, nq, nkv, first, 50 + T, coded, act, layers=1, layer=0)
+    if M > 2:
+        first[1], count[2] = -1, 0
+        off = torch.randint(0, T, (M, T), generator=g).tolist()
+        check_write(M, T, nq, nkv, first, T, coded, act, offset=off, count=count, layers=1, layer=0, seed=1)
+    else:
+        check_write(M, T, nq, nkv, first, T // 2, coded, act, norms=False, layers=1, layer=0, seed=1)
+
+
 @CACHES
 def test_write_trees_counts_and_edges(cuda, coded):
     off = [[0, 1, 1, 2, 2], [0, 0, 0, 1, 3], [0, 1, 2, 3, 4], [0, 0, 1, 1, 1], [0] * 5]
