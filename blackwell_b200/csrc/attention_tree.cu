@@ -140,11 +140,12 @@ static size_t kept_bytes(long blocks) { return (size_t)blocks * 2 * kHd * 128 * 
 }  // namespace bw
 
 // A bound for any smaller call too.  The blocks are at most as many as SMs; mma.sync kernel: records of 32 rows of two waves, or of long
-// contexts' shares of four warps for rows of few heads.
+// contexts' shares of four warps for rows of few heads.  tcgen05 kernel: where its rows are many enough, or it is forced.
 extern "C" size_t bw_attention_tree_scratch_bytes(int M, int T, int num_q_heads, int num_kv_heads, int max_context) {
     if (M < 1 || T < 1 || T > tree::kMaxNodes || num_kv_heads < 1 || num_q_heads < 1 || num_q_heads % num_kv_heads || max_context < 1) return 0;
     const int sms = sm_count(current_device()), rows = T * (num_q_heads / num_kv_heads), few = rows < tree::kFewRows ? rows : tree::kFewRows;
-    size_t need = rows <= tree::kFewRows ? tree::record_bytes(sms, 32) : tree::kLineBytes + tree::record_bytes(sms, rows < 256 ? rows : 256) + tree::kept_bytes(sms);
+    const size_t tc = tree::kLineBytes + tree::record_bytes(sms, rows < 256 ? rows : 256) + tree::kept_bytes(sms);
+    const size_t need = rows <= tree::kFewRows && tree::g_route != 2 ? tree::record_bytes(sms, 32) : tc;
     const long positions = 4L * tree::kCut * tree::kMaxCluster, groups = ((long)max_context + positions - 1) / positions;
     const size_t shares = (size_t)M * num_kv_heads * few * groups * tree::kPart * sizeof(float);
     return groups > 1 && shares > need ? shares : need;

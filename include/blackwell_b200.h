@@ -611,7 +611,8 @@ int bw_reserve_scratch(size_t gemv_bytes, size_t attention_bytes);
  * key 23 = bfloat16 linear: up to value - 1 rows (8 at most) take the weight-streaming kernel, more the tcgen05 kernel (0 =
  * automatic), key 24 = products of more than 8 sequences on the tcgen05 kernel's bf16 form (positive: always, negative:
  * never, 0 = by its estimate of both forms; key 6 there: 1 = whole tiles, 2 to 8 = CTAs of a cluster that share a tile,
- * more = equal shares of all chunks), key 25 = bw_attention_tree: 1 = always its mma.sync kernel, 2 = always the tcgen05 kernel, 0 = by size. */
+ * more = equal shares of all chunks), key 25 = bw_attention_tree: 1 = always its mma.sync kernel, 2 = always the tcgen05 kernel, 0 = by size
+ * (bw_attention_tree_scratch_bytes goes by it too: ask after it is set). */
 int bw_set_tuning(int key, int value);
 /* Number of kernels launched by this library since the last call with reset != 0. */
 long long bw_launch_count(int reset);

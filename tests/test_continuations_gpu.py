@@ -364,6 +364,20 @@ def test_attention_shares_of_long_contexts(cuda, coded):
         check_attention(19, 1, 8, 8, [33000 + m for m in range(19)], 34000, coded, torch.float32)
 
 
+@BOTH
+@pytest.mark.parametrize("M, T, nq, nkv, top", [(1, 1, 32, 8, 1500), (32, 1, 32, 8, 3000), (3, 4, 32, 4, 900), (2, 32, 8, 8, 40000), (2, 33, 8, 8, 700),
+                                                (4, 64, 32, 8, 2000), (1, 9, 16, 1, 60000)])
+def test_attention_scratch_of_the_size_given(cuda, M, T, nq, nkv, top, act):
+    """Scratch of the size that the library gives for the call, whichever kernel takes it."""
+    k = kernels()
+
+    def call(out, q, cache, first, mask, count, hint, nq, M, T, _):
+        n = k.attention_tree_scratch_bytes(M, T, nq, nkv, top + T)
+        k.attention_tree(out, q, cache, first, mask, count, hint, nq, M, T, torch.full((n,), 255, dtype=torch.uint8, device="cuda"))
+
+    check_attention(M, T, nq, nkv, [top - 17 * m for m in range(M)], top + T, True, act, call=call)
+
+
 def test_attention_far_offsets(cuda):
     """Sequences whose rows lie beyond 2^32 bytes and elements."""
     g = torch.Generator("cuda").manual_seed(4)
