@@ -8,8 +8,9 @@
 //   S^T [16 positions x 8 rows] = K Q^T,   O^T [16 dimensions x 8 rows] = V^T P^T
 // A warp takes 16 positions at a time for all 8 * NT rows of its block; its softmax state and the unnormalised O^T stay in registers.
 // P goes from the accumulator layout to the operand layout by movmatrix.  e4m3 codes become f16 exactly (no rounding); the key scale
-// multiplies the score, the value scale the probability, there relative to the largest one met so far (a power of two), which keeps
-// the f16 operand in range whatever the values' size.
+// multiplies the score, the value scale the probability.  What the f16 operand has to hold is that product: a row's reference is the maximum of
+// score + log2(value scale) over what it sees, for its sum as well, so that neither a row that it does not see nor one that it hardly weighs takes
+// bits from it.  Scales are taken relative to the size of the warp's first (a power of two), so that scores and references are of one size.
 // fp32 activations: Q and P are split in an f16 high part and an f16 remainder (22 significant bits) and multiplied twice, or, with four
 // rows or fewer (kPair), once with the remainders in the other four columns; bfloat16 activations: once, which rounds P to 11 bits where
 // the result keeps 8.  Each query row is brought to a maximum of 1 to 2 by a power
@@ -38,6 +39,7 @@ constexpr int kMaxNodes = 64;
 constexpr int kTile = 16;               // positions a warp takes at once
 constexpr int kPart = kHd + 4;          // floats of a partial record: outputs, maximum, sum, padding
 constexpr float kHead = 6.f, kSlack = 14.f;   // P up to 2^6 when the maximum is new, 2^14 before it is moved
+constexpr float kLeastScale = -66.f;    // log2; a smaller value scale counts as this one in the reference: sums of P without it stay below 2^80 a position
 
 struct Args {
     void* out;                          // [M * T][nq * 128]
@@ -125,6 +127,18 @@ __device__ __forceinline__ float2 binade(float x) {
     uint32_t e = __float_as_uint(x) >> 23 & 255;
     e = e < 1 ? 127 : min(max(e, 2u), 252u);
     return make_float2(__uint_as_float(e << 23), __uint_as_float((254 - e) << 23));
+}
+
+// The power of two that value scales are taken relative to, at or above their largest (bits of its magnitude).
+__device__ __forceinline__ float scale_unit(uint32_t top) { return __uint_as_float(min(max((top + 0x7FFFFFu) & 0x7F800000u, 87u << 23), 167u << 23)); }
+__device__ __forceinline__ float scale_log2(float relative) { return fmaxf(__log2f(fabsf(relative)), kLeastScale); }
+
+// 2^(from - to), to >= from, in two factors: references that value scales keep far apart (or rows of scale zero) may differ by more than the 2^126 of
+// one, and a sum of probabilities, which is as far from 1, has to outlast that.  Sums of P V that far below do not count.
+template <bool kFar>
+__device__ __forceinline__ float2 step(float from, float to) {
+    const float h = lm::exp2_fast(kFar ? 0.5f * (from - to) : from - to);
+    return make_float2(h, kFar ? h : 1.f);
 }
 
 // What a sequence's rows see: positions [0, first) all of them, node j (position first + j) by bit j of a row's mask.
@@ -263,7 +277,7 @@ __global__ void __launch_bounds__(Shape<NT, kCoded>::kWarps * 32, 2) attend_kern
 #pragma unroll
         for (int e = 0; e < 2; ++e) qf[j][e] = s_unit[8 * j + ((2 * tq + e) & kRowOf)];
 
-    float o[NT][8][4], mx[NT][2], l[NT][2], vref = __uint_as_float(2u << 23);
+    float o[NT][8][4], mx[NT][2], l[NT][2], vunit = 1.f, vcap = -1.f, slack = kSlack;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
         mx[j][0] = mx[j][1] = -FLT_MAX;
@@ -354,36 +368,38 @@ __global__ void __launch_bounds__(Shape<NT, kCoded>::kWarps * 32, 2) attend_kern
                     s[j][e] = yes ? s[j][e] : -INFINITY;
                 }
         }
-        bool move = false;
+        // Codes: a score is compared beside a cap of the value scales that the lane multiplies with, set anew (to four times the present one) when
+        // one exceeds it or the reference moves.
+        bool move = kCoded && fmaxf(fabsf(sc[2]), fabsf(sc[3])) > vcap;
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) move |= fmaxf(s[j][e], s[j][e + 2]) > mx[j][e] + kSlack;
-        float vtop = vref;
-        if (kCoded) {
-            vtop = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fabsf(sc[2]), fabsf(sc[3])))));
-            move |= vtop > vref;
-        }
+            for (int e = 0; e < 2; ++e) move |= fmaxf(s[j][e], s[j][e + 2]) > mx[j][e] + slack;
         if (__any_sync(0xffffffffu, move)) {
-            float fv = 1.f;
-            if (kCoded && vtop > vref) {                // the next power of two
-                const float to = __uint_as_float(min((__float_as_uint(vtop) + 0x7FFFFFu) & 0x7F800000u, 252u << 23));
-                fv = vref * __uint_as_float((254u << 23) - __float_as_uint(to));
-                vref = to;
+            float lg[2] = {0.f, 0.f};
+            if (kCoded) {
+                const float top = fmaxf(fabsf(sc[2]), fabsf(sc[3])), unit = scale_unit(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+                vunit = tile == tile0 + warp ? unit : vunit;     // (the first tile comes here)
+                const float vdiv = __uint_as_float((254u << 23) - __float_as_uint(vunit));
+                lg[0] = scale_log2(sc[2] * vdiv);
+                lg[1] = scale_log2(sc[3] * vdiv);
+                vcap = 4.f * top;
+                slack = kSlack - scale_log2(vcap * vdiv);
             }
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
                 float f[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    float top = fmaxf(s[j][e], s[j][e + 2]);
+                    float top = fmaxf(s[j][e] + lg[0], s[j][e + 2] + lg[1]);
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                    const float to = fmaxf(mx[j][e], top - kHead), cc = lm::exp2_fast(mx[j][e] - to);
+                    const float to = fmaxf(mx[j][e], top - kHead);
+                    const float2 h = step<kCoded>(mx[j][e], to);
                     mx[j][e] = to;
-                    l[j][e] *= cc;
-                    f[e] = cc * fv;
+                    l[j][e] = l[j][e] * h.x * h.y;
+                    f[e] = h.x * h.y;
                 }
 #pragma unroll
                 for (int d = 0; d < 8; ++d) {
@@ -393,8 +409,11 @@ __global__ void __launch_bounds__(Shape<NT, kCoded>::kWarps * 32, 2) attend_kern
             }
         }
         // ---- P^T, and to the operand layout
-        const float vdiv = kCoded ? __uint_as_float((254u << 23) - __float_as_uint(vref)) : 1.f;
-        const float vr[2] = {sc[2] * vdiv, sc[3] * vdiv};
+        if (kCoded) {
+            const float vdiv = __uint_as_float((254u << 23) - __float_as_uint(vunit));
+            sc[2] *= vdiv;
+            sc[3] *= vdiv;
+        }
         uint32_t ph[NT][2], pl[kSplit ? NT : 1][2];
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
@@ -403,7 +422,7 @@ __global__ void __launch_bounds__(Shape<NT, kCoded>::kWarps * 32, 2) attend_kern
             for (int e = 0; e < 4; ++e) {
                 p[e] = lm::exp2_fast(s[j][e] - mx[j][e & 1]);
                 l[j][e & 1] += p[e];
-                if (kCoded) p[e] *= vr[e >> 1];
+                if (kCoded) p[e] *= sc[2 + (e >> 1)];
             }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
@@ -479,7 +498,6 @@ __global__ void __launch_bounds__(Shape<NT, kCoded>::kWarps * 32, 2) attend_kern
 
     // ---- the warps' results to shared memory: [row][128]
     float* so = reinterpret_cast<float*>(dsm + warp * Sh::kPerWarp);
-    const float vmul = kCoded ? vref : 1.f;
     if (kPair) {                                        // high parts and remainders: lanes of columns 0-3 get dimension tiles 0-3, the others 4-7
 #pragma unroll
         for (int d = 0; d < 4; ++d)
@@ -504,7 +522,7 @@ __global__ void __launch_bounds__(Shape<NT, kCoded>::kWarps * 32, 2) attend_kern
 #pragma unroll
             for (int d = 0; d < kTiles; ++d) {
                 if (kCoded) {
-                    *reinterpret_cast<float2*>(so + r * kHd + 16 * g + 2 * (d0 + d)) = make_float2(o[j][d][e] * vmul, o[j][d][e + 2] * vmul);
+                    *reinterpret_cast<float2*>(so + r * kHd + 16 * g + 2 * (d0 + d)) = make_float2(o[j][d][e] * vunit, o[j][d][e + 2] * vunit);
                 } else {
                     so[r * kHd + 16 * (d0 + d) + g] = o[j][d][e];
                     so[r * kHd + 16 * (d0 + d) + g + 8] = o[j][d][e + 2];
@@ -534,9 +552,10 @@ __global__ void __launch_bounds__(Shape<NT, kCoded>::kWarps * 32, 2) attend_kern
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-            const float cc = lm::exp2_fast(s_m[w][r] - top);
+            const float2 h = step<kCoded>(s_m[w][r], top);
+            const float cc = h.x * h.y;
             const float4 v = *reinterpret_cast<const float4*>(dsm + w * Sh::kPerWarp + (r * kHd + 4 * lane) * 4);
-            sum = fmaf(s_l[w][r], cc, sum);
+            sum = fmaf(s_l[w][r] * h.y, h.x, sum);
             acc.x = fmaf(v.x, cc, acc.x); acc.y = fmaf(v.y, cc, acc.y); acc.z = fmaf(v.z, cc, acc.z); acc.w = fmaf(v.w, cc, acc.w);
         }
         if (a.cluster == 1) {
@@ -553,7 +572,9 @@ __global__ void __launch_bounds__(Shape<NT, kCoded>::kWarps * 32, 2) attend_kern
         const uint32_t ml = smem_u32(&s_ml[r]), ov = smem_u32(dsm) + (r * kHd + 4 * lane) * 4;
         const bool has = lane < a.cluster;
         const float tb = has ? ld_dsmem(ml, lane) : -FLT_MAX, lb = has ? ld_dsmem(ml + 4, lane) : 0.f;
-        const float top = warp_max(tb), wgt = lm::exp2_fast(tb - top), sum = warp_sum(lb * wgt);
+        const float top = warp_max(tb);
+        const float2 h = step<kCoded>(tb, top);
+        const float wgt = h.x * h.y, sum = warp_sum(lb * h.x * h.y);
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
         for (int b = 0; b < a.cluster; ++b) {
@@ -586,8 +607,9 @@ __global__ void __launch_bounds__(128) attend_merge_kernel(const Args a) {
     for (int s = 0; s < parts; ++s) {
         const float2 ml = *reinterpret_cast<const float2*>(rec + (size_t)s * kPart + kHd);
         const float4 v = *reinterpret_cast<const float4*>(rec + (size_t)s * kPart + 4 * lane);
-        const float c = lm::exp2_fast(ml.x - top);
-        sum = fmaf(ml.y, c, sum);
+        const float2 h = step<true>(ml.x, top);
+        const float c = h.x * h.y;
+        sum = fmaf(ml.y * h.y, h.x, sum);
         acc.x = fmaf(v.x, c, acc.x); acc.y = fmaf(v.y, c, acc.y); acc.z = fmaf(v.z, c, acc.z); acc.w = fmaf(v.w, c, acc.w);
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;

@@ -11,7 +11,7 @@
 // fp32 activations: Q and P as f16 high parts and remainders, multiplied one after the other.  The accumulator's sums are cut, not rounded, at
 // 24 bits, which adds up: so the remainders of a score come first, and O is added to a sum in the scratch memory (L2) every four tiles and
 // starts afresh (64 nodes over 5,279 positions: error 1.1e-6 of the result, as that of 32-bit sums; every eight tiles 2.3e-6 and a tenth faster).
-// Scales and the moving maximum as in attention_tree.cuh; a warp brings its rows of O to a new maximum by itself.
+// Scales and the moving reference as in attention_tree.cuh (scales relative to the size of a part's first); a warp brings its rows of O to a new one by itself.
 // Work is shared out in tiles of 64 positions: all sequences' tiles, heads and row groups in one line, an equal stretch of it per block; what
 // a block has of a head's context that it does not have whole goes to a record that the merge kernel joins.
 // All waits are bounded; a wait that gives up raises an abort flag.
@@ -31,6 +31,7 @@ constexpr int kTcKeys = 64, kTcPanel = kTcKeys * 128, kTcThreads = 512;   // pos
 constexpr int kTcStage = 4 * kTcPanel;                                    // K and V of a tile
 constexpr int kTcRaw = 2 * kTcKeys * kHd + 2 * kTcKeys * 4;               // codes and scales of a tile
 constexpr int kFlush = 4;
+constexpr float kNear = 4.f;                                               // value scales of a tile up to 2^4 apart are of one size
 constexpr int kPlanned = 448;                                              // sequences whose work is laid out in a line
 
 template <bool kTall, bool kCoded, bool kSplit>
@@ -120,7 +121,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
     float* s_qf = reinterpret_cast<float*>(smem + 13824);          // [128] factors of the rows that both streams have
     static_assert(768 + kPlanned * 4 <= 2560 && 2560 + kPlanned * sizeof(Seq) <= 9728 && 9728 + 4096 <= 13824 && 13824 + 512 <= Sh::kHead, "layout");
     float* s_scale = reinterpret_cast<float*>(smem + Sh::kHead);   // [stage][K 64, V 64]
-    float* s_vref = reinterpret_cast<float*>(smem + 520);          // [stage]: what the values' scales are relative to
+    // [stage]: what the part's value scales are relative to; log2 of the tile's largest, and of its smallest (zeros left out)
+    float *s_unit = reinterpret_cast<float*>(smem + 520), *s_top = reinterpret_cast<float*>(smem + 536), *s_low = reinterpret_cast<float*>(smem + 552);
     const int t = threadIdx.x, warp = __shfl_sync(0xffffffffu, t >> 5, 0), lane = t & 31;
     auto bar = [&](int i) { return bar0 + 8 * i; };
     auto wait = [&](int i, uint32_t parity) { mbar_wait_or_abort(bar(i), parity, flag); };
@@ -389,7 +391,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
             }
             lm::cp_async_commit();
         };
-        float vref = 0.f;                                          // warp 10: the largest value scale of the part so far, a power of two
+        float vunit = 1.f;                                         // warp 10: what the part's value scales are relative to
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) issue();
         while ((more || it_out < it_in) && !*abort_flag) {
@@ -399,17 +401,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
                 wait(Sh::kEmptyKV + st, lap_out);
                 const uint32_t from = sraw + raw_out * kTcRaw, to = skv + st * kTcStage;
                 if ((warp & 1) == 0) {
-                    // The scales, by whom copied them.  A value's is given relative to the largest one met so far in the part.
+                    // The scales, by whom copied them.  A value's is given relative to the size of the part's first.
                     const float* fs = reinterpret_cast<const float*>(smem + (from - bar0) + 2 * kTcKeys * kHd) + (warp - 8) * 32 + lane;
                     float s0 = fs[0], s1 = fs[32];
                     if (warp == 10) {
-                        if (opens >> (it_out & 31) & 1) vref = __uint_as_float(2u << 23);
-                        const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fabsf(s0), fabsf(s1)))));
-                        if (top > vref) vref = __uint_as_float(min((__float_as_uint(top) + 0x7FFFFFu) & 0x7F800000u, 252u << 23));
-                        const float inv = __uint_as_float((254u << 23) - __float_as_uint(vref));
+                        const uint32_t b0 = __float_as_uint(fabsf(s0)), b1 = __float_as_uint(fabsf(s1)), top = __reduce_max_sync(0xffffffffu, max(b0, b1));
+                        const uint32_t low = __reduce_min_sync(0xffffffffu, min(b0 - 1, b1 - 1)) + 1;   // (zeros wrap around)
+                        if (opens >> (it_out & 31) & 1) vunit = scale_unit(top);
+                        const float inv = __uint_as_float((254u << 23) - __float_as_uint(vunit));
                         s0 *= inv;
                         s1 *= inv;
-                        if (lane == 0) s_vref[st] = vref;
+                        if (lane == 0) {
+                            s_unit[st] = vunit;
+                            s_top[st] = scale_log2(__uint_as_float(top) * inv);
+                            s_low[st] = scale_log2(__uint_as_float(low) * inv);
+                        }
                     }
                     s_scale[st * 2 * kTcKeys + (warp - 8) * 32 + lane] = s0;
                     s_scale[st * 2 * kTcKeys + (warp - 8) * 32 + lane + 32] = s1;
@@ -548,7 +554,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
                 wait(Sh::kFullQ, nth & 1);
                 if (mine) qf = s_qf[rt];
             }
-            float m = -FLT_MAX, l = 0.f, vref = 1.f, m_kept = -FLT_MAX, v_kept = 1.f;
+            float m = -FLT_MAX, l = 0.f, vunit = 1.f, m_kept = -FLT_MAX;
             bool has_kept = false;
             const int tiles = p.t1 - p.t0, jobs = kTall ? tiles : (tiles + 1 - w) >> 1;
             auto walk = [&]() {                               // a tile on in the ring of stages
@@ -569,7 +575,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
                     if (kSplit && k > 0 && k % kFlush == 0) {                    // O so far to the sum; the next product starts afresh
                         wait(Sh::kDoneO + 2 * w + (b ^ 1), ((kk - 1) >> 1) & 1);
                         tc::tc_fence_after();
-                        const float f = has_kept ? lm::exp2_fast(m_kept - m) * (v_kept * __uint_as_float((254u << 23) - __float_as_uint(vref))) : 0.f;
+                        const float f = has_kept ? lm::exp2_fast(m_kept - m) : 0.f;
 #pragma unroll 1
                         for (int d = 0; d < kHd; d += 64) {                      // (half of it on its way at once: the latency of L2)
                             uint32_t o[64];
@@ -587,7 +593,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
                         }
                         has_kept = true;
                         m_kept = m;
-                        v_kept = vref;
                     }
                     uint32_t r[64];
                     tc::tmem_ld32(at, r);
@@ -614,15 +619,28 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
                     for (int i = 0; i < 64; i += 8)
 #pragma unroll
                         for (int d = 0; d < 4; ++d) mx[d] = fmaxf(fmaxf(mx[d], __uint_as_float(r[i + d])), __uint_as_float(r[i + 4 + d]));
-                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * qf;
-                    const float vnew = kCoded ? s_vref[st] : 1.f;
-                    if (__any_sync(0xffffffffu, top > m + kSlack || vnew != vref)) {
-                        const float to = fmaxf(m, top - kHead), e = lm::exp2_fast(m - to);
-                        const float f = kCoded && vnew != vref ? e * vref * __uint_as_float((254u << 23) - __float_as_uint(vnew)) : e;
+                    float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * qf;
+                    if (kCoded && k == 0) vunit = s_unit[st];
+                    // Codes: the row's largest score beside the tile's largest value scale, a bound that is near enough where the scales are of one size.
+                    const float bound = kCoded ? top + s_top[st] : top;
+                    if (__any_sync(0xffffffffu, bound > m + kSlack)) {
+                        top = bound;
+                        if (kCoded && s_top[st] - s_low[st] > kNear) {
+                            top = -INFINITY;
+#pragma unroll
+                            for (int i = 0; i < 64; i += 4) {
+                                const float4 f = *reinterpret_cast<const float4*>(vs + i);
+                                top = fmaxf(top, fmaxf(fmaxf(fmaf(__uint_as_float(r[i]), qf, scale_log2(f.x)), fmaf(__uint_as_float(r[i + 1]), qf, scale_log2(f.y))),
+                                                       fmaxf(fmaf(__uint_as_float(r[i + 2]), qf, scale_log2(f.z)), fmaf(__uint_as_float(r[i + 3]), qf, scale_log2(f.w)))));
+                            }
+                        }
+                        const float to = fmaxf(m, top - kHead);
+                        const float2 h = step<kCoded>(m, to);
+                        const float f = h.x * h.y;
+                        const bool moves = !kCoded || __any_sync(0xffffffffu, to > m);
                         m = to;
-                        vref = vnew;
-                        l *= e;
-                        if (kSplit ? k % kFlush != 0 : k > 0) {
+                        l = l * h.x * h.y;
+                        if (moves && (kSplit ? k % kFlush != 0 : k > 0)) {
                             wait(Sh::kDoneO + 2 * w + (b ^ 1), ((kk - 1) >> 1) & 1);   // O is complete up to the tile before
                             tc::tc_fence_after();
 #pragma unroll 1
@@ -683,7 +701,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
             tc::tc_fence_after();
             // kTall: a stream has its rows' results.  Otherwise both have a share of the same rows, O in the same lanes of tensor memory: with
             // the other's maximum, sum and scale, each joins half of the columns.
-            float top = m, c0 = kCoded ? vref : 1.f, c1 = 0.f, f0 = has_kept ? lm::exp2_fast(m_kept - m) * v_kept : 0.f, f1 = 0.f;
+            float top = m, c0 = vunit, c1 = 0.f, f0 = has_kept ? lm::exp2_fast(m_kept - m) * vunit : 0.f, f1 = 0.f;
             const bool other = ((tiles + w) >> 1) > 0;               // the other stream had a tile
             if (!kTall) {
                 s_ml[w * 128 + rt] = make_float4(m, l, c0, f0);
@@ -692,8 +710,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
                 tc::tc_fence_after();
                 const float4 ml = s_ml[(w ^ 1) * 128 + rt];
                 top = fmaxf(m, ml.x);
-                const float e0 = lm::exp2_fast(m - top), e1 = lm::exp2_fast(ml.x - top);
-                l = fmaf(l, e0, ml.y * e1);
+                const float2 h0 = step<kCoded>(m, top), h1 = step<kCoded>(ml.x, top);
+                const float e0 = h0.x * h0.y, e1 = h1.x * h1.y;
+                l = fmaf(l * h0.y, h0.x, ml.y * h1.x * h1.y);
                 c0 *= e0;
                 f0 *= e0;
                 c1 = ml.z * e1;
@@ -843,15 +862,18 @@ __global__ void __launch_bounds__(256) attend_tc_merge_kernel(const Args a) {
                 v[j][i] = x.x; v[j][i + 1] = x.y; v[j][i + 2] = x.z; v[j][i + 3] = x.w;
             }
         }
-        const float to = fmaxf(top, fmaxf(fmaxf(mt[0], mt[1]), fmaxf(mt[2], mt[3]))), f = lm::exp2_fast(top - to);
+        const float to = fmaxf(top, fmaxf(fmaxf(mt[0], mt[1]), fmaxf(mt[2], mt[3])));
+        const float2 h = step<true>(top, to);
+        const float f = h.x * h.y;
         top = to;
-        sum *= f;
+        sum = sum * h.x * h.y;
 #pragma unroll
         for (int i = 0; i < 8; ++i) acc[i] *= f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float e = lm::exp2_fast(mt[j] - to);
-            sum = fmaf(lt[j], e, sum);
+            const float2 h = step<true>(mt[j], to);
+            const float e = h.x * h.y;
+            sum = fmaf(lt[j] * h.y, h.x, sum);
 #pragma unroll
             for (int i = 0; i < 8; ++i) acc[i] = fmaf(v[j][i], e, acc[i]);
         }

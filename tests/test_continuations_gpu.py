@@ -326,6 +326,38 @@ def test_attention_value_scales_of_all_sizes(cuda):
 
 
 @BOTH
+@pytest.mark.parametrize("M, T, nq, nkv, top", [(2, 5, 32, 8, 300), (1, 4, 4, 4, 40), (2, 64, 32, 8, 700), (2, 20, 8, 8, 1500), (3, 64, 32, 4, 5000)])
+@pytest.mark.parametrize("weighed", [False, True], ids=["hidden", "light"])
+def test_attention_value_scales_that_a_row_does_not_weigh(cuda, M, T, nq, nkv, top, act, weighed):
+    """Value scales 2^25 times the others', of nodes that other branches do not see, or of positions whose probability is nothing: the rows keep
+    their precision, held to the values that they weigh themselves."""
+    g = torch.Generator("cuda").manual_seed(T)
+    st = Store(g, M, 1, nkv, top + T, True)
+    masks = [[1 << i | (1 if i % 3 == 0 else 0) | (2 if i == T - 1 else 0) for i in range(T)] for _ in range(M)]
+    first = [top - 3 * m for m in range(M)]
+    for m in range(M):
+        st.vs[m, :, :, first[m] + 1] *= 2.0 ** 25
+        if weighed:
+            for at in (0, 9, top // 2, first[m] - 1):   # scores of some 60 either way
+                st.ks[m, :, :, at] = 0.4
+                st.vs[m, :, :, at] *= 2.0 ** 25
+    check_attention(M, T, nq, nkv, first, top + T, True, act, masks=masks, store=st)
+
+
+@BOTH
+def test_attention_value_scales_that_fall_and_end(cuda, act):
+    """Value scales that fall by 2^60 along the context, rows of scale -0 and stretches of scale zero at its start, inside and at its end."""
+    for T in (3, 64):
+        st = Store(torch.Generator("cuda").manual_seed(T), 2, 1, 4, 900, True)
+        st.vs *= 2.0 ** torch.linspace(20, -40, 900, device="cuda")
+        st.vs[..., :70] = 0
+        st.vs[..., 300:450] = -0.0
+        st.vs[..., 5::11] = -0.0
+        st.vs[0, ..., 760:] = 0
+        check_attention(2, T, 16, 4, [800, 830], 900, True, act, store=st)
+
+
+@BOTH
 @CACHES
 @pytest.mark.parametrize("M, T, nq, nkv, top", [(40, 9, 32, 8, 1500), (20, 64, 32, 8, 1200), (23, 13, 28, 4, 2050), (80, 3, 24, 8, 700), (460, 2, 20, 1, 300), (90, 40, 32, 8, 130)])
 def test_attention_many_tiles_of_a_block(cuda, M, T, nq, nkv, top, coded, act):
