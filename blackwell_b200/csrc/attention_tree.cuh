@@ -113,15 +113,6 @@ __device__ __forceinline__ float4 ld_dsmem4(uint32_t addr, uint32_t rank) {
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(ra) : "memory");
     return v;
 }
-__device__ __forceinline__ float4 load_q4(const float* p) { return *reinterpret_cast<const float4*>(p); }
-__device__ __forceinline__ float4 load_q4(const __nv_bfloat16* p) {
-    const uint2 u = *reinterpret_cast<const uint2*>(p);
-    return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u), __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xFFFF0000u));
-}
-__device__ __forceinline__ void store_o4(float* p, const float4& v) { *reinterpret_cast<float4*>(p) = v; }
-__device__ __forceinline__ void store_o4(__nv_bfloat16* p, const float4& v) {
-    *reinterpret_cast<uint2*>(p) = make_uint2(lm::pack_bf16(v.x, v.y), lm::pack_bf16(v.z, v.w));
-}
 // Power of two at or below |x| (1 for zero and what has no such), and its reciprocal.
 __device__ __forceinline__ float2 binade(float x) {
     uint32_t e = __float_as_uint(x) >> 23 & 255;
@@ -234,7 +225,7 @@ __global__ void __launch_bounds__(Shape<NT, kCoded>::kWarps * 32, 2) attend_kern
         float4 x[8];
         float top = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = in ? load_q4(q + 16 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = 0; i < 8; ++i) x[i] = in ? lm::load4(q + 16 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = fmaxf(top, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -537,7 +528,7 @@ __global__ void __launch_bounds__(Shape<NT, kCoded>::kWarps * 32, 2) attend_kern
         if (groups == 1) {
             const float inv = sum == 0.f ? 0.f : 1.f / sum;   // a row that sees nothing: 0
             A* out = static_cast<A*>(a.out) + (((size_t)m * a.T + node) * a.nq + head * a.group + row - node * a.group) * kHd + 4 * lane;
-            store_o4(out, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+            lm::store4(out, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
         } else {
             float* rec = a.part + ((((size_t)m * a.c.heads + head) * a.rows + row) * groups + grp) * kPart;
             *reinterpret_cast<float4*>(rec + 4 * lane) = acc;
@@ -614,7 +605,7 @@ __global__ void __launch_bounds__(128) attend_merge_kernel(const Args a) {
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     A* out = static_cast<A*>(a.out) + (((size_t)m * a.T + node) * a.nq + head * a.group + row - node * a.group) * kHd + 4 * lane;
-    store_o4(out, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+    lm::store4(out, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
 }
 
 }  // namespace tree

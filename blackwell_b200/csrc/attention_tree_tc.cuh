@@ -888,7 +888,7 @@ __global__ void __launch_bounds__(256) attend_tc_merge_kernel(const Args a) {
         const int r = r0 + 2 * warp + (lane >> 4) + 16 * i;
         if (r >= rows) break;
         const uint32_t node = (uint32_t)r / (uint32_t)a.group;
-        store_o4(static_cast<A*>(a.out) + (((size_t)m * a.T + node) * a.nq + head * a.group + r - node * a.group) * kHd + c0 + 4 * (lane & 15),
+        lm::store4(static_cast<A*>(a.out) + (((size_t)m * a.T + node) * a.nq + head * a.group + r - node * a.group) * kHd + c0 + 4 * (lane & 15),
                  *reinterpret_cast<const float4*>(&s_out[r - r0][4 * (lane & 15)]));
     }
 }

@@ -21,15 +21,6 @@ struct WriteArgs {
     int nq, M, T;
     float eps;
 };
-__device__ __forceinline__ float4 load_act4(const float* p) { return *reinterpret_cast<const float4*>(p); }
-__device__ __forceinline__ float4 load_act4(const __nv_bfloat16* p) {
-    const uint2 u = *reinterpret_cast<const uint2*>(p);
-    return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u), __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xFFFF0000u));
-}
-__device__ __forceinline__ void store_act4(float* p, const float4& v) { *reinterpret_cast<float4*>(p) = v; }
-__device__ __forceinline__ void store_act4(__nv_bfloat16* p, const float4& v) {
-    *reinterpret_cast<uint2*>(p) = make_uint2(lm::pack_bf16(v.x, v.y), lm::pack_bf16(v.z, v.w));
-}
 // base^(-2i/128) / 2 pi, i = 0..63: turns per position, as fractions of 2^64.  A position times one of them, modulo 2^64, is the angle to 2^-64 turns
 // a position, whatever the position: in 32-bit floating point it would be off by position * 2^-24, visible from some thousand positions on.
 struct Turns {
@@ -67,7 +58,7 @@ __global__ void __launch_bounds__(kWriteWarps * 32, 3) write_rows_kernel(const W
     const A* x = static_cast<const A*>(a.qkv) + (at * heads + h0) * kHd + 4 * lane;
     float4 v[HW];
 #pragma unroll
-    for (int j = 0; j < HW; ++j) v[j] = h0 + j < heads ? load_act4(x + j * kHd) : make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int j = 0; j < HW; ++j) v[j] = h0 + j < heads ? lm::load4(x + j * kHd) : make_float4(0.f, 0.f, 0.f, 0.f);
     const int turned = a.nq + a.c.heads;                // heads that are normed and turned
     for (int e = threadIdx.x; e < kHd / 2; e += blockDim.x)
         s_turn[e] = turn_of((long long)first + (a.offset ? a.offset[at] : i), turns.f[e]);
@@ -105,7 +96,7 @@ __global__ void __launch_bounds__(kWriteWarps * 32, 3) write_rows_kernel(const W
         if (h >= heads) break;
         const float4 y = v[j];
         if (h < a.nq) {
-            store_act4(static_cast<A*>(a.q_out) + (at * a.nq + h) * kHd + 4 * lane, y);
+            lm::store4(static_cast<A*>(a.q_out) + (at * a.nq + h) * kHd + 4 * lane, y);
             continue;
         }
         if (row >= a.c.max_seq) continue;               // a row outside of the cache is never written
