@@ -410,6 +410,35 @@ def test_attention_scratch_of_the_size_given(cuda, M, T, nq, nkv, top, act):
     check_attention(M, T, nq, nkv, [top - 17 * m for m in range(M)], top + T, True, act, call=call)
 
 
+@CACHES
+@pytest.mark.parametrize("M, T, nq, nkv, top", [(2, 1, 8, 2, 40000), (1, 3, 28, 4, 33000), (1, 40, 8, 2, 40000), (1, 64, 16, 2, 20000)])
+def test_attention_root_mean_square_of_long_contexts(cuda, M, T, nq, nkv, top, coded):
+    """The largest error may grow with the number of sums; the root mean square hardly does, and shows a probability of fewer bits."""
+    g = torch.Generator("cuda").manual_seed(T)
+    k, group = kernels(), nq // nkv
+    st = Store(g, M, 1, nkv, top + T, coded)
+    q = torch.empty((M, T, nq, HD), device="cuda").normal_(generator=g)
+    kk, vv = st.value()
+    s = torch.einsum("mihgd,mhtd->mhigt", q.double().view(M, T, nkv, group, HD), kk) / math.sqrt(HD)
+    size = float(torch.einsum("mihgd,mhtd->mhigt", q.abs().view(M, T, nkv, group, HD), kk.abs().float()).amax()) / math.sqrt(HD)
+    s.masked_fill_((torch.arange(top + T, device="cuda") > top + torch.arange(T, device="cuda")[:, None])[:, None], -math.inf)
+    want = torch.einsum("mhigt,mhtd->mihgd", torch.softmax(s, -1), vv).reshape(M, T, nq, HD)
+    del s
+    try:
+        for route in (0, 1, 2):
+            k.set_tuning(25, route)
+            out = torch.zeros_like(q)
+            scratch = torch.empty(k.attention_tree_scratch_bytes(M, T, nq, nkv, top + T), dtype=torch.uint8, device="cuda")
+            k.attention_tree(out, q, st.args(), ints([top] * M), None, None, 0, nq, M, T, scratch)
+            # A probability is off by 2^-20 and, twice, by what its score is (2^-21 of sum |q k| / sqrt(128)); rounded sums of 16 positions walk: sqrt(n / 16)
+            # steps of 2^-23.  P in 11 bits alone would be 2^-12 / sqrt(3) = 1.4e-4.
+            bar = 2.0 ** -20 * (1 + size) + math.sqrt(top / 16) * 2.0 ** -23
+            off = float((out.double() - want).square().mean().sqrt() / want.square().mean().sqrt())
+            assert off <= bar and bar < 5e-5, (route, off, bar)
+    finally:
+        k.set_tuning(25, 0)
+
+
 def test_attention_far_offsets(cuda):
     """Sequences whose rows lie beyond 2^32 bytes and elements."""
     g = torch.Generator("cuda").manual_seed(4)
