@@ -135,9 +135,9 @@ __device__ __noinline__ int first_of_equal(uint32_t at0, uint32_t at1, int in, c
     };
     const uint32_t beam0 = in & 1 ? at0 / vocab : 0xFFFFFFFFu, beam1 = in & 2 ? at1 / vocab : 0xFFFFFFFFu;
     const uint32_t beam = __reduce_min_sync(0xffffffffu, min(beam0, beam1));
-    const uint32_t v0 = beam0 == beam ? logit(at0) : 0, v1 = beam1 == beam ? logit(at1) : 0;     // (order32 of a finite number is not 0)
+    const uint32_t v0 = beam0 == beam ? logit(at0) : 0, v1 = beam1 == beam ? logit(at1) : 0;     // (an ended beam's one may have any bits)
     const uint32_t v = __reduce_max_sync(0xffffffffu, max(v0, v1));
-    const uint32_t c0 = v0 == v ? at0 : 0xFFFFFFFFu, c1 = v1 == v ? at1 : 0xFFFFFFFFu;
+    const uint32_t c0 = beam0 == beam && v0 == v ? at0 : 0xFFFFFFFFu, c1 = beam1 == beam && v1 == v ? at1 : 0xFFFFFFFFu;
     const uint32_t at = __reduce_min_sync(0xffffffffu, min(c0, c1));
     return c0 == at ? 4 : c1 == at ? 5 : 0;
 }

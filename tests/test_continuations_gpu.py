@@ -610,6 +610,16 @@ def test_select_scores_of_both_zeros(cuda):
     check_select(logits, score, torch.ones((1, 3), dtype=torch.uint8, device="cuda"), 7, 1, 1, 3)
 
 
+@pytest.mark.parametrize("V", [60, 20000])
+def test_select_equal_scores_of_ended_beams_whose_logits_are_nothing(cuda, V):
+    """Beams that have ended with the same score: their logits are not looked at, whatever their bits."""
+    logits = torch.empty((4, V), device="cuda").normal_(generator=torch.Generator("cuda").manual_seed(V))
+    logits[1:3].view(torch.int32).fill_(-1)             # NaN with every bit set
+    score = torch.tensor([[-40.0, -1.5, -1.5, -60.0]], device="cuda")
+    for keep in (1, 2, 4, 9):
+        check_select(logits, score, torch.tensor([[0, 1, 1, 0]], dtype=torch.uint8, device="cuda"), 7, keep, 1, 4)
+
+
 @pytest.mark.parametrize("B, V, keep", [(1, 300, 5), (2, 30000, 6), (1, 200000, 40), (8, 151643, 8), (16, 40000, 20)])
 def test_select_logits_closer_than_their_scores(cuda, B, V, keep):
     """Scores that fall together in 64 bits: within a beam the larger logit first, wherever in the row; equal logits by token."""
