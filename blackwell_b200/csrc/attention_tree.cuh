@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(Shape<NT, kCoded>::kWarps * 32, 2) attend_kern
             }
             if (kCoded) {
                 const bool in = there(p0 + (lane & (kTile - 1)));
-                cp_async4z(to + 2 * Sh::kSide + lane * 4, scale + (in ? p0 : 0), in);
+                cp_async4z(to + 2 * Sh::kSide + lane * 4, scale + (in ? p0 : -(lane & (kTile - 1))), in);   // (the head's first row: in the cache, however short)
             }
         }
     };
