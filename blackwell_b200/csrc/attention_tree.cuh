@@ -39,7 +39,7 @@ constexpr int kMaxNodes = 64;
 constexpr int kTile = 16;               // positions a warp takes at once
 constexpr int kPart = kHd + 4;          // floats of a partial record: outputs, maximum, sum, padding
 constexpr float kHead = 6.f, kSlack = 14.f;   // P up to 2^6 when the maximum is new, 2^14 before it is moved
-constexpr float kLeastScale = -66.f;    // log2; a smaller value scale counts as this one in the reference: sums of P without it stay below 2^80 a position
+constexpr float kLeastScale = -90.f;    // log2; a smaller value scale counts as this one in the reference: sums of P without it stay below 2^104 a position
 
 struct Args {
     void* out;                          // [M * T][nq * 128]

@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
     float* s_qf = reinterpret_cast<float*>(smem + 13824);          // [128] factors of the rows that both streams have
     static_assert(768 + kPlanned * 4 <= 2560 && 2560 + kPlanned * sizeof(Seq) <= 9728 && 9728 + 4096 <= 13824 && 13824 + 512 <= Sh::kHead, "layout");
     float* s_scale = reinterpret_cast<float*>(smem + Sh::kHead);   // [stage][K 64, V 64]
-    // [stage]: what the part's value scales are relative to; log2 of the tile's largest, and of its smallest (zeros left out)
+    // [stage]: what the part's value scales are relative to; log2 of the tile's largest, and of its smallest
     float *s_unit = reinterpret_cast<float*>(smem + 520), *s_top = reinterpret_cast<float*>(smem + 536), *s_low = reinterpret_cast<float*>(smem + 552);
     const int t = threadIdx.x, warp = __shfl_sync(0xffffffffu, t >> 5, 0), lane = t & 31;
     auto bar = [&](int i) { return bar0 + 8 * i; };
@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const Args a) 
                     float s0 = fs[0], s1 = fs[32];
                     if (warp == 10) {
                         const uint32_t b0 = __float_as_uint(fabsf(s0)), b1 = __float_as_uint(fabsf(s1)), top = __reduce_max_sync(0xffffffffu, max(b0, b1));
-                        const uint32_t low = __reduce_min_sync(0xffffffffu, min(b0 - 1, b1 - 1)) + 1;   // (zeros wrap around)
+                        const uint32_t low = __reduce_min_sync(0xffffffffu, min(b0, b1));   // (0 in a tile with rows that nobody sees, too)
                         if (opens >> (it_out & 31) & 1) vunit = scale_unit(top);
                         const float inv = __uint_as_float((254u << 23) - __float_as_uint(vunit));
                         s0 *= inv;

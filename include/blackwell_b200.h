@@ -325,7 +325,7 @@ int bw_qk_norm_rope_kv_rows(void* q_out, const bw_kv_cache* cache, const void* q
  * i >= count[m] (NULL: T) do not exist: nobody sees them and their outputs are left as they were, as are those of a sequence with
  * first[m] < 0.  Rows at or beyond max_seq are not seen.  A node that sees nothing gets zeros.  Cached rows that no node of the sequence sees may
  * hold anything; the others must be finite.  Probability * value scale is kept to 22 bits (11 with bf16) of the largest that a node has: what it does
- * not see or hardly weighs takes none of them.  num_q_heads is any multiple of the cache's heads.  ctx_hint is a bound on
+ * not see or hardly weighs takes none of them (what weighs less than 2^-100 of the whole counts for nothing).  num_q_heads is any multiple of the cache's heads.  ctx_hint is a bound on
  * first[m] + T that sizes the splits (0: max_seq); longer sequences are still right.  scratch: bw_attention_tree_scratch_bytes, with the largest
  * sizes in use. */
 int bw_attention_tree(void* out, const void* q, const bw_kv_cache* cache, const int* d_first_row, const unsigned long long* d_mask_or_null,

@@ -358,6 +358,42 @@ def test_attention_value_scales_that_fall_and_end(cuda, act):
 
 
 @BOTH
+@pytest.mark.parametrize("M, T, nq, nkv, top", [(10, 1, 28, 4, 7), (5, 14, 48, 3, 2), (6, 7, 48, 3, 39), (2, 40, 20, 1, 700)])
+def test_attention_value_scales_of_zero_where_the_scores_are_largest(cuda, M, T, nq, nkv, top, act):
+    """Rows whose values are zero take the probability, but no bits of the others' products."""
+    g = torch.Generator("cuda").manual_seed(top)
+    k, group = kernels(), nq // nkv
+    st = Store(g, M, 1, nkv, top + T, True)
+    st.vs[..., ::3] = 0
+    st.ks[..., ::3] *= 8                               # scores of some 40 either way
+    q = (torch.empty((M, T, nq, HD), device="cuda").normal_(generator=g) * 1.5).to(act)
+    kk, vv = st.value()
+    x = q.double().view(M, T, nkv, group, HD)
+    hide = (torch.arange(top + T, device="cuda") > top + torch.arange(T, device="cuda")[:, None])[:, None]
+    s = (torch.einsum("mihgd,mhtd->mhigt", x, kk) / math.sqrt(HD)).masked_fill(hide, -math.inf)
+    size = (torch.einsum("mihgd,mhtd->mhigt", x.abs(), kk.abs()) / math.sqrt(HD)).masked_fill(hide, 0).amax(-1, keepdim=True)
+    p = torch.softmax(s, -1)
+    want, weight = [torch.einsum("mhigt,mhtd->mhigd", p, v) for v in (vv, vv.abs())]
+    # As in one_attention: a score is off by 2^-21 of sum |q k| / sqrt(128), a probability by that, by its rounding (2^-21 / 2^-12) and, where the references are
+    # some 100 apart, by that of their difference (2^-18); sums of 16 products at a time.  A scale of zero counts as 2^-90: f16 steps of 2^-24 are then
+    # 2^-114 of the largest probability, over fewer than 2^10 positions 2^-104.
+    fine = 2.0 ** -12 if act == torch.bfloat16 else 2.0 ** -21
+    bar = (2 * 2.0 ** -21 * size + 2 * fine + 2.0 ** -18 + ((top + T) / 16 + 64) * 2.0 ** -23) * weight.amax(-1, keepdim=True) + 2.0 ** -104 * vv.abs().amax()
+    if act == torch.bfloat16:
+        bar = bar + want.abs() * 2.0 ** -8
+    try:
+        for route in (0, 1, 2):
+            k.set_tuning(25, route)
+            out = torch.zeros_like(q)
+            scratch = torch.empty(k.attention_tree_scratch_bytes(M, T, nq, nkv, top + T), dtype=torch.uint8, device="cuda")
+            k.attention_tree(out, q, st.args(), ints([top] * M), None, None, 0, nq, M, T, scratch)
+            got = out.double().view(M, T, nkv, group, HD).permute(0, 2, 1, 3, 4)
+            assert ((got - want).abs() <= bar).all(), (route, float(((got - want).abs() / bar).max()))
+    finally:
+        k.set_tuning(25, 0)
+
+
+@BOTH
 @CACHES
 @pytest.mark.parametrize("M, T, nq, nkv, top", [(40, 9, 32, 8, 1500), (20, 64, 32, 8, 1200), (23, 13, 28, 4, 2050), (80, 3, 24, 8, 700), (460, 2, 20, 1, 300), (90, 40, 32, 8, 130)])
 def test_attention_many_tiles_of_a_block(cuda, M, T, nq, nkv, top, coded, act):
