@@ -359,8 +359,9 @@ __global__ void __launch_bounds__(Shape<NT, kCoded>::kWarps * 32, 2) attend_kern
                     s[j][e] = yes ? s[j][e] : -INFINITY;
                 }
         }
-        // Codes: a score is compared beside a cap of the value scales that the lane multiplies with, set anew (to four times the present one) when
-        // one exceeds it or the reference moves.
+        // Codes: a score is compared beside a cap of the value scales that the lane multiplies with, set anew when one exceeds it or the reference
+        // moves: to four times the present one or more, at most 2^8 times (2^(kSlack - kHead): a cap up to there hardly moves a reference in vain;
+        // scales up to 2^8 apart cost 1 to 2 %, where a cap of four times the last one cost 8 to 16).
         bool move = kCoded && fmaxf(fabsf(sc[2]), fabsf(sc[3])) > vcap;
 #pragma unroll
         for (int j = 0; j < NT; ++j)
@@ -374,7 +375,7 @@ __global__ void __launch_bounds__(Shape<NT, kCoded>::kWarps * 32, 2) attend_kern
                 const float vdiv = __uint_as_float((254u << 23) - __float_as_uint(vunit));
                 lg[0] = scale_log2(sc[2] * vdiv);
                 lg[1] = scale_log2(sc[3] * vdiv);
-                vcap = 4.f * top;
+                vcap = fmaxf(4.f * top, fminf(vcap, 256.f * top));
                 slack = kSlack - scale_log2(vcap * vdiv);
             }
 #pragma unroll
