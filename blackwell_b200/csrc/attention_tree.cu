@@ -116,7 +116,9 @@ static cudaError_t launch_tc_rows(const Args& a, cudaStream_t st) {
 // tile of the mma.sync kernel (32 rows, 16 positions) takes a block 0.4 us.  So: by the tiles that an SM gets.  One or two row tiles leave the 128
 // lanes of an accumulator half empty, the more so the more heads there are to begin with.  Measured (us, mma.sync / tcgen05; 32 / 8 heads, fp32, 8 bits): 64
 // nodes, 8 x 2,048 positions 152 / 60, 4 x 1,000 40 / 32, 4 x 300 20 / 28; 24 nodes, 8 x 2,048 55 / 39, 4 x 1,000 22 / 26; 16 nodes, 32 x 1,000 67 / 70,
-// 8 x 5,310 83 / 63; 10 nodes, 8 x 1,300 29 / 30, 8 x 3,000 53 / 43, 32 x 400 35 / 46; 8 nodes, 32 x 4,000 117 / 148.
+// 8 x 5,310 83 / 63; 10 nodes, 8 x 1,300 29 / 30, 8 x 3,000 53 / 43, 32 x 400 35 / 46; 8 nodes, 32 x 4,000 119 / 148.  More than 64 rows: contexts of up to
+// two tiles stay whole in a block, without records and merge (64 nodes, 8 x 60 positions 25 / 16, 16 x 60 46 / 16), longer ones are laid in a line (8 x 100
+// 28 / 31, 8 x 200 31 / 32, 8 x 300 36 / 34, 16 x 128 51 / 39, 4 x 128 16 / 28, 4 x 600 29 / 30): the step from 16 to 80 tiles.
 static bool many_rows(long heads, int rows, int ctx, int sms) {
     if (rows <= kFewRows) return false;
     const double tiles = (double)heads * ((rows + 31) / 32) * ((ctx + 15) / 16) / sms;

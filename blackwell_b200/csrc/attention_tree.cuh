@@ -17,11 +17,12 @@
 // of two first.
 // The running maximum moves only when a score exceeds the reference by more than 2^14 / 2^6: otherwise no lane needs another's score.  The
 // tensor core's sums are cut at 24 bits: with fp32 activations a tile's P V starts at zero and is added to O by a rounded addition.
-// Measured (32 / 8 heads, fp32, 8 bits): 32 sequences of 4,096 to 8,192 positions 75 us, 5.6 TB/s; 8 of 2,000 to 4,000 15 us; one of 2,048 6.6 us, most
+// Measured (32 / 8 heads, fp32, 8 bits): 32 sequences of 4,096 to 8,192 positions 75 us, 5.6 TB/s; 8 of 2,000 to 4,000 15 us; one of 2,048 6.7 us, most
 // of it the chain of a launch, the position, the first tile from memory and the merge inside the cluster.  What it took: the scales with the tiles by
 // cp.async (loaded to registers a tile ahead: 92 us), queries brought to their place once per block (by every warp: + 2,000 cycles), and the remainders in
-// the idle columns (8 us at 32 sequences).  Trees of up to 32 rows a head are bound by mma.sync, whose rate is a sixth of
-// tcgen05's: 4 of 8 nodes over 1,000 positions, 28 / 4 heads, binary16, 13.9 us.  Tried and not kept: an equal stretch of all contexts per block with records
+// the idle columns (8 us at 32 sequences).  Trees of 17 to 32 rows a head have two warps per scheduler (255 registers).  32 of 8 nodes over 2,000 to 4,000
+// positions, 8 bits: 119 us in fp32, 83 in bf16, the tensor pipe at 38 % and issue at 36: the waits between dependent instructions, then mma.sync itself.  4 of
+// 8 nodes over 1,000 positions, 28 / 4 heads, binary16: 13.9 us, tensor pipe 9 %, issue 20 %: start, barriers and the chain of two tiles a warp.  Tried and not kept: an equal stretch of all contexts per block with records
 // and a merge (10 us more below 16,000 positions, as much beyond).
 #pragma once
 #include <float.h>

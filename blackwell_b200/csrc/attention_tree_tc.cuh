@@ -10,12 +10,12 @@
 //   O += P V     P over the scores' columns as the f16 A operand, V from shared memory as it lies there ([position][column])
 // fp32 activations: Q and P as f16 high parts and remainders, multiplied one after the other.  The accumulator's sums are cut, not rounded, at
 // 24 bits, which adds up: so the remainders of a score come first, and O is added to a sum in the scratch memory (L2) every four tiles and
-// starts afresh (64 nodes over 5,279 positions: error 1.1e-6 of the result, as that of 32-bit sums; every eight tiles 2.3e-6 and a tenth faster).
+// starts afresh (57 nodes over 5,279 positions: error 1.1e-6 of the result, as that of 32-bit sums; every eight tiles 2.3e-6 and a tenth faster).
 // Scales and the moving reference as in attention_tree.cuh (scales relative to the size of a part's first); a warp brings its rows of O to a new one by itself.
 // Work is shared out in tiles of 64 positions: all sequences' tiles, heads and row groups in one line, an equal stretch of it per block; what
 // a block has of a head's context that it does not have whole goes to a record that the merge kernel joins.
 // All waits are bounded; a wait that gives up raises an abort flag.
-// Measured (8 trees of 64 nodes over 2,000 to 4,096 positions, 32 / 8 heads, 8 bits): bf16 58 us, 0.43 PFLOP/s, fp32 90.  Of a block's 85,000 cycles a
+// Measured (8 trees of 64 nodes over 2,000 to 4,096 positions, 32 / 8 heads, 8 bits): bf16 57 us, 0.43 PFLOP/s, fp32 92.5.  Of a block's 85,000 cycles a
 // tile takes 2,600, the softmax of a stream that long from one tile to the next (scores out of tensor memory 250, scales and maximum 600, exponentials 1,200;
 // the units' own rates would allow 1,100, the rest is latency of one warp per scheduler and stream); the start 4,000, and each of two parts 10,000 to
 // 12,000 for the queries' place, the first scores and the record of 128 KB (stored a column at a time it took 5,000).  The merge takes 5 us.  Tried and not kept: maximum and exponentials in

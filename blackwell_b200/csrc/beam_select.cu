@@ -8,8 +8,9 @@
 // each other: a stale one lowers the bar.  A list that has grown is cut to its best.  The second launch, a block per request, forms the rows' log-sums and ranks the
 // stretches' candidates across the beams, scores in 64 bits: two beams' candidates may lie closer to each other than 32 bits tell apart.
 // The exponentials and their sums are 32-bit, taken of differences that are exact where they matter; a log-sum is right to some 1e-7.
-// Measured (16 x 8 beams of 151,643 tokens, 78 MB): 23.9 us, 3.2 TB/s, of which the merge and its launch are 4; the first launch alone is bound
-// by the instructions that a value takes, not by memory (the exponentials some 5 us of it).
+// Measured (16 x 8 beams of 151,643 tokens, 78 MB): 24.4 us, 3.2 TB/s, of which the merge and its launch are 4; the first launch alone is bound
+// by the instructions that a value takes, not by memory (the exponentials some 5 us of it).  One request of 8 or 16 such beams, whose 2,432 or 8,192
+// candidates do not fit shared memory: 12.6 and 20.4 us.
 #include <float.h>
 
 #include <mutex>
@@ -436,8 +437,8 @@ __global__ void __launch_bounds__(kThreads, 4) chunk_kernel(const Args a) {
 }
 
 // Stretches of a row: whole turns, four blocks per SM where that many are to be had.  A few requests that a cluster each reads in three turns or fewer:
-// one launch.  On the device both take much the same (1 x 4 beams of 32,768 tokens 7.1 us, in two launches 6.4), but a launch costs the caller 2 us:
-// calls in a row take 9 instead of 11.  skew: elements that rows may start behind a 16-byte boundary.
+// one launch.  On the device both take much the same (1 x 4 beams of 32,768 tokens 7.2 us, in two launches 6.4), but a launch costs the caller 2 us:
+// calls in a row took 9 instead of 11.  skew: elements that rows may start behind a 16-byte boundary.
 constexpr int kFusedBlocks = 16, kFusedTurns = 3;
 static bool stretches(int vocab, int skew, int beams, long rows, int sms, Args* a) {
     const int vectors = (vocab + skew + 3) / 4, turns = (vectors + kTurn - 1) / kTurn;

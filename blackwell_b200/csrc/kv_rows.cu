@@ -21,8 +21,8 @@ struct WriteArgs {
     int nq, M, T;
     float eps;
 };
-// base^(-2i/128) / 2 pi, i = 0..63: turns per position, as fractions of 2^64.  A position times one of them, modulo 2^64, is the angle to 2^-64 turns
-// a position, whatever the position: in 32-bit floating point it would be off by position * 2^-24, visible from some thousand positions on.
+// base^(-2i/128) / 2 pi, i = 0..63: turns per position, as fractions of 2^64, right to 2^-55 (53-bit products on the host).  A position times one of them,
+// modulo 2^64, is the angle to position * 2^-55 turns: in 32-bit floating point it would be off by position * 2^-24, visible from some thousand positions on.
 struct Turns {
     unsigned long long f[kHd / 2];
 };
@@ -126,7 +126,7 @@ static cudaError_t write_launch(const WriteArgs& a, const Turns& turns, cudaStre
     const int heads = a.nq + 2 * a.c.heads;
     const long rows = (long)a.M * a.T;
     // A block has a row, or part of its heads.  Few rows: a head per warp and two warps per block, everything is latency.  Many: four heads per
-    // warp.  Measured (8 x 512 rows, 32 / 8 heads, fp32 to 8 bits, 176 MB): 32.0 us, 5.5 TB/s; with the angles formed by every warp 34.3, in 64-bit
+    // warp.  Measured (8 x 512 rows, 32 / 8 heads, fp32 to 8 bits, 176 MB): 32.2 us, 5.5 TB/s; with the angles formed by every warp 34.3, in 64-bit
     // floating point 37.6; eight heads per warp leave too few warps (44).
     const bool many = rows * heads > 32L * sm_count(current_device());
     const int per_row = many ? (heads + 3) / 4 : heads, warps = many ? (per_row < kWriteWarps ? per_row : kWriteWarps) : 2;
@@ -149,7 +149,7 @@ constexpr int kMaxBeams = 32, kMaxPath = 64;
 
 // Sequence m * beams + b takes the rows [from, to) of m * beams + parent[b].  A thread owns 16 bytes of a row (and the row's scale,
 // the first of them) in all beams of a group: it reads what every changed beam gets, then writes, so that parents may change too.  Bound by
-// memory: 32 beams of 1,500 binary16 rows, 6 layers, 8 heads, 1.5 GB read and written: 231 us, 6.4 TB/s.
+// memory: 32 beams of 1,500 binary16 rows, 6 layers, 8 heads, 1.5 GB read and written: 232 us, 6.4 TB/s.
 template <int NB>
 __global__ void __launch_bounds__(256) reorder_kernel(const MoveArgs a) {
     pdl_trigger();
