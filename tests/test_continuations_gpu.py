@@ -876,6 +876,68 @@ def test_beams_share_a_prompt_and_part(cuda):
     del again
 
 
+@CACHES
+@pytest.mark.parametrize("T, nq", [(3, 8), (40, 32)])
+def test_whole_steps_captured_and_replayed(cuda, T, nq, coded):
+    """A tree's step (rows, attention, accepted path) and a beam's (selection, reordering, rows, attention) in one graph, replayed with other positions,
+    masks, paths and logits: the bits of the same calls one after the other."""
+    g = torch.Generator("cuda").manual_seed(T)
+    k, M, B, L, nkv, top, V = kernels(), 2, 3, 2, 4, 500, 3000
+    a, b = Store(g, M * B, L, nkv, top, coded), Store(g, M * B, L, nkv, top, coded)
+    for x, y in zip((a.k, a.v) + ((a.ks, a.vs) if coded else ()), (b.k, b.v) + ((b.ks, b.vs) if coded else ())):
+        y.copy_(x)
+    N = M * B
+    tree, token = torch.empty((N, T, nq + 2 * nkv, HD), device="cuda"), torch.empty((N, 1, nq + 2 * nkv, HD), device="cuda")
+    logits, first, offset = torch.empty((N, V), device="cuda"), ints([0] * N), torch.zeros((N, T), dtype=torch.int32, device="cuda")
+    mask, path, count, lo = torch.zeros((N, T), dtype=torch.int64, device="cuda"), torch.zeros((N, T), dtype=torch.int32, device="cuda"), ints([0] * N), ints([0] * M)
+    hi, score0 = ints([0] * M), torch.zeros((M, B), device="cuda")
+
+    def buffers():
+        one = lambda *s, dtype=torch.float32: torch.zeros(s, dtype=dtype, device="cuda")  # noqa: E731
+        return dict(q=one(N, T, nq, HD), o=one(N, T, nq, HD), q1=one(N, 1, nq, HD), o1=one(N, 1, nq, HD), parent=one(M, B, dtype=torch.int32), token=one(M, B, dtype=torch.int32),
+                    score=one(M, B), w=one(k.attention_tree_scratch_bytes(N, T, nq, nkv, top), dtype=torch.uint8), w2=one(k.beam_select_scratch_bytes(V, B, B, M), dtype=torch.uint8))
+
+    def step(st, z):
+        for layer in range(L):
+            k.qk_norm_rope_kv_rows(z["q"], st.args(layer), tree, None, None, first, offset, None, nq, N, T, 1e-6, 1e4)
+            k.attention_tree(z["o"], z["q"], st.args(layer), first, mask, None, 0, nq, N, T, z["w"])
+        k.kv_keep_rows(st.args(), first, path, count, N, T, L, st.plane)
+        k.beam_select(z["parent"], z["token"], z["score"], None, logits, V, V, score0, None, -1, B, B, M, z["w2"])
+        k.kv_reorder(st.args(), z["parent"], lo, hi, B, M, L, st.plane)
+        for layer in range(L):
+            k.qk_norm_rope_kv_rows(z["q1"], st.args(layer), token, None, None, first, None, None, nq, N, 1, 1e-6, 1e4)
+            k.attention_tree(z["o1"], z["q1"], st.args(layer), first, None, None, 0, nq, N, 1, z["w"])
+
+    def inputs(seed):
+        h = torch.Generator().manual_seed(seed)
+        for x in (tree, token, logits):
+            x.normal_(generator=g)
+        first.copy_(torch.randint(0, top - T, (N,), generator=h))
+        offset.copy_(torch.randint(0, T, (N, T), generator=h))
+        mask.copy_(words(tree_masks(h, N, T)))
+        path.copy_(torch.randint(0, T, (N, T), generator=h).sort(1).values)
+        count.copy_(torch.randint(0, T + 1, (N,), generator=h))
+        lo.copy_(torch.randint(0, 100, (M,), generator=h))
+        hi.copy_(torch.randint(0, top + 1, (M,), generator=h))
+        score0.copy_(-torch.rand((M, B), generator=h))
+
+    za, zb = buffers(), buffers()
+    inputs(0)
+    step(a, za)
+    step(b, zb)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(a, za)
+    for seed in range(1, 5):
+        inputs(seed)
+        graph.replay()
+        graph.replay()
+        for _ in range(2):
+            step(b, zb)
+        assert all(torch.equal(za[n], zb[n]) for n in ("q", "o", "q1", "o1", "parent", "token", "score"))
+        assert all(torch.equal(x, y) for x, y in zip(a.bits(), b.bits()))
+
+
 # ------------------------------------------------------------------------------------------------------------------ refusals of the tensors
 def test_refused_tensors(cuda):
     k = kernels()
